@@ -24,11 +24,14 @@ SAS_STATUS_BAD_BLOCK = 0x2
 SAS_STATUS_NO_PROGRESS = 0x4
 SAS_STATUS_WAIT_TIMEOUT = 0x8
 SAS_STATUS_BAD_TOKEN = 0x10
+SAS_STATUS_BAD_SCALE = 0x20
+SAS_STATUS_BAD_POSITION = 0x40
 
 SAS_NOALLOC_SCRATCH_BYTES = 16 << 20
 
 SAS_DTYPE_BF16 = 0
 SAS_DTYPE_FP16 = 1
+SAS_DTYPE_E4M3 = 2
 
 SAS_FWD_FLAG_CU_SEQLENS = 0x1
 SAS_FWD_FLAG_TEST_STALL = 0x100
@@ -51,6 +54,10 @@ EXPORTS = (
     "sas_split_metadata",
     "sas_read_status",
     "sas_set_kernel_events",
+    "sas_cache_append",
+    "sas_kvq_workspace_size",
+    "sas_kvq_forward",
+    "sas_kvq_read_status",
     "sas_metadata_workspace_size",
     "sas_metadata",
     "sas_strerror",
@@ -119,6 +126,53 @@ class SasMetaArgs(ctypes.Structure):
     ]
 
 
+class SasAppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32),
+        ("num_tokens", ctypes.c_int32),
+        ("num_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("rope_dim", ctypes.c_int32),
+        ("rope_interleaved", ctypes.c_int32),
+        ("rope_step", ctypes.c_int32),
+        ("rope_rows", ctypes.c_int32),
+        ("block_num", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("table_len", ctypes.c_int32),
+        ("max_q_len", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("cache_dtype", ctypes.c_int32),
+        ("kv_row_stride", ctypes.c_int64),
+        ("reserved", ctypes.c_int32 * 4),
+    ]
+
+
+class SasFp8Args(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32),
+        ("num_tokens", ctypes.c_int32),
+        ("max_q_len", ctypes.c_int32),
+        ("num_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("v_head_dim", ctypes.c_int32),
+        ("ori_block_num", ctypes.c_int32),
+        ("ori_block_size", ctypes.c_int32),
+        ("ori_table_len", ctypes.c_int32),
+        ("cmp_block_num", ctypes.c_int32),
+        ("cmp_block_size", ctypes.c_int32),
+        ("cmp_table_len", ctypes.c_int32),
+        ("topk", ctypes.c_int32),
+        ("cmp_ratio", ctypes.c_int32),
+        ("scenario", ctypes.c_int32),
+        ("ori_win_left", ctypes.c_int32),
+        ("ori_first", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("softmax_scale", ctypes.c_float),
+        ("kernel", ctypes.c_int32),
+        ("reserved", ctypes.c_int32 * 4),
+    ]
+
+
 _P = ctypes.c_void_p
 _SZ = ctypes.c_size_t
 
@@ -137,6 +191,10 @@ _SIGNATURES = {
     "sas_set_kernel_events": (ctypes.c_int, [_P, _P]),
     "sas_metadata_workspace_size": (ctypes.c_int, [ctypes.POINTER(SasMetaArgs), ctypes.POINTER(_SZ)]),
     "sas_metadata": (ctypes.c_int, [ctypes.POINTER(SasMetaArgs)] + [_P] * 5 + [_P, _SZ, _P]),
+    "sas_cache_append": (ctypes.c_int, [ctypes.POINTER(SasAppendArgs)] + [_P] * 12),
+    "sas_kvq_workspace_size": (ctypes.c_int, [ctypes.POINTER(SasFp8Args), ctypes.POINTER(_SZ)]),
+    "sas_kvq_forward": (ctypes.c_int, [ctypes.POINTER(SasFp8Args)] + [_P] * 14 + [_P, _SZ, _P]),
+    "sas_kvq_read_status": (ctypes.c_int, [ctypes.POINTER(SasFp8Args), _P, ctypes.POINTER(ctypes.c_uint32), _P]),
     "sas_strerror": (ctypes.c_char_p, [ctypes.c_int]),
     "sas_abi_version": (ctypes.c_int, []),
 }
@@ -188,6 +246,8 @@ def status_names(bits: int):
         ("no_progress", SAS_STATUS_NO_PROGRESS),
         ("wait_timeout", SAS_STATUS_WAIT_TIMEOUT),
         ("bad_token", SAS_STATUS_BAD_TOKEN),
+        ("bad_scale", SAS_STATUS_BAD_SCALE),
+        ("bad_position", SAS_STATUS_BAD_POSITION),
     ):
         if bits & bit:
             names.append(name)

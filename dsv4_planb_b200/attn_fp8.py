@@ -1,0 +1,211 @@
+"""Sparse shared-KV attention over an 8-bit paged cache.
+
+``sparse_attn_sharedkv_fp8`` is ``sparse_attn_sharedkv`` (same scenarios, layouts, index rules and
+results up to the cache's rounding) over ``float8_e4m3fn`` pools with one fp32 scale per block, which
+halves the cache and what a decode step reads.  ``ori_first`` keeps the first positions of a sequence
+visible next to the sliding window.  The reference has neither.
+"""
+
+from __future__ import annotations
+
+import functools
+from typing import Optional, Tuple, Union
+
+import torch
+
+from . import _lib
+from .api import _dense16, _dtype_code, _i32, _out_shapes, _pool16, _ptr, _scenario, _workspace
+from .cache import _eager, _no_grad, _on, _ops
+
+KERNELS = {"auto": 0, "simt": 1, "tc": 2}
+
+
+@functools.lru_cache(maxsize=512)
+def _call_args(*sizes) -> Tuple["_lib.SasFp8Args", int]:
+    """The call's sizes as the C struct, and the workspace they need (nothing of the tensors)."""
+    args = _lib.SasFp8Args(*sizes)
+    n = _lib.ctypes.c_size_t(0)
+    _lib.check(_lib.load().sas_kvq_workspace_size(args, n), "sas_kvq_workspace_size")
+    return args, n.value
+
+
+def _launch(q, ori_kv, ori_kv_scale, cmp_kv, cmp_kv_scale, cmp_sparse_indices, ori_block_table, cmp_block_table,
+            cu_seqlens_q, seqused_kv, sinks, softmax_scale, cmp_ratio, ori_win_left, ori_first, layout_q, v_head_dim,
+            kernel, check_status, out, lse):
+    dev = q.device
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _launch(q, ori_kv, ori_kv_scale, cmp_kv, cmp_kv_scale, cmp_sparse_indices, ori_block_table,
+                           cmp_block_table, cu_seqlens_q, seqused_kv, sinks, softmax_scale, cmp_ratio, ori_win_left,
+                           ori_first, layout_q, v_head_dim, kernel, check_status, out, lse)
+    scenario = _scenario(cmp_kv, cmp_sparse_indices)
+    N1, D = q.shape[-2], q.shape[-1]
+    act_q = None
+    if layout_q == "TND":
+        T, S = q.shape[0], 0
+        cu = _i32(cu_seqlens_q, dev)
+        B = cu.numel() - 1
+    else:
+        B, S = q.shape[0], q.shape[1]
+        T, cu = B * S, None
+        if cu_seqlens_q is not None:
+            lens = _i32(cu_seqlens_q, dev)
+            act_q = (lens[1:] - lens[:-1]).contiguous()
+    _pool16(ori_kv, "ori_kv")
+    ori_bt, seq = _i32(ori_block_table, dev), _i32(seqused_kv, dev)
+    cmp_bt = idx = None
+    cb = cs = ct = K = 0
+    if scenario >= 2:
+        _pool16(cmp_kv, "cmp_kv")
+        cmp_bt = _i32(cmp_block_table, dev)
+        cb, cs, ct = cmp_kv.shape[0], cmp_kv.shape[1], cmp_bt.shape[1]
+    if scenario == 3:
+        idx = _i32(cmp_sparse_indices, dev)
+        K = idx.shape[-1]
+    if sinks is not None:
+        sinks = sinks.to(device=dev, dtype=torch.float32).contiguous()
+    q = _dense16(q)
+    args, nbytes = _call_args(B, T, S, N1, D, v_head_dim, ori_kv.shape[0], ori_kv.shape[1], ori_bt.shape[1], cb, cs, ct,
+                              K, cmp_ratio, scenario, ori_win_left, ori_first, _dtype_code(q.dtype), softmax_scale,
+                              KERNELS[kernel])
+    ws = _workspace(nbytes, dev)
+    out_user = None
+    if out.data_ptr() % 16:  # a caller's out that starts inside a 16-byte vector
+        out_user, out = out, torch.empty_like(out)
+    lib = _lib.load()
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    rc = lib.sas_kvq_forward(args, q.data_ptr(), ori_kv.data_ptr(), ori_kv_scale.data_ptr(), ori_bt.data_ptr(),
+                             _ptr(cmp_kv), _ptr(cmp_kv_scale), _ptr(cmp_bt), _ptr(idx), _ptr(cu), _ptr(act_q),
+                             seq.data_ptr(), _ptr(sinks), out.data_ptr(), _ptr(lse), ws.data_ptr(), nbytes, stream)
+    if rc:
+        _lib.check(rc, "sas_kvq_forward")
+    if out_user is not None:
+        out_user.copy_(out)
+    if check_status:
+        st = _lib.ctypes.c_uint32(0)
+        _lib.check(lib.sas_kvq_read_status(args, ws.data_ptr(), st, stream), "sas_kvq_read_status")
+        if st.value:
+            raise RuntimeError(f"sas_kvq_forward device status: {_lib.status_names(st.value)}")
+
+
+_SCHEMA = ("(Tensor q, Tensor ori_kv, Tensor ori_kv_scale, Tensor? cmp_kv, Tensor? cmp_kv_scale, "
+           "Tensor? cmp_sparse_indices, Tensor ori_block_table, Tensor? cmp_block_table, Tensor? cu_seqlens_q, "
+           "Tensor seqused_kv, Tensor? sinks, float softmax_scale, int cmp_ratio, int ori_win_left, int ori_first, "
+           "str layout_q, int v_head_dim, str kernel, bool check_status, Tensor(a!) out, Tensor(b!)? lse) -> ()")
+_ops.define("sparse_attn_sharedkv_fp8" + _SCHEMA)
+_ops.impl("sparse_attn_sharedkv_fp8", _launch, "CUDA")
+
+
+@torch.library.register_fake("sas_b200::sparse_attn_sharedkv_fp8")
+def _fake(*args):
+    return None
+
+
+def _check_pool(name, pool, scale, D):
+    if pool.dtype != torch.float8_e4m3fn:
+        raise ValueError(f"{name} must be float8_e4m3fn (got {pool.dtype}); 16-bit pools go to sparse_attn_sharedkv")
+    if pool.dim() != 4 or pool.shape[2] != 1 or pool.shape[3] != D:
+        raise ValueError(f"{name} must be [blocks, block_size, 1, {D}] (got {tuple(pool.shape)})")
+    if scale is None or scale.dtype != torch.float32 or not scale.is_contiguous() or scale.numel() != pool.shape[0]:
+        raise ValueError(f"{name}_scale must be contiguous float32 with one entry per block of {name}")
+
+
+def sparse_attn_sharedkv_fp8(
+    q: torch.Tensor,
+    *,
+    ori_kv: torch.Tensor,
+    ori_kv_scale: torch.Tensor,
+    cmp_kv: Optional[torch.Tensor] = None,
+    cmp_kv_scale: Optional[torch.Tensor] = None,
+    cmp_sparse_indices: Optional[torch.Tensor] = None,
+    ori_block_table: torch.Tensor,
+    cmp_block_table: Optional[torch.Tensor] = None,
+    cu_seqlens_q: Optional[torch.Tensor] = None,
+    seqused_kv: torch.Tensor,
+    sinks: Optional[torch.Tensor] = None,
+    softmax_scale: float,
+    cmp_ratio: Optional[int] = None,
+    ori_win_left: int = 127,
+    ori_first: int = 0,
+    layout_q: str = "TND",
+    return_softmax_lse: bool = False,
+    v_head_dim: Optional[int] = None,
+    kernel: str = "auto",
+    out: Optional[torch.Tensor] = None,
+    lse_out: Optional[torch.Tensor] = None,
+    check_status: bool = False,
+) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """Attention over 8-bit pools: the keywords, scenarios and results of ``sparse_attn_sharedkv``.
+
+    ``ori_kv`` / ``cmp_kv`` are ``float8_e4m3fn`` ``[blocks, block_size, 1, D]`` and ``*_scale`` fp32
+    ``[blocks]`` or ``[blocks, 1]`` (in [2^-60, 2^60]; ``cache.sharedkv_cache_append`` writes both).  A key
+    row is code x scale of its block, and its first ``v_head_dim`` dims are its value.  A token at
+    position p sees the window [max(p - ``ori_win_left``, 0), p], the positions below ``ori_first`` that
+    lie before it, and the compressed rows that ``sparse_attn_sharedkv`` gives it.  ``sinks`` (``[N1]`` or None) adds
+    exp(sink) to the softmax's denominator.  Returns ``out`` in the type and layout of ``q`` (last dim
+    ``v_head_dim``) and with ``return_softmax_lse`` the natural-log LSE in fp32.
+
+    No host synchronisation (``check_status`` reads the status bits and raises); graph-capturable; no
+    backward pass.  ``kernel``: "tc" (tensor cores: D 512 or 576, ``v_head_dim`` 512, up to 128 heads, bf16
+    q), "simt" (every shape), "auto".
+    """
+    assert layout_q in ("TND", "BSND"), f"unsupported layout_q={layout_q!r}"
+    if kernel not in KERNELS:
+        raise ValueError(f"kernel must be one of {sorted(KERNELS)}")
+    if not q.is_cuda:
+        raise ValueError("q must be a CUDA tensor (sas_b200 has no CPU path)")
+    lead = 1 if layout_q == "TND" else 2
+    if q.dim() != lead + 2:
+        raise ValueError(f"q must be {'[T, N1, D]' if lead == 1 else '[B, S, N1, D]'} (got {tuple(q.shape)})")
+    _no_grad("sparse_attn_sharedkv_fp8", q, sinks)
+    dev = q.device
+    N1, D = q.shape[-2], q.shape[-1]
+    _on(dev, ori_kv=ori_kv, ori_kv_scale=ori_kv_scale, cmp_kv=cmp_kv, cmp_kv_scale=cmp_kv_scale, out=out,
+        lse_out=lse_out)
+    _check_pool("ori_kv", ori_kv, ori_kv_scale, D)
+    Dv = D if v_head_dim is None else int(v_head_dim)
+    if layout_q == "TND":
+        assert cu_seqlens_q is not None, "cu_seqlens_q is required for TND"
+        B, T = cu_seqlens_q.numel() - 1, q.shape[0]
+    else:
+        B, T = q.shape[0], q.shape[0] * q.shape[1]
+        if cu_seqlens_q is not None and cu_seqlens_q.numel() != B + 1:
+            raise ValueError(f"cu_seqlens_q must have {B + 1} entries (got {cu_seqlens_q.numel()})")
+    if ori_block_table.dim() != 2 or ori_block_table.shape[0] < B:
+        raise ValueError(f"ori_block_table must be [B>={B}, table_len] (got {tuple(ori_block_table.shape)})")
+    if seqused_kv.numel() < B:
+        raise ValueError(f"seqused_kv must have {B} entries (got {seqused_kv.numel()})")
+    if cmp_kv is not None:
+        assert cmp_ratio is not None, "cmp_ratio is required with cmp_kv"
+        _check_pool("cmp_kv", cmp_kv, cmp_kv_scale, D)
+        if cmp_block_table is None or cmp_block_table.dim() != 2 or cmp_block_table.shape[0] < B:
+            raise ValueError(f"cmp_block_table must be [B>={B}, table_len]")
+        if cmp_sparse_indices is not None:
+            if cmp_sparse_indices.dim() != lead + 2 or cmp_sparse_indices.shape[:lead] != q.shape[:lead] \
+                    or cmp_sparse_indices.shape[lead] != 1:
+                raise ValueError(f"cmp_sparse_indices must hold [1, K] per token (got {tuple(cmp_sparse_indices.shape)})")
+    elif cmp_sparse_indices is not None:
+        raise ValueError("cmp_sparse_indices goes with cmp_kv")
+    if sinks is not None and sinks.numel() != N1:
+        raise ValueError(f"sinks must have {N1} entries (got {sinks.numel()})")
+    if ori_win_left < 0 or ori_first < 0:
+        raise ValueError("ori_win_left and ori_first must be >= 0")
+    o_shape, l_shape = _out_shapes(q, layout_q, Dv)
+    if out is None:
+        out = torch.empty(o_shape, dtype=q.dtype, device=dev)
+    elif out.dtype != q.dtype or out.numel() != T * N1 * Dv or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous {q.dtype} of shape {o_shape}")
+    lse = lse_out
+    if lse is None:
+        lse = torch.empty(l_shape, dtype=torch.float32, device=dev) if return_softmax_lse else None
+    elif lse.dtype != torch.float32 or lse.numel() != T * N1 or not lse.is_contiguous():
+        raise ValueError(f"lse_out must be contiguous float32 of shape {l_shape}")
+    call = (q, ori_kv, ori_kv_scale, cmp_kv, cmp_kv_scale, cmp_sparse_indices, ori_block_table, cmp_block_table,
+            cu_seqlens_q, seqused_kv, sinks, float(softmax_scale), 4 if cmp_ratio is None else int(cmp_ratio),
+            int(ori_win_left), int(ori_first), layout_q, Dv, kernel, bool(check_status), out, lse)
+    if _eager(q):
+        _launch(*call)
+    else:
+        torch.ops.sas_b200.sparse_attn_sharedkv_fp8(*call)
+    out, lse = out.view(o_shape), lse.view(l_shape) if lse is not None else None
+    return (out, lse) if return_softmax_lse else out

@@ -1,0 +1,246 @@
+"""Writing the paged shared-KV cache that the attention operators read.
+
+``sharedkv_cache_append`` puts the new K = V rows of a batch at their positions in a paged pool (the
+full-resolution or the compressed one) and rotates the positional tail of each row on the way; given
+query heads it rotates those too, in the same launch.  A pool holds 16-bit rows (``bfloat16`` or
+``float16``, what ``sparse_attn_sharedkv`` reads) or ``float8_e4m3fn`` codes with one power-of-two scale
+per block (what ``sparse_attn_sharedkv_fp8`` reads).  The reference has no counterpart: its caches come
+filled.
+"""
+
+from __future__ import annotations
+
+import functools
+from typing import Optional
+
+import torch
+
+from . import _lib
+from .api import _dense16, _dtype_code, _i32, _pool16, _ptr
+
+_CACHE_DTYPES = {torch.bfloat16: _lib.SAS_DTYPE_BF16, torch.float16: _lib.SAS_DTYPE_FP16,
+                 torch.float8_e4m3fn: _lib.SAS_DTYPE_E4M3}
+
+
+def rope_table(positions: int, rope_dim: int, *, base: float = 10000.0, inv_freq: Optional[torch.Tensor] = None,
+               device="cuda") -> torch.Tensor:
+    """Angles of positions 0 .. ``positions`` - 1 as fp32 ``[positions, rope_dim]``: cos of the
+    ``rope_dim`` / 2 frequencies, then sin.  ``inv_freq`` (``[rope_dim / 2]``) replaces
+    ``base ** (-2 i / rope_dim)``.  Products and functions are taken in 64 bits: at position 2^17 an
+    angle in 32 bits is off by up to 2^-8."""
+    if rope_dim % 2:
+        raise ValueError(f"rope_dim must be even (got {rope_dim})")
+    if inv_freq is None:
+        inv_freq = base ** (-torch.arange(0, rope_dim, 2, dtype=torch.float64, device=device) / rope_dim)
+    if inv_freq.numel() != rope_dim // 2:
+        raise ValueError(f"inv_freq must have {rope_dim // 2} entries (got {inv_freq.numel()})")
+    ang = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * inv_freq.to(device, torch.float64)
+    return torch.cat([ang.cos(), ang.sin()], dim=1).to(torch.float32)
+
+
+def _on(dev, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} must be on {dev} (got {t.device})")
+
+
+def _no_grad(what, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError(f"{what} has no backward pass: call it under torch.no_grad() or detach its inputs")
+
+
+def _eager(t: torch.Tensor) -> bool:
+    """A plain tensor outside tracing: the launch needs no dispatcher (whose Python kernels cost
+    about 10 us a call); fake tensors and torch.compile take the registered op."""
+    return type(t) is torch.Tensor and not torch.compiler.is_compiling()
+
+
+def _rows2d(kv: torch.Tensor, T: int, D: int) -> torch.Tensor:
+    """``kv`` as T rows of D consecutive elements, 16-byte aligned; rows may be further apart (a slice
+    of a wider projection), anything else is copied."""
+    try:
+        v = kv.view(T, D)
+    except RuntimeError:
+        v = kv.reshape(T, D)
+    if v.stride(1) != 1 or (T > 1 and (v.stride(0) % 8 or v.stride(0) < D)) or v.data_ptr() % 16:
+        v = v.contiguous()
+        if v.data_ptr() % 16:
+            v = v.clone()
+    return v
+
+
+@functools.lru_cache(maxsize=512)
+def _append_args(*sizes) -> "_lib.SasAppendArgs":
+    """The call's sizes as the C struct (nothing of the tensors themselves)."""
+    return _lib.SasAppendArgs(*sizes)
+
+
+def _append(kv, cache, cache_scale, block_table, seqused_kv, cu_seqlens_q, rope_table, rope_interleaved, rope_step, q,
+            q_out, layout_q, check_status):
+    dev = cache.device
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _append_on(dev, kv, cache, cache_scale, block_table, seqused_kv, cu_seqlens_q, rope_table,
+                              rope_interleaved, rope_step, q, q_out, layout_q, check_status)
+    return _append_on(dev, kv, cache, cache_scale, block_table, seqused_kv, cu_seqlens_q, rope_table, rope_interleaved,
+                      rope_step, q, q_out, layout_q, check_status)
+
+
+def _append_on(dev, kv, cache, cache_scale, block_table, seqused_kv, cu_seqlens_q, rope_table, rope_interleaved,
+               rope_step, q, q_out, layout_q, check_status):
+    _pool16(cache, "cache")
+    if rope_table is not None and rope_table.data_ptr() % 16:
+        raise ValueError("rope_table must start on a 16-byte boundary")
+    D = cache.shape[3]
+    if layout_q == "TND":
+        T, S = kv.shape[0], 0
+        B = cu_seqlens_q.numel() - 1
+        cu, act_q = _i32(cu_seqlens_q, dev), None
+    else:
+        B, S = kv.shape[0], kv.shape[1]
+        T, cu, act_q = B * S, None, None
+        if cu_seqlens_q is not None:
+            lens = _i32(cu_seqlens_q, dev)
+            act_q = (lens[1:] - lens[:-1]).contiguous()
+    rows = _rows2d(kv, T, D)
+    table, seq = _i32(block_table, dev), _i32(seqused_kv, dev)
+    R = 0 if rope_table is None else rope_table.shape[1]
+    heads = 0
+    if q_out is not None:
+        heads = q_out.shape[-2]
+        at = q_out.data_ptr()
+        if at % 16:
+            raise ValueError("q_out must start on a 16-byte boundary")
+        if q is None:
+            q = q_out  # turned in place
+        else:
+            d = q.data_ptr() - at
+            n = q_out.numel() * q_out.element_size()
+            if -n < d < n and n and not (d == 0 and q.is_contiguous()):
+                raise ValueError("q_out must be q itself or share nothing with it")
+            q = _dense16(q)
+    args = _append_args(B, T, heads, D, R, int(rope_interleaved), rope_step, 0 if R == 0 else rope_table.shape[0],
+                        cache.shape[0], cache.shape[1], table.shape[1], S, _dtype_code(kv.dtype),
+                        _CACHE_DTYPES[cache.dtype], max(rows.stride(0), D) if T > 1 else D)
+    lib = _lib.load()
+    word = torch.zeros(1, dtype=torch.int32, device=dev) if check_status else None
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    rc = lib.sas_cache_append(args, rows.data_ptr(), _ptr(q if heads else None), _ptr(q_out), _ptr(rope_table),
+                              table.data_ptr(), _ptr(cu), _ptr(act_q), seq.data_ptr(), cache.data_ptr(),
+                              _ptr(cache_scale), _ptr(word), stream)
+    if rc:
+        _lib.check(rc, "sas_cache_append")
+    if check_status:
+        bits = int(word.item())
+        if bits:
+            raise RuntimeError(f"sas_cache_append device status: {_lib.status_names(bits)}")
+
+
+_ops = torch.library.Library("sas_b200", "FRAGMENT")
+_ops.define("sharedkv_cache_append(Tensor kv, Tensor(a!) cache, Tensor(b!)? cache_scale, Tensor block_table, "
+            "Tensor seqused_kv, Tensor? cu_seqlens_q, Tensor? rope_table, bool rope_interleaved, int rope_step, "
+            "Tensor? q, Tensor(c!)? q_out, str layout_q, bool check_status) -> ()")
+_ops.impl("sharedkv_cache_append", _append, "CUDA")
+
+
+@torch.library.register_fake("sas_b200::sharedkv_cache_append")
+def _append_fake(kv, cache, cache_scale, block_table, seqused_kv, cu_seqlens_q, rope_table, rope_interleaved, rope_step,
+                 q, q_out, layout_q, check_status):
+    return None
+
+
+def sharedkv_cache_append(
+    kv: torch.Tensor,
+    *,
+    cache: torch.Tensor,
+    cache_scale: Optional[torch.Tensor] = None,
+    block_table: torch.Tensor,
+    seqused_kv: torch.Tensor,
+    cu_seqlens_q: Optional[torch.Tensor] = None,
+    rope_table: Optional[torch.Tensor] = None,
+    rope_interleaved: bool = True,
+    rope_step: int = 1,
+    q: Optional[torch.Tensor] = None,
+    q_out: Optional[torch.Tensor] = None,
+    layout_q: str = "TND",
+    check_status: bool = False,
+) -> Optional[torch.Tensor]:
+    """Append the new K = V rows of a batch to a paged cache, rotated on the way.
+
+    ``kv`` ``[T, D]`` (or ``[T, 1, D]``; BSND: ``[B, S, D]`` or ``[B, S, 1, D]``), ``bfloat16`` or
+    ``float16``; rows may be strided.  ``cache`` ``[blocks, block_size, 1, D]`` in the type of ``kv`` or in
+    ``float8_e4m3fn``, then with ``cache_scale`` ``[blocks]`` or ``[blocks, 1]`` fp32: a code stands for
+    code x scale of its block.  ``block_table``, ``seqused_kv`` (lengths with the new rows counted in) and
+    ``cu_seqlens_q`` are the attention's: row s of a request's n new rows goes to position
+    ``seqused_kv - n + s``.  For the compressed pool pass its block table, the compressed lengths and the
+    cumulative counts of new compressed rows, with ``rope_step = cmp_ratio`` where a compressed row takes
+    the position of its first token.
+
+    ``rope_table`` (``rope_table()``; fp32 ``[positions, R]``) turns the last R dims: row p x ``rope_step``
+    for position p; ``rope_interleaved`` pairs dims (2 i, 2 i + 1), else (i, i + R / 2).  ``q`` (``[T, N1, D]``
+    or ``[B, S, N1, D]``) is turned by the same angles into ``q_out`` (new when None; ``q`` itself turns in
+    place), which is returned.
+
+    Writes rows of the call's tokens only: padding rows, unmapped blocks, negative positions and positions
+    past the table are skipped (``check_status`` synchronises and raises on the last two and on a block
+    without a valid scale).  In an 8-bit cache a block takes the smallest power-of-two scale that its rows
+    need when its first row arrives, and raises it when later rows need more; the rows already there are
+    then rounded to the new scale.  A block must receive rows of one request only per call.  No host
+    synchronisation; graph-capturable.  No backward pass.
+    """
+    assert layout_q in ("TND", "BSND"), f"unsupported layout_q={layout_q!r}"
+    if not cache.is_cuda:
+        raise ValueError("cache must be a CUDA tensor (sas_b200 has no CPU path)")
+    _no_grad("sharedkv_cache_append", kv, q, cache, cache_scale, rope_table)
+    dev = cache.device
+    _on(dev, kv=kv, cache_scale=cache_scale, rope_table=rope_table, q=q, q_out=q_out)
+    if kv.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"kv must be bfloat16 or float16 (got {kv.dtype})")
+    if cache.dim() != 4 or cache.shape[2] != 1:
+        raise ValueError(f"cache must be [blocks, block_size, 1, D] (got {tuple(cache.shape)})")
+    D = cache.shape[3]
+    lead = 1 if layout_q == "TND" else 2
+    if kv.dim() not in (lead + 1, lead + 2) or kv.shape[-1] != D or (kv.dim() == lead + 2 and kv.shape[lead] != 1):
+        raise ValueError(f"kv must hold one row of {D} per token in layout {layout_q} (got {tuple(kv.shape)})")
+    if cache.dtype == torch.float8_e4m3fn:
+        if cache_scale is None or cache_scale.dtype != torch.float32 or not cache_scale.is_contiguous() \
+                or cache_scale.numel() != cache.shape[0]:
+            raise ValueError("a float8_e4m3fn cache needs cache_scale: contiguous float32, one entry per block")
+    elif cache.dtype != kv.dtype:
+        raise ValueError(f"cache must be of the type of kv or float8_e4m3fn (got {cache.dtype})")
+    elif cache_scale is not None:
+        raise ValueError("cache_scale goes with a float8_e4m3fn cache only")
+    if layout_q == "TND":
+        assert cu_seqlens_q is not None, "cu_seqlens_q is required for TND"
+        B = cu_seqlens_q.numel() - 1
+    else:
+        B = kv.shape[0]
+        if cu_seqlens_q is not None and cu_seqlens_q.numel() != B + 1:
+            raise ValueError(f"cu_seqlens_q must have {B + 1} entries (got {cu_seqlens_q.numel()})")
+    if block_table.dim() != 2 or block_table.shape[0] < B or block_table.shape[1] < 1:
+        raise ValueError(f"block_table must be [B>={B}, table_len] (got {tuple(block_table.shape)})")
+    if seqused_kv.numel() < B:
+        raise ValueError(f"seqused_kv must have {B} entries (got {seqused_kv.numel()})")
+    if rope_step < 1:
+        raise ValueError("rope_step must be >= 1")
+    if rope_table is not None:
+        if rope_table.dtype != torch.float32 or rope_table.dim() != 2 or not rope_table.is_contiguous():
+            raise ValueError("rope_table must be a contiguous float32 [positions, rope_dim]")
+        if rope_table.shape[1] % 16 or not 0 < rope_table.shape[1] <= D:
+            raise ValueError(f"rope_dim must be a multiple of 16 up to {D} (got {rope_table.shape[1]})")
+    if q is not None:
+        if q.dtype != kv.dtype or q.dim() != lead + 2 or q.shape[:lead] != kv.shape[:lead] or q.shape[-1] != D:
+            raise ValueError(f"q must be of kv's type and hold [N1, {D}] per token (got {q.dtype} {tuple(q.shape)})")
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        elif q_out.shape != q.shape or q_out.dtype != q.dtype or not q_out.is_contiguous():
+            raise ValueError("q_out must be contiguous and of q's shape and type")
+    elif q_out is not None:
+        raise ValueError("q_out goes with q")
+    call = (kv, cache, cache_scale, block_table, seqused_kv, cu_seqlens_q, rope_table, bool(rope_interleaved),
+            int(rope_step), None if q_out is q else q, q_out, layout_q, bool(check_status))
+    if _eager(cache):
+        _append(*call)
+    else:
+        torch.ops.sas_b200.sharedkv_cache_append(*call)
+    return q_out

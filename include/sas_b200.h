@@ -41,7 +41,12 @@ enum {
 #define SAS_STATUS_WAIT_TIMEOUT 0x8u /* a bounded device-side wait gave up */
 #define SAS_STATUS_BAD_TOKEN 0x10u   /* q_prefix[b] + s fell outside [0, num_tokens) */
 
-typedef enum { SAS_DTYPE_BF16 = 0, SAS_DTYPE_FP16 = 1 } SasDtype;
+/* bits set by the calls on the 8-bit cache and by sas_cache_append only */
+#define SAS_STATUS_BAD_SCALE 0x20u    /* a block's scale outside [2^-60, 2^60] (zero, negative, infinite, NaN) */
+#define SAS_STATUS_BAD_POSITION 0x40u /* sas_cache_append: a position past the rope table; the row was skipped */
+
+/* SAS_DTYPE_E4M3 is a cache type only (sas_cache_append, sas_kvq_forward). */
+typedef enum { SAS_DTYPE_BF16 = 0, SAS_DTYPE_FP16 = 1, SAS_DTYPE_E4M3 = 2 } SasDtype;
 
 /*
  * Kernel choice for sas_forward (SasFwdArgs.kernel).  SAS_KERNEL_TC: tensor
@@ -294,6 +299,88 @@ int sas_forward_noalloc(const SasFwdArgs *args, const void *q, const void *ori_k
  * allocates nothing.  No counterpart in the reference.
  */
 int sas_noalloc_read_status(uint32_t *status, void *stream);
+
+/* ---- writing the cache -----------------------------------------------------
+ * sas_cache_append writes the new K = V rows of a batch into a paged cache (the
+ * full-resolution or the compressed one), at the positions sas_forward reads
+ * them from, with the rotation of the rows' last rope_dim dims applied on the
+ * way.  No counterpart in the reference, whose caches come filled.
+ *   kv           [T][kv_row_stride] dtype: head_dim elements of each row are read
+ *   q, q_out     [T][num_heads][head_dim] dtype, or NULL (num_heads 0): query heads,
+ *                rotated by the same angles; q_out may be q (then only the rotated
+ *                dims are written)
+ *   rope_table   [rope_rows][rope_dim] fp32: cos of the rope_dim / 2 angles, then sin
+ *   block_table  [B][table_len] int32
+ *   cu_seqlens_q [B + 1] int32, or NULL: then request b's rows start at b * max_q_len
+ *                and act_q_len [B] (NULL: max_q_len each) counts them
+ *   act_kv_len   [B] int32: the sequences' lengths with the new rows counted in, so
+ *                that row s of n lies at position act_kv_len - n + s
+ *   cache        [block_num][block_size][1][head_dim] cache_dtype (dtype, or e4m3)
+ *   cache_scale  [block_num] fp32, e4m3 only: a code stands for code * scale
+ *   status       a device word the call ORs SAS_STATUS_* bits into, or NULL
+ * Rows of no request, rows before position 0, rows of unmapped blocks and rows past
+ * the rope table are not written.  An e4m3 block whose first row is among the new
+ * rows takes the smallest power of two s with max |x| <= 448 s (s in [2^-60, 2^60]);
+ * any other block keeps its scale or raises it to that value, and the rows already
+ * in it are then rounded to the new scale.  Infinities saturate, NaN stays NaN, and
+ * neither raises a scale.  A block receives rows of one request per call.
+ * kv, q, q_out, cache and rope_table start on 16-byte boundaries.
+ */
+typedef struct SasAppendArgs {
+    int32_t batch, num_tokens;
+    int32_t num_heads;        /* of q; 0: no q */
+    int32_t head_dim;         /* a multiple of 16, at most 1024 */
+    int32_t rope_dim;         /* a multiple of 16, at most head_dim; 0: no rotation */
+    int32_t rope_interleaved; /* pairs (2 i, 2 i + 1), else (i, i + rope_dim / 2) */
+    int32_t rope_step;        /* angles of position p: table row rope_step * p */
+    int32_t rope_rows;
+    int32_t block_num, block_size, table_len;
+    int32_t max_q_len;        /* rows per request where cu_seqlens_q is NULL */
+    int32_t dtype, cache_dtype;
+    int64_t kv_row_stride;    /* elements, a multiple of 8 */
+    int32_t reserved[4];      /* must be 0 */
+} SasAppendArgs;
+
+int sas_cache_append(const SasAppendArgs *args, const void *kv, const void *q, void *q_out, const float *rope_table,
+                     const int32_t *block_table, const int32_t *cu_seqlens_q, const int32_t *act_q_len,
+                     const int32_t *act_kv_len, void *cache, float *cache_scale, uint32_t *status, void *stream);
+
+/* ---- attention over an 8-bit cache --------------------------------------------
+ * sas_kvq_forward is sas_forward's attention over e4m3 caches with one scale per
+ * block of tokens (a row is code * scale of its physical block), plus the first
+ * ori_first positions of a sequence, which stay visible when the window has moved
+ * past them.  Keys of a token at position p: positions [0, min(ori_first, left)),
+ * the window [left, p] with left = max(p - ori_win_left, 0), and the compressed rows
+ * of sas_forward (scenarios 2 and 3, same index rules).  sinks may be NULL (no sink).
+ * Unmapped blocks and blocks without a valid scale read as zero rows.  A token that
+ * sees no key gets out = 0 and lse = its sink (-inf without one); rows of no request
+ * get zeros in both.  lse may be NULL.  q and out in bf16 or fp16; the pools, q and
+ * out start on 16-byte boundaries; head_dim is a multiple of 16.
+ */
+typedef struct SasFp8Args {
+    int32_t batch, num_tokens;
+    int32_t max_q_len;      /* rows per request where cu_seqlens_q is NULL (batch * max_q_len == num_tokens) */
+    int32_t num_heads, head_dim, v_head_dim;
+    int32_t ori_block_num, ori_block_size, ori_table_len;
+    int32_t cmp_block_num, cmp_block_size, cmp_table_len;
+    int32_t topk, cmp_ratio, scenario, ori_win_left;
+    int32_t ori_first;      /* first positions that stay visible */
+    int32_t dtype;          /* of q and out */
+    float softmax_scale;
+    int32_t kernel;         /* SAS_KERNEL_AUTO, SAS_KERNEL_SIMT or SAS_KERNEL_TC */
+    int32_t reserved[4];    /* must be 0 */
+} SasFp8Args;
+
+int sas_kvq_workspace_size(const SasFp8Args *args, size_t *bytes);
+
+int sas_kvq_forward(const SasFp8Args *args, const void *q, const void *ori_kv, const float *ori_scale,
+                    const int32_t *ori_block_table, const void *cmp_kv, const float *cmp_scale,
+                    const int32_t *cmp_block_table, const int32_t *cmp_indices, const int32_t *cu_seqlens_q,
+                    const int32_t *act_q_len, const int32_t *act_kv_len, const float *sinks, void *out, float *lse,
+                    void *workspace, size_t workspace_bytes, void *stream);
+
+/* The SAS_STATUS_* bits of a sas_kvq_forward call on `workspace` with the same args.  Synchronises. */
+int sas_kvq_read_status(const SasFp8Args *args, void *workspace, uint32_t *status, void *stream);
 
 /* ---- metadata scheduler ----------------------------------------------------
  * Replaces sparse_attn_sharedkv_metadata (metadata.py:1018-1086, the Python
