@@ -44,10 +44,12 @@
 
 #include "sas_common.cuh"
 #include "sas_tc_ptx.cuh"
+#include "sas_tc_sync.cuh"
 
 namespace {
 
 using namespace sas_ptx;
+using namespace sas_tc;
 
 constexpr int kBK = 64;           // keys per tile
 constexpr int kKStages = 3;       // score CTA: K ring
@@ -67,7 +69,6 @@ constexpr int kMaxDv = 512;
 // 0, 99.58-99.87 % with 0.25 and 99.18-99.67 % with 8; on B200 the lazy threshold makes the c2
 // decode kernel ~15 % faster.  Both meet the north-star bars against the fp32 golden.
 constexpr float kTauLazy = 8.0f;
-constexpr uint64_t kTimeoutNs = 4000000000ull;
 
 // P message: bf16 P [128 heads][64 keys] (SW128 K-major) + per-head floats.
 constexpr int kPBytes = 128 * kBK * 2;  // 16 KiB
@@ -111,12 +112,6 @@ constexpr int kQFirstStages = 1;
 __device__ __forceinline__ int q_stages(int tiles, bool first) {
     return !first || tiles < kQRegMinTiles ? kQStages : kQFirstStages;
 }
-
-// Unit queue: the score CTA's producer warp 4 takes unit ids from a global counter (the next one
-// fetched while the current one runs) and publishes them to every role of both CTAs through a
-// kTq-entry ring; an entry is reused once all kTqReaders consumer warps have read it.
-constexpr int kTq = 8;
-constexpr uint32_t kTqReaders = 17;  // every warp of the cluster but the writer: 8 in the score CTA, 9 in the output CTA
 
 constexpr int kMaxPieces = 64;  // pieces per token in split KV
 constexpr int kTmemCols = 512;
@@ -218,113 +213,6 @@ __device__ __forceinline__ Item load_unit(const TcArgs &p, int u) {
     it.j0 = it.np > 1 ? piece * p.M : 0;
     it.j1 = it.np > 1 && piece < it.np - 1 ? it.j0 + p.M : it.ntiles;  // the last piece takes the rest
     return it;
-}
-
-// What the helpers below need of a kernel's shared header: its abort flag and its unit queue
-// (both kernels lay these out in their own header struct).
-struct Sync {
-    volatile int *abort;
-    uint32_t *status;
-    uint32_t peer_abort;  // shared::cluster address of the peer CTA's abort flag
-    uint64_t *tq_full, *tq_empty;
-    volatile int *tq;
-};
-
-__device__ __noinline__ void raise_abort(const Sync &s, uint32_t bits) {
-    sas::set_status(s.status, bits);
-    *s.abort = 1;
-    st_cluster_u32(s.peer_abort, 1u);
-}
-
-// Wait for the phase of parity `parity` of mbarrier `bar`; false on abort / timeout.
-__device__ __forceinline__ bool wait_bar(const Sync &s, uint32_t bar, uint32_t parity, bool cluster_scope = false) {
-    uint64_t t0 = 0;
-    for (uint32_t it = 0;; ++it) {
-        if (cluster_scope ? mbar_try_cluster(bar, parity) : mbar_try(bar, parity)) return true;
-        if ((it & 15u) == 15u) {
-            if (*s.abort) return false;
-            const uint64_t now = globaltimer();
-            if (t0 == 0) t0 = now;
-            else if (now - t0 > kTimeoutNs) {
-                raise_abort(s, SAS_STATUS_WAIT_TIMEOUT);
-                return false;
-            }
-        }
-    }
-}
-
-// Warp-uniform wait: every lane polls; if any lane gives up, all do.
-__device__ __forceinline__ bool wait_warp(const Sync &s, uint32_t bar, uint32_t parity, bool cluster_scope = false) {
-    return __all_sync(0xffffffffu, wait_bar(s, bar, parity, cluster_scope));
-}
-
-// Warp-uniform poll: true (for every lane, each having acquired the phase) once
-// any lane sees the phase complete.  Used on rs_req and o_full, whose next phase
-// needs an arrival this warp makes later (rs_done / o_empty), so a phase one
-// lane saw complete stays complete and the lanes that lagged acquire it on their
-// first test.  The bound only guards that argument; it never binds.
-__device__ __forceinline__ bool poll_warp(uint32_t bar, uint32_t parity) {
-    // test_wait never suspends: a try_wait on one barrier could sleep through the other's phase
-    const bool mine = mbar_test(bar, parity);
-    if (!__any_sync(0xffffffffu, mine)) return false;
-    if (!mine)
-        for (uint32_t i = 0; i < (1u << 16) && !mbar_test(bar, parity); ++i) {
-        }
-    return true;
-}
-
-// Unit queue.  Cluster c's first unit is c (every role takes it without the queue); later ones
-// come from the counter, offset by the cluster count, and pass through the queue: entry k >= 1
-// lives in slot (k - 1) % kTq.
-__device__ __forceinline__ int first_unit(const TcArgs &p) {
-    return (int)cluster_id_x() < p.U ? (int)cluster_id_x() : -1;
-}
-
-// Reader side (every warp of the cluster but the writer; warp-uniform): the k-th unit id of this
-// cluster, or -1 once the counter has passed the last unit.  False on abort / timeout.
-__device__ __forceinline__ bool tq_read(const TcArgs &p, const Sync &sy, uint32_t rank, uint32_t k, int &t) {
-    if (k == 0) {
-        t = first_unit(p);
-        return true;
-    }
-    const int s = (k - 1) % kTq;
-    if (!wait_warp(sy, smem_u32(&sy.tq_full[s]), ((k - 1) / kTq) & 1, true)) return false;
-    t = sy.tq[s];
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) {
-        const uint32_t e = smem_u32(&sy.tq_empty[s]);
-        if (rank == 0)
-            mbar_arrive(e);
-        else
-            mbar_arrive_remote(map_to_cta(e, 0));
-    }
-    return true;
-}
-
-// Writer side (score CTA, warp 4; warp-uniform).  `pend` (lane 0) holds the id taken while the
-// previous unit's last tiles were being gathered (-1: none yet, take one now); taking it only
-// then keeps a cluster from holding a unit it cannot start soon.
-__device__ __forceinline__ bool tq_publish(const TcArgs &p, const Sync &sy, uint32_t k, int &pend, int &t) {
-    if (k == 0) {
-        t = first_unit(p);
-        return true;
-    }
-    const int s = (k - 1) % kTq;
-    const int lane = threadIdx.x & 31;
-    if (k - 1 >= (uint32_t)kTq && !wait_warp(sy, smem_u32(&sy.tq_empty[s]), (((k - 1) / kTq) - 1) & 1))
-        return false;
-    int v = 0;
-    if (lane == 0) {
-        if (pend < 0) pend = (int)ncluster_x() + atomicAdd(p.counter, 1);
-        v = pend < p.U ? pend : -1;
-        pend = -1;
-        sy.tq[s] = v;
-        st_cluster_u32(map_to_cta(smem_u32((const void *)&sy.tq[s]), 1), (uint32_t)v);
-        mbar_arrive(smem_u32(&sy.tq_full[s]));
-        mbar_arrive_remote(map_to_cta(smem_u32(&sy.tq_full[s]), 1));
-    }
-    t = __shfl_sync(0xffffffffu, v, 0);
-    return true;
 }
 
 // Row lookup of key k of tile j of an item, split in two so that the global
@@ -1738,22 +1626,6 @@ __global__ void __launch_bounds__(1024) split_metadata_kernel(const int32_t *tin
         __syncthreads();
     }
     if (tid == 0) out[864] = base_s;
-}
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-    static EncodeTiledFn fn = [] {
-        void *ptr = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            return reinterpret_cast<EncodeTiledFn>(ptr);
-        return static_cast<EncodeTiledFn>(nullptr);
-    }();
-    return fn;
 }
 
 // Tensor map over a [rows, D] array with 128-byte swizzle and boxes of 64 columns x `box_rows` rows.
