@@ -82,8 +82,9 @@ def check(m, out, lse, tokens=None, where=None):
     whose 36 partial sums lose at most 2^-22 of the sum of magnitudes each: a score is off by
     d = 36 * 2^-22 * reach, with the softmax's exp (2^-21) and the log2-domain products of scores up to
     reach (3 * 2^-24 * reach).  Weights: off by a factor e^(2 d + 2^-20), rounded on the tensor cores to
-    two e4m3 terms (relative 2^-9, after a rounding to fp16, 2^-12; and 2^-18 of the largest weight where
-    the second term is subnormal).
+    two e4m3 terms: relative 2^-9, after a rounding to fp16, 2^-12; and half of e4m3's smallest step,
+    2^-10, where the second term is subnormal.  The weights' frame leaves the largest weight of a row at
+    2^5.75 or more (the running maximum lags by less than 2^3 of 2^8.75), so 2^-10 is 2^-15.75 of it.
     The sums of out lose 2^-22 per step of the running magnitude.  One rounding at the end."""
     where = m["where"] if where is None else where
     cmp_ = m["cmp"]
@@ -102,7 +103,7 @@ def check(m, out, lse, tokens=None, where=None):
         err = (lse[t].double() - l).abs()[finite]
         tol = (d + 2.0 ** -20 + 2.0 ** -22 * l.abs())[finite]
         assert (err <= tol).all(), (t, float((err - tol).max()), float(err.max()))
-        tol = HALF_STEP[m["src"]] * o.abs() + 2.0 ** -24 + spread * (2 * d + 2.0 ** -20 + 2.0 ** -9 + 2.0 ** -12 + 70 * 2.0 ** -22)[:, None] + 2.0 ** -18 * top
+        tol = HALF_STEP[m["src"]] * o.abs() + 2.0 ** -24 + spread * (2 * d + 2.0 ** -20 + 2.0 ** -9 + 2.0 ** -12 + 70 * 2.0 ** -22)[:, None] + 2.0 ** -15.75 * top
         err = (out[t].double() - o).abs()
         assert (err <= tol).all(), (t, float((err - tol).max()), float(err.max()))
 
