@@ -18,29 +18,34 @@
 // by role, because O alone (128 heads x 512 fp32) fills one SM's tensor memory:
 //
 //   CTA 0 ("score")                              CTA 1 ("output")
-//   TMEM: Q hi / lo of 512 dims (256 columns),   TMEM: O (128 x 512 fp32)
-//         S (2 x 128 columns); the Q of dims
-//         512 .. 575 lies in shared memory
-//   4 warps gather 128 key rows per tile (TMA    4 warps gather the first 512 bytes of the rows
-//           tile::gather4, 128-byte swizzle)
+//   TMEM: Q hi / lo (D_qk / 2 columns),          TMEM: O (128 x 512 fp32)
+//         S (2 x 96 columns)
+//   4 warps gather 96 key rows per tile          4 warps gather the first 512 bytes of the rows
+//           (cp.async into the MMA's swizzle)
 //   1 warp  S = Q K^T: 2 MMAs (hi, lo) of M 128, 1 warp  O += P V: 2 (hi, lo) per 32 keys and 128
-//           N 128, K 32 per 32 dims                      value dims; V is the N-major B operand, the
+//           N 96, K 32 per 32 dims                       value dims; V is the N-major B operand, the
 //                                                        same bytes in the same swizzle as K
-//   8 warps split Q; softmax (two threads per    8 warps rescale O where a maximum rose; epilogue
-//           head, 64 keys each); P and factors
-//           go to CTA 1 (st.async)
+//   8 warps split Q; softmax (thread = head;     8 warps rescale O where a maximum rose; epilogue
+//           warps 0-3 take the even tiles,
+//           4-7 the odd ones); P and factors
+//           go to CTA 1 by bulk copies
 //
-// Tiles hold 128 keys because an MMA of N 64 takes nearly as long as one of N 128 (58 and 70 cycles).
-// The ring of the gather holds slabs (128 rows x 128 dims), each released as soon as its MMAs have
-// read it.  The maximum follows a rise of more than 2^3 only (P <= 2^8.75, the e4m3 range): with 128
-// heads some maximum rises in nearly every tile, and a rescale of O (512 columns read and written)
-// takes longer than the tile's MMAs.  The largest weight is then at least 2^5.75, and the 2^-10 that a
-// weight can be off by where its lo is subnormal are 2^-15.75 of it.  The softmax reads S twice from TMEM in short loops: unrolled
-// over 64 keys it was bound by instruction fetch (3.7 times the cycles of the same code alone).
+// What the pieces measured on B200, each alone, and what follows from it:
+//   - An MMA of N 64 takes 58 cycles, as one of N 96; N 128 takes 70-83.  96 keys leave room in TMEM for
+//     all of Q beside two S.
+//   - TMA tile::gather4 takes 24 cycles for 4 x 128 bytes wherever the rows lie (37 GB/s per SM);
+//     16-byte cp.async reaches 56 bytes per cycle from L2 (110 GB/s), and the HBM's rate over all SMs.
+//   - st.async to the other SM moves 12 bytes per cycle and holds the issuing warps meanwhile; a tile's
+//     P is 24 KiB.  Bulk copies from a staging buffer run beside the next tile's softmax.
+//   - Unrolled over a whole tile the softmax was bound by instruction fetch (3.7 times the cycles of the
+//     same code alone): it reads S twice from TMEM in loops of 32 keys.
+//   - With 128 heads some maximum rises in most tiles.  It is followed only past 2^3 (P <= 2^8.75, the
+//     e4m3 range; the largest weight is then at least 2^5.75, and the 2^-10 that a weight can be off by
+//     where its lo is subnormal are 2^-15.75 of it), and O is rescaled 128 columns at a time, each as
+//     soon as the last tile's product of these columns is complete.
 //
-// Keys of a token: first positions, then the window, padded to a multiple of 4, then the compressed
-// rows, so that the four rows of one gather come from one pool.  Slots without a key carry weight 0
-// (log2 s = -inf); rows of unmapped blocks are gathered from one past the pool, which reads zeros.
+// Keys of a token: first positions, then the window, then the compressed rows.  Slots without a key
+// carry weight 0 (log2 s = -inf); they and rows of unmapped blocks are filled with zeros.
 //
 // Every wait is bounded (sas_tc_sync.cuh): a timeout sets SAS_STATUS_WAIT_TIMEOUT and every role falls
 // through to the teardown, which frees TMEM after a cluster barrier.
@@ -60,23 +65,28 @@ using namespace sas_ptx;
 using namespace sas_tc;
 using namespace sas_fp8;
 
-constexpr int kBK = 128;             // keys per tile
-constexpr int kUnit = kBK * 128;     // ring unit: 128 dims of a tile's rows, or 64 bf16 dims of 128 query rows
-constexpr int kKUnits = 12, kVUnits = 7, kPStages = 2;
-constexpr int kDv = 512, kVSlabs = kDv / 128, kQChunks = 8;
+constexpr int kBK = 96;              // keys per tile
+constexpr int kSlab = kBK * 128;     // 128 dims of a tile's rows
+constexpr int kStages = 3;
+constexpr int kDv = 512, kVSlabs = kDv / 128;
+constexpr int kVStage = kVSlabs * kSlab, kKStage = kVStage + kBK * 64;  // K: dims 512 .. 575 as 64-byte rows behind
+constexpr int kQChunk = 128 * 128, kQPerStage = 3;  // raw Q: 64 bf16 dims of 128 heads; chunks per stage of the K ring
 constexpr int kSoftWarps = 8, kMmaWarp = 8, kProdWarp0 = 9, kProdWarps = 4;
+constexpr int kRowsPerWarp = kBK / kProdWarps;
 constexpr int kThreads = 32 * (kProdWarp0 + kProdWarps);
 constexpr uint32_t kReaders = 2 * (kSoftWarps + 1 + kProdWarps) - 1;  // of the unit queue: every warp but its writer
-constexpr int kTmemCols = 512, kTmemS = 256;
-constexpr int kConsts = 8;           // ring of per-tile key constants; the gather is at most 5 tiles ahead
+constexpr int kTmemCols = 512, kTmemS = 320;
+// Ring of per-tile key constants.  Those of tile n are written once the stage of tile n - 1 is free: the
+// scores of tile n - 4 are complete, so those of n - 6 have been read for the last time.
+constexpr int kConsts = 6;
 constexpr float kTop = 8.75f;        // log2 of the largest P: 431, within e4m3's 448
 constexpr float kRise = 3.f;         // log2 of the rise of a maximum that is left to P
 constexpr int kMaxPieces = 64;
 
-// P message: per head 128 hi codes (a 128-byte row, SW128), then the lo codes the same way, then alpha
-// and the unit's final factor per head.
-constexpr int kMsgLo = 128 * 128, kMsgStats = 2 * kMsgLo, kMsgBytes = kMsgStats + 1024;
-constexpr uint32_t kMsgTx = 128 * (256 + 8);
+// P message: per head a 128-byte row (SW128) of 96 hi codes and the first 32 lo codes, then a 64-byte
+// row (SW64) of the other lo codes, then {alpha, the unit's final factor}.  The 32 heads of a warp are
+// contiguous in each part.
+constexpr int kMsgLo = 128 * 128, kMsgStats = kMsgLo + 128 * 64, kMsgBytes = kMsgStats + 1024;
 
 struct KeyConst {
     float s[kBK];   // scale; 0: a zero row or no key
@@ -85,35 +95,35 @@ struct KeyConst {
 };
 
 struct Hdr {
-    uint64_t full[kKUnits], empty[kKUnits], s_full[2], s_free[2], q_raw, q_full, p_empty[kPStages], c_full[kConsts];
-    uint64_t p_full[kPStages], o_full, o_empty, rs_req, rs_done, pv_done, fin_ready;
+    uint64_t full[kStages], empty[kStages], s_full[2], s_free[2], q_raw, q_full, c_full[kConsts];
+    uint64_t x_bar[4][2], m_bar[4][2], l_bar[4];  // of the two warps that share 32 heads
+    uint64_t p_full[2], p_empty[2], o_full, o_empty, event, rs_done[kVSlabs], pv_done[kVSlabs];
     uint64_t tq_full[kTq], tq_empty[kTq];
     volatile int tq[kTq];
     uint32_t tmem_base;
     volatile int abort;
-    int rs_stage;
-    float fin[128];       // per head: factor of O at the end of the unit
-    float pair[2][2][128];  // what the two threads of a head tell each other, two exchanges
+    volatile int event_code;  // output CTA: tile (>= 0) whose alpha the warps apply to O; -1: the unit's last product is issued
+    float fin[128];           // per head: factor of O at the end of the unit
+    float amax[2][128], m[2][128], l[2][2][128];
 };
-constexpr int kHdr = 4 * 1024;
-static_assert(sizeof(Hdr) <= kHdr && kVUnits <= kKUnits, "header");
+constexpr int kHdr = 6 * 1024;
+static_assert(sizeof(Hdr) <= kHdr, "header");
 constexpr int kConstOff = kHdr;
-constexpr int kQRope = kConstOff + kConsts * (int)sizeof(KeyConst);  // [128 rows][64 hi | 64 lo codes], SW128
-constexpr int kScoreRing = kQRope + 128 * 128;
-constexpr int kScoreSmem = kScoreRing + kKUnits * kUnit;
+constexpr int kScoreMsgs = (kConstOff + kConsts * (int)sizeof(KeyConst) + 1023) / 1024 * 1024;
+constexpr int kScoreRing = kScoreMsgs + 2 * kMsgBytes;
+constexpr int kScoreSmem = kScoreRing + kStages * kKStage;
 constexpr int kOutRing = kHdr;
-constexpr int kOutMsgs = kOutRing + kVUnits * kUnit;
-constexpr int kOutStage = kOutMsgs + kPStages * kMsgBytes;  // epilogue staging: 64 columns of 32 heads per warp
-constexpr int kWarpSlab = 32 * 128;
+constexpr int kOutMsgs = kOutRing + kStages * kVStage;
+constexpr int kOutStage = kOutMsgs + 2 * kMsgBytes;  // epilogue staging: 32 columns of 32 heads per warp
+constexpr int kWarpSlab = 32 * 64;
 constexpr int kOutSmem = kOutStage + kSoftWarps * kWarpSlab;
 constexpr int kSmemBytes = (kScoreSmem > kOutSmem ? kScoreSmem : kOutSmem) + 1024;  // + alignment slack
-static_assert(kQRope % 1024 == 0 && kScoreRing % 1024 == 0 && kOutRing % 1024 == 0 && kOutMsgs % 1024 == 0 &&
-              kMsgBytes % 1024 == 0 && kOutStage % 1024 == 0, "128B-swizzled tiles are 1 KiB aligned");
-static_assert(kSmemBytes <= 232448, "shared memory");
+static_assert(kScoreMsgs % 1024 == 0 && kScoreRing % 1024 == 0 && kKStage % 1024 == 0 && kOutRing % 1024 == 0 &&
+              kOutMsgs % 1024 == 0 && kMsgBytes % 1024 == 0 && kOutStage % 1024 == 0, "swizzled tiles are 1 KiB aligned");
+static_assert(kQPerStage * kQChunk <= kKStage && kSmemBytes <= 232448, "shared memory");
 
 struct TcArgs : Args {
     uint32_t *status;
-    int ori_rows, cmp_rows;  // rows of each pool: the index one past the end reads zeros
     int U, P, M;             // units; pieces per token, tiles per piece (P = 1: whole tokens)
     float *part_o, *part_s;
 };
@@ -139,11 +149,6 @@ __device__ __forceinline__ void mma8_ss(uint32_t d, uint64_t a, uint64_t b, uint
 __host__ __device__ constexpr uint32_t idesc_e4m3(uint32_t m, uint32_t n, uint32_t b_mn) {
     return (1u << 4) | (b_mn << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
-__device__ __forceinline__ void st_async_v2(uint32_t addr, uint32_t a, uint32_t b, uint32_t cluster_bar) {
-    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];" ::"r"(addr), "r"(a),
-                 "r"(b), "r"(cluster_bar)
-                 : "memory");
-}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
@@ -155,8 +160,8 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 
 struct Item {
     int32_t rec[TR_INTS];
-    int t, piece, np, n4, ntiles, j0, j1;  // tiles [j0, j1) of token t; slots below n4 belong to the window's pool
-    bool skip;                             // a piece past the token's last tile
+    int t, piece, np, ntiles, j0, j1;  // tiles [j0, j1) of token t
+    bool skip;                         // a piece past the token's last tile
 };
 
 __device__ __forceinline__ Item load_unit(const TcArgs &p, int u) {
@@ -171,8 +176,7 @@ __device__ __forceinline__ Item load_unit(const TcArgs &p, int u) {
     it.rec[TR_NORI] = a.w;
     it.rec[TR_NCMP] = b.x;
     it.rec[TR_VALID] = b.y;
-    it.n4 = (a.w + 3) & ~3;
-    it.ntiles = b.y && a.w + b.x > 0 ? (it.n4 + b.x + kBK - 1) / kBK : 0;
+    it.ntiles = b.y ? (a.w + b.x + kBK - 1) / kBK : 0;
     it.np = p.P > 1 && it.ntiles > p.M ? min((it.ntiles + p.M - 1) / p.M, p.P) : 1;
     it.skip = it.piece >= it.np;
     it.j0 = it.np > 1 ? it.piece * p.M : 0;
@@ -185,11 +189,10 @@ __device__ __forceinline__ Item load_unit(const TcArgs &p, int u) {
 __device__ __forceinline__ int32_t key_fetch(const TcArgs &p, const Item &it, int i) {
     const int32_t *table = p.ori_bt;
     int slot = i, bs = p.ori_bs, len = p.ori_table_len;
-    if (i < it.n4) {
-        if (i >= it.rec[TR_NORI]) return -1;
+    if (i < it.rec[TR_NORI]) {
         slot = ori_position(it.rec, i);
     } else {
-        slot = i - it.n4;
+        slot = i - it.rec[TR_NORI];
         if (slot >= it.rec[TR_NCMP]) return -1;
         if (p.scenario == 3) return __ldg(p.rows + (int64_t)it.t * p.K + slot);
         table = p.cmp_bt, bs = p.cmp_bs, len = p.cmp_table_len;
@@ -206,9 +209,9 @@ struct Key {
 
 __device__ __forceinline__ Key key_row(const TcArgs &p, const Item &it, int i, int32_t fetched, uint32_t &bits) {
     Key key{-1, 1.f, false};
-    const bool win = i < it.n4;
-    const int slot = win ? i : i - it.n4;
-    key.live = slot < (win ? it.rec[TR_NORI] : it.rec[TR_NCMP]);
+    const bool win = i < it.rec[TR_NORI];
+    const int slot = win ? i : i - it.rec[TR_NORI];
+    key.live = win || slot < it.rec[TR_NCMP];
     if (!key.live) return key;
     const int bs = win ? p.ori_bs : p.cmp_bs;
     int blk = fetched;
@@ -225,24 +228,31 @@ __device__ __forceinline__ Key key_row(const TcArgs &p, const Item &it, int i, i
     return key;
 }
 
-// The gather warps.  Each takes 32 of a tile's 128 key slots (a lane per slot) and copies its rows slab
-// by slab with TMA tile::gather4 (4 rows x 128 bytes): row r of a unit at r * 128, its 16-byte granules
-// permuted by r % 8, the MMA's 128-byte swizzle.  The slab behind D_qk 512 reads 64 bytes past the
-// row's end as zeros.  A unit's full barrier counts the four warps, each of which announces its own
-// 4 KiB first.  The warps share nothing else.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32_t bytes) {  // bytes 0: zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+// The gather warps.  Each takes 24 of a tile's 96 key slots (a lane per slot) and copies its rows with
+// 16-byte cp.async: an instruction moves 512 bytes of one row, 32 granules over the four slabs (row r of
+// a slab at r * 128, granule g at g ^ r % 8: the MMA's 128-byte swizzle); dims 512 .. 575 go to 64-byte
+// rows (granule g at g ^ r / 2 % 4: the 64-byte swizzle), 8 rows per instruction.  A stage's full
+// barrier counts the 128 threads; each arrives when its copies have landed.  The warps share nothing else.
 template <bool kScore>
-__device__ void producer(const TcArgs &p, const Sync &sy, const CUtensorMap *ori_map, const CUtensorMap *cmp_map,
-                         const CUtensorMap *q_map, uint8_t *ring, Hdr *hd, KeyConst *consts) {
-    constexpr uint32_t kUnits = kScore ? kKUnits : kVUnits;
-    const int w = (threadIdx.x >> 5) - kProdWarp0, lane = threadIdx.x & 31, key_at = w * 32 + lane;
-    const int slabs = kScore ? (p.Dq + 127) / 128 : kVSlabs;
+__device__ void producer(const TcArgs &p, const Sync &sy, const CUtensorMap *q_map, uint8_t *ring, Hdr *hd,
+                         KeyConst *consts) {
+    constexpr uint32_t kStageBytes = kScore ? kKStage : kVStage;
+    const int w = (threadIdx.x >> 5) - kProdWarp0, lane = threadIdx.x & 31;
+    const bool holds = lane < kRowsPerWarp;  // this lane looks a key up
+    const int key_at = w * kRowsPerWarp + (holds ? lane : 0);
     const bool writer = kScore && w == 0;
-    const uint32_t dst0 = smem_u32(ring) + w * 4096;
-    uint32_t at = 0, phase = 1, tiles = 0, bits = 0;  // unit of the ring, and the parity its empty barrier is waited on
+    const bool tail = kScore && p.Dq > 512;
+    const uint32_t ring_at = smem_u32(ring);
+    const uint32_t dst_lane = (lane >> 3) * kSlab + w * kRowsPerWarp * 128, gran = (lane & 7) << 4;
+    uint32_t st = 0, phase = 1, tiles = 0, bits = 0;  // stage, and the parity its empty barrier is waited on
     int pend = -1;
     auto next = [&] {
-        if (++at == kUnits) {
-            at = 0;
+        if (++st == kStages) {
+            st = 0;
             phase ^= 1;
         }
     };
@@ -258,31 +268,35 @@ __device__ void producer(const TcArgs &p, const Sync &sy, const CUtensorMap *ori
         int32_t fetched = i + kBK < end ? key_fetch(p, it, i + kBK) : -1;
         Key key = key_row(p, it, i, f0, bits);
         if constexpr (kScore) {
-            // raw Q of the token, 64 of its first 512 dims per unit: this warp's 32 head rows
-            for (int c = 0; c < kQChunks; ++c, next()) {
-                if (!wait_warp(sy, smem_u32(&hd->empty[at]), phase)) return;
-                if (lane == 0) {
-                    const uint32_t fb = smem_u32(&hd->full[at]);
-                    if (w * 32 < p.N1) {
-                        mbar_arrive_expect_tx(fb, 4096);
-                        tma_load_2d(dst0 + at * kUnit, q_map, c * 64, it.t * p.N1 + w * 32, fb);
-                    } else {
-                        mbar_arrive(fb);  // rows of no head: whatever lies there
-                    }
+            // raw Q of the token, three chunks of 64 dims per stage: this warp's 32 head rows, by TMA
+            const int chunks = p.Dq / 64;
+            for (int c = 0; c < chunks; c += kQPerStage, next()) {
+                if (!wait_warp(sy, smem_u32(&hd->empty[st]), phase)) return;
+                const uint32_t fb = smem_u32(&hd->full[st]);
+                if (lane == 0 && w * 32 < p.N1) {
+                    const int n = min(kQPerStage, chunks - c);
+                    mbar_arrive_expect_tx(fb, n * 4096);
+                    for (int e = 0; e < n; ++e)
+                        tma_load_2d(ring_at + st * kStageBytes + e * kQChunk + w * 4096, q_map, (c + e) * 64,
+                                    it.t * p.N1 + w * 32, fb);
+                } else {
+                    mbar_arrive(fb);  // rows of no head: whatever lies there
                 }
             }
         }
-        for (int j = it.j0; j < it.j1; ++j, i += kBK, ++tiles) {
+        for (int j = it.j0; j < it.j1; ++j, i += kBK, ++tiles, next()) {
             if (key.row >= 0 && !scale_ok(key.s)) {
                 bits |= SAS_STATUS_BAD_SCALE;
                 key.row = -1;
             }
             if constexpr (kScore) {
                 KeyConst &c = consts[tiles % kConsts];
-                const bool row = key.row >= 0;
-                c.s[key_at] = row ? key.s : 0.f;
-                c.ls[key_at] = row ? log2f(key.s) : key.live ? -60.f : -INFINITY;
-                c.r[key_at] = row ? 1.f / key.s : key.live ? kScaleMax : 0.f;
+                if (holds) {
+                    const bool row = key.row >= 0;
+                    c.s[key_at] = row ? key.s : 0.f;
+                    c.ls[key_at] = row ? log2f(key.s) : key.live ? -60.f : -INFINITY;
+                    c.r[key_at] = row ? 1.f / key.s : key.live ? kScaleMax : 0.f;
+                }
                 __syncwarp();
                 if (lane == 0) {
                     mbar_arrive(smem_u32(&hd->c_full[tiles % kConsts]));
@@ -290,31 +304,34 @@ __device__ void producer(const TcArgs &p, const Sync &sy, const CUtensorMap *ori
                         pend = (int)ncluster_x() + atomicAdd(p.counter, 1);
                 }
             }
-            // lane q < 8 copies the rows of lanes 4 q .. 4 q + 3
-            const bool win = j * kBK + w * 32 + (lane & 7) * 4 < it.n4;
-            const CUtensorMap *map = win ? ori_map : cmp_map;
-            const int32_t oob = win ? p.ori_rows : p.cmp_rows;
-            int32_t r[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int32_t v = __shfl_sync(0xffffffffu, key.row, (lane & 7) * 4 + e);
-                r[e] = v >= 0 ? v : oob;
+            if (!wait_warp(sy, smem_u32(&hd->empty[st]), phase)) return;
+            const uint32_t base = ring_at + st * kStageBytes;
+            const uint8_t *src = key.row < 0 ? nullptr
+                                             : (i < it.rec[TR_NORI] ? p.ori : p.cmp) + (int64_t)key.row * p.Dq;
+            const uint64_t src64 = reinterpret_cast<uint64_t>(src);
+#pragma unroll 8
+            for (int r = 0; r < kRowsPerWarp; ++r) {
+                const uint64_t a = __shfl_sync(0xffffffffu, src64, r);
+                cp_async16(base + dst_lane + r * 128 + (gran ^ ((r & 7) << 4)),
+                           reinterpret_cast<const uint8_t *>(a ? a : reinterpret_cast<uint64_t>(p.ori)) + lane * 16, a ? 16 : 0);
             }
-            const int32_t f = fetched;
-            for (int c = 0; c < slabs; ++c, next()) {
-                if (!wait_warp(sy, smem_u32(&hd->empty[at]), phase)) return;
-                const uint32_t fb = smem_u32(&hd->full[at]);
-                if (lane == 0) mbar_arrive_expect_tx(fb, 4096);
-                __syncwarp();
-                if (lane < 8) tma_gather4(dst0 + at * kUnit + lane * 512, map, c * 128, r[0], r[1], r[2], r[3], fb);
-                if (c == 0) {  // the next tile's lookups, behind the copies
-                    key = Key{-1, 1.f, false};
-                    if (i + kBK < end) key = key_row(p, it, i + kBK, f, bits);
-                    fetched = i + 2 * kBK < end ? key_fetch(p, it, i + 2 * kBK) : -1;
+            if (tail) {
+#pragma unroll
+                for (int r0 = 0; r0 < kRowsPerWarp; r0 += 8) {
+                    const int r = r0 + (lane >> 2), row = w * kRowsPerWarp + r;
+                    const uint64_t a = __shfl_sync(0xffffffffu, src64, r);
+                    cp_async16(base + kVStage + row * 64 + (((lane & 3) ^ ((row >> 1) & 3)) << 4),
+                               a ? reinterpret_cast<const uint8_t *>(a) + 512 + (lane & 3) * 16 : p.ori, a ? 16 : 0);
                 }
             }
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&hd->full[st])) : "memory");
+            key = Key{-1, 1.f, false};  // the next tile's lookups, behind the copies
+            if (i + kBK < end) key = key_row(p, it, i + kBK, fetched, bits);
+            fetched = i + 2 * kBK < end ? key_fetch(p, it, i + 2 * kBK) : -1;
         }
     }
+    // the copies' barriers are shared memory of this CTA: none may land after it has exited
+    asm volatile("cp.async.wait_all;" ::: "memory");
     if (bits) sas::set_status(p.status, bits);
 }
 
@@ -336,23 +353,7 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t 
     lo = l;
 }
 
-// What the other thread of a head says (x: what this one says).  Exchanges alternate between two
-// buffers, so one barrier of the two warps each is enough: a buffer is written again only past the
-// next exchange's barrier, which the partner reaches after it has read.
-__device__ __forceinline__ float exchange(float (*pair)[2][128], uint32_t &n, float x) {
-    const int g = threadIdx.x >> 7, h = threadIdx.x & 127;
-    float (*buf)[128] = pair[n++ & 1];
-    buf[g][h] = x;
-    asm volatile("bar.sync %0, 64;" ::"r"(1 + (h >> 5)) : "memory");
-    return buf[g ^ 1][h];
-}
-
-__device__ __forceinline__ void note_max(uint32_t v, float &amax, bool &odd) {
-    const float2 f = sas::DT<__nv_bfloat16>::to_f2(v);
-    amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
-    odd |= f.x - f.x != 0.f || f.y - f.y != 0.f;
-}
-
+// Four bf16 values times f into four hi and four lo codes.
 __device__ __forceinline__ void split4(uint32_t a, uint32_t b, float f, uint32_t &hi, uint32_t &lo) {
     const float2 x = sas::DT<__nv_bfloat16>::to_f2(a), y = sas::DT<__nv_bfloat16>::to_f2(b);
     uint32_t h0, l0, h1, l1;
@@ -362,43 +363,34 @@ __device__ __forceinline__ void split4(uint32_t a, uint32_t b, float f, uint32_t
     lo = l0 | (l1 << 16);
 }
 
-// Q of head row h into hi and lo codes.  Dims below 512, raw bf16 in TMEM columns [0, 256): chunk c of
-// 64 dims keeps its 32 columns, hi codes in the first 16 and lo codes in the last 16.  Dims 512 .. 575
-// (rope, this thread's 32 of them) go to shared memory.  The row's two threads take half each and
-// agree on the largest element.  Returns the row's power-of-two factor f (q f = hi + lo), NaN for a row
-// that holds an infinity or NaN.
-__device__ float split_q(uint32_t trow, int warp, int h, const uint4 *rope, uint32_t rope_row, float (*pair)[2][128],
-                         uint32_t &xc) {
-    const int g = warp >> 2;
-    uint32_t rp[16];
-    if (rope) {
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            const uint4 x = __ldg(rope + g * 4 + v);
-            rp[4 * v] = x.x, rp[4 * v + 1] = x.y, rp[4 * v + 2] = x.z, rp[4 * v + 3] = x.w;
-        }
-    }
-    float amax = 0.f;
-    bool odd = false;
+// Q of head row h, raw bf16 in TMEM columns [0, D_qk / 2), into hi and lo codes in place: chunk c of 64
+// dims keeps its 32 columns, hi codes in the first 16 and lo codes in the last 16.  The row's two
+// threads (warp and warp ^ 4) take every other chunk and agree on the largest element.  Returns the
+// row's power-of-two factor f (q f = hi + lo), NaN for a row that holds an infinity or NaN; false in
+// `ok` on abort.
+__device__ float split_q(const Sync &sy, Hdr *hd, uint32_t trow, int chunks, uint32_t parity, bool &ok) {
+    const int warp = threadIdx.x >> 5, g = warp >> 2, h = threadIdx.x & 127;
+    __nv_bfloat162 top = __floats2bfloat162_rn(0.f, 0.f);
 #pragma unroll 1
-    for (int c = 4 * g; c < 4 * g + 4; ++c) {
+    for (int c = g; c < chunks; c += 2) {
         uint32_t r[32];
         tmem_ld32(trow + c * 32, r);
         tc_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) note_max(r[i], amax, odd);
+        for (int i = 0; i < 32; ++i) top = __hmax2_nan(top, __habs2(*reinterpret_cast<__nv_bfloat162 *>(&r[i])));
     }
-    if (rope) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) note_max(rp[i], amax, odd);
-    }
-    if (odd) amax = INFINITY;
-    amax = fmaxf(amax, exchange(pair, xc, amax));
+    const float2 t2 = __bfloat1622float2(top);
+    float amax = t2.x + t2.y != t2.x + t2.y ? INFINITY : fmaxf(t2.x, t2.y);
+    hd->amax[g][h] = amax;
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&hd->x_bar[warp & 3][g]));
+    ok = wait_warp(sy, smem_u32(&hd->x_bar[warp & 3][g ^ 1]), parity);
+    amax = fmaxf(amax, hd->amax[g ^ 1][h]);
     // largest element to [128, 256); rows of zeros and of the smallest subnormals: f = 2^126
     const int e = (int)(__float_as_uint(amax) >> 23) - 127;
     const float f = amax == INFINITY ? NAN : __uint_as_float((uint32_t)(min(126, 7 - e) + 127) << 23);
 #pragma unroll 1
-    for (int c = 4 * g; c < 4 * g + 4; ++c) {
+    for (int c = g; c < chunks; c += 2) {
         uint32_t r[32], hi[16], lo[16];
         tmem_ld32(trow + c * 32, r);
         tc_wait_ld();
@@ -407,24 +399,51 @@ __device__ float split_q(uint32_t trow, int warp, int h, const uint4 *rope, uint
         tmem_st16(trow + c * 32, hi);
         tmem_st16(trow + c * 32 + 16, lo);
     }
-    if (rope) {
-        uint32_t hi[8], lo[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) split4(rp[2 * i], rp[2 * i + 1], f, hi[i], lo[i]);
-#pragma unroll
-        for (int v = 0; v < 2; ++v) {
-            st_shared_v4(rope_row + (((2 * g + v) ^ (h & 7)) << 4), hi[4 * v], hi[4 * v + 1], hi[4 * v + 2], hi[4 * v + 3]);
-            st_shared_v4(rope_row + (((4 + 2 * g + v) ^ (h & 7)) << 4), lo[4 * v], lo[4 * v + 1], lo[4 * v + 2], lo[4 * v + 3]);
-        }
-        fence_proxy_async_smem();
-    }
     tc_wait_st();
     return f;
 }
 
+// Two fp32 operations per instruction.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// Bulk copy of this CTA's shared memory to the cluster peer's, completing bytes on the peer's mbarrier.
+__device__ __forceinline__ void bulk_to_peer(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t cluster_bar) {
+    asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "r"(src), "r"(bytes), "r"(cluster_bar)
+                 : "memory");
+}
+
+// Shared-memory matrix descriptor, K-major rows of 64 bytes, 64-byte swizzle.
+__device__ __forceinline__ uint64_t sdesc_sw64(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)1 << 16 | (uint64_t)(512 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)4 << 61;
+}
+
 __global__ void __launch_bounds__(kThreads, 1)
-    fp8_tc_kernel(const TcArgs p, const __grid_constant__ CUtensorMap ori_map, const __grid_constant__ CUtensorMap cmp_map,
-                  const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap out_map) {
+    fp8_tc_kernel(const TcArgs p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap out_map) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
     Hdr *hd = reinterpret_cast<Hdr *>(smem);
@@ -435,28 +454,30 @@ __global__ void __launch_bounds__(kThreads, 1)
         auto init = [](uint64_t *b, int n, uint32_t count) {
             for (int i = 0; i < n; ++i) mbar_init(smem_u32(b + i), count);
         };
-        init(hd->full, kKUnits, kProdWarps);
-        init(hd->empty, kKUnits, 1);
+        init(hd->full, kStages, 32 * kProdWarps);
+        init(hd->empty, kStages, 1);
         init(hd->s_full, 2, 1);
-        init(hd->s_free, 2, kSoftWarps);
+        init(hd->s_free, 2, 4);
         init(&hd->q_raw, 1, 1);
         init(&hd->q_full, 1, kSoftWarps);
-        init(hd->p_empty, kPStages, 1);
         init(hd->c_full, kConsts, kProdWarps);
-        init(hd->p_full, kPStages, 1);
+        init(&hd->x_bar[0][0], 8, 1);
+        init(&hd->m_bar[0][0], 8, 1);
+        init(hd->l_bar, 4, 1);
+        init(hd->p_full, 2, 1);
+        init(hd->p_empty, 2, 1);
         init(&hd->o_full, 1, 1);
         init(&hd->o_empty, 1, kSoftWarps);
-        init(&hd->rs_req, 1, 1);
-        init(&hd->rs_done, 1, kSoftWarps);
-        init(&hd->pv_done, 1, 1);
-        init(&hd->fin_ready, 1, 1);
+        init(&hd->event, 1, 1);
+        init(hd->rs_done, kVSlabs, kSoftWarps);
+        init(hd->pv_done, kVSlabs, 1);
         init(hd->tq_full, kTq, 1);
         init(hd->tq_empty, kTq, kReaders);
         hd->abort = 0;
-        hd->rs_stage = 0;
-        // the output CTA expects the first message of each P stage (st.async complete_tx)
+        hd->event_code = 0;
+        // the output CTA expects the first message of each P slot (bulk copies complete it)
         if (rank == 1)
-            for (int i = 0; i < kPStages; ++i) mbar_arrive_expect_tx(smem_u32(&hd->p_full[i]), kMsgTx);
+            for (int i = 0; i < 2; ++i) mbar_arrive_expect_tx(smem_u32(&hd->p_full[i]), kMsgBytes);
         mbar_fence_init();
     }
     if (warp == kMmaWarp) {
@@ -479,14 +500,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint8_t *ring = smem + kScoreRing;
         KeyConst *consts = reinterpret_cast<KeyConst *>(smem + kConstOff);
         if (warp >= kProdWarp0) {
-            producer<true>(p, sy, &ori_map, &cmp_map, &q_map, ring, hd, consts);
+            producer<true>(p, sy, &q_map, ring, hd, consts);
         } else if (warp == kMmaWarp) {
             constexpr uint32_t idesc = idesc_e4m3(128, kBK, 0);
-            const int slabs = (p.Dq + 127) / 128;
-            uint32_t at = 0, phase = 0, sc = 0, qc = 0;
+            const int chunks = p.Dq / 64;
+            uint32_t st = 0, phase = 0, sc = 0, qc = 0;
             auto next = [&] {
-                if (++at == kKUnits) {
-                    at = 0;
+                if (++st == kStages) {
+                    st = 0;
                     phase ^= 1;
                 }
             };
@@ -498,58 +519,65 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (it.skip || it.j1 <= it.j0) continue;
                 // raw Q -> TMEM, once the previous unit's last product has read the old one
                 if (sc > 0 && !wait_warp(sy, smem_u32(&hd->s_full[(sc - 1) & 1]), ((sc - 1) >> 1) & 1)) goto done;
-                for (int c = 0; c < kQChunks; ++c, next()) {
-                    if (!wait_warp(sy, smem_u32(&hd->full[at]), phase)) goto done;
+                for (int c = 0; c < chunks; c += kQPerStage, next()) {
+                    if (!wait_warp(sy, smem_u32(&hd->full[st]), phase)) goto done;
                     tc_fence_after();
                     if (lane == 0) {
-                        const uint64_t d = sdesc_sw128(smem_u32(ring) + at * kUnit, 16, 1024);
-                        for (int kq = 0; kq < 4; ++kq) tmem_cp_128x256b(tmem + (c * 4 + kq) * 8, d + 2 * kq);
-                        tc_commit(smem_u32(&hd->empty[at]));
-                        if (c == kQChunks - 1) tc_commit(smem_u32(&hd->q_raw));
+                        for (int e = 0; e < kQPerStage && c + e < chunks; ++e) {
+                            const uint64_t d = sdesc_sw128(smem_u32(ring) + st * kKStage + e * kQChunk, 16, 1024);
+                            for (int kq = 0; kq < 4; ++kq) tmem_cp_128x256b(tmem + ((c + e) * 4 + kq) * 8, d + 2 * kq);
+                        }
+                        tc_commit(smem_u32(&hd->empty[st]));
+                        if (c + kQPerStage >= chunks) tc_commit(smem_u32(&hd->q_raw));
                     }
                     __syncwarp();
                 }
                 if (!wait_warp(sy, smem_u32(&hd->q_full), qc & 1)) goto done;
                 ++qc;
-                for (int j = it.j0; j < it.j1; ++j, ++sc) {
+                for (int j = it.j0; j < it.j1; ++j, ++sc, next()) {
                     const int sb = sc & 1;
                     const uint32_t d = tmem + kTmemS + sb * kBK;
                     if (!wait_warp(sy, smem_u32(&hd->s_free[sb]), ((sc >> 1) & 1) ^ 1)) goto done;
-                    for (int c = 0; c < slabs; ++c, next()) {
-                        if (!wait_warp(sy, smem_u32(&hd->full[at]), phase)) goto done;
-                        tc_fence_after();
-                        if (lane == 0) {
-                            const uint64_t b = sdesc_sw128(smem_u32(ring) + at * kUnit, 16, 1024);
-                            if (c < kQChunks / 2) {
+                    if (!wait_warp(sy, smem_u32(&hd->full[st]), phase)) goto done;
+                    tc_fence_after();
+                    fence_proxy_async_smem();  // the rows were written by cp.async
+                    if (lane == 0) {
+                        const uint32_t base = smem_u32(ring) + st * kKStage;
+#pragma unroll 1
+                        for (int c = 0; c < kVSlabs; ++c) {
+                            const uint64_t b = sdesc_sw128(base + c * kSlab, 16, 1024);
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    const uint32_t a = tmem + c * 64 + (i >> 1) * 32 + (i & 1) * 8;
-                                    mma8_ts(d, a, b + 2 * i, idesc, c + i > 0 ? 1u : 0u);
-                                    mma8_ts(d, a + 16, b + 2 * i, idesc, 1u);
-                                }
-                            } else {
-                                const uint64_t a = sdesc_sw128(smem_u32(smem + kQRope), 16, 1024);
-#pragma unroll
-                                for (int i = 0; i < 2; ++i) {
-                                    mma8_ss(d, a + 2 * i, b + 2 * i, idesc, 1u);
-                                    mma8_ss(d, a + 4 + 2 * i, b + 2 * i, idesc, 1u);
-                                }
+                            for (int i = 0; i < 4; ++i) {
+                                const uint32_t a = tmem + c * 64 + (i >> 1) * 32 + (i & 1) * 8;
+                                mma8_ts(d, a, b + 2 * i, idesc, c + i > 0 ? 1u : 0u);
+                                mma8_ts(d, a + 16, b + 2 * i, idesc, 1u);
                             }
-                            tc_commit(smem_u32(&hd->empty[at]));
-                            if (c == slabs - 1) tc_commit(smem_u32(&hd->s_full[sb]));
                         }
-                        __syncwarp();
+                        if (chunks > 8) {
+                            const uint64_t b = sdesc_sw64(base + kVStage);
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                mma8_ts(d, tmem + 256 + i * 8, b + 2 * i, idesc, 1u);
+                                mma8_ts(d, tmem + 256 + 16 + i * 8, b + 2 * i, idesc, 1u);
+                            }
+                        }
+                        tc_commit(smem_u32(&hd->empty[st]));
+                        tc_commit(smem_u32(&hd->s_full[sb]));
                     }
+                    __syncwarp();
                 }
             }
         } else {
-            const int g = warp >> 2, h = threadIdx.x & 127;  // head row, and which half of the keys
+            const int g = warp >> 2, h = threadIdx.x & 127;  // tile parity, head row
             const bool head = h < p.N1;
             const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-            const uint32_t msg0 = map_to_cta(smem_u32(smem + kOutMsgs), 1);
-            const uint32_t pfull0 = map_to_cta(smem_u32(&hd->p_full[0]), 1);
+            const uint32_t s_at = trow + kTmemS + g * kBK;
+            uint8_t *stage = smem + kScoreMsgs + g * kMsgBytes;
+            const uint32_t row1 = smem_u32(stage) + h * 128, row2 = smem_u32(stage) + kMsgLo + h * 64;
+            const uint32_t peer_msg = map_to_cta(smem_u32(smem + kOutMsgs), 1) + g * kMsgBytes;
+            const uint32_t peer_full = map_to_cta(smem_u32(&hd->p_full[g]), 1);
             const float sink = head && p.sinks ? p.sinks[h] : -INFINITY;
-            uint32_t sc = 0, qc = 0, xc = 0;
+            uint32_t sc0 = 0, qc = 0, lc = 0, mine = 0;  // the unit's first tile; units; units of two tiles or more; own tiles
             for (uint32_t k = 0;; ++k) {
                 int u;
                 if (!tq_read(p, sy, rank, k, u)) goto done;
@@ -560,73 +588,77 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (p.lse && head && g == 0) p.lse[(int64_t)it.t * p.N1 + h] = it.rec[TR_VALID] ? sink : 0.f;
                     continue;
                 }
+                const int nt = it.j1 - it.j0;
                 if (!wait_warp(sy, smem_u32(&hd->q_raw), qc & 1)) goto done;
-                ++qc;
                 tc_fence_after();
-                const uint4 *rope = reinterpret_cast<const uint4 *>(
-                    reinterpret_cast<const uint16_t *>(p.q) + ((int64_t)it.t * p.N1 + (head ? h : 0)) * p.Dq + 512);
-                const float rq = p.scale_log2 / split_q(trow, warp, h, p.Dq > 512 ? rope : nullptr,
-                                                        smem_u32(smem + kQRope) + h * 128, hd->pair, xc);
+                bool ok;
+                const float rq = p.scale_log2 / split_q(sy, hd, trow, p.Dq / 64, qc & 1, ok);
+                if (!ok) goto done;
+                ++qc;
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&hd->q_full));
-                float m = -INFINITY, l = 0.f;  // l: of this thread's keys
-                for (int j = it.j0; j < it.j1; ++j, ++sc) {
-                    const int sb = sc & 1;
+                const uint64_t rq2 = pack2(rq, rq);
+                float m = -INFINITY, l = 0.f;  // of this thread's tiles, l in the frame of m
+                for (int e = (sc0 & 1) == (uint32_t)g ? 0 : 1; e < nt; e += 2, ++mine) {
+                    const uint32_t sc = sc0 + e;
                     if (!wait_warp(sy, smem_u32(&hd->c_full[sc % kConsts]), (sc / kConsts) & 1)) goto done;
-                    if (!wait_warp(sy, smem_u32(&hd->s_full[sb]), (sc >> 1) & 1)) goto done;
+                    if (!wait_warp(sy, smem_u32(&hd->s_full[g]), mine & 1)) goto done;
                     tc_fence_after();
-                    const uint32_t s_at = trow + kTmemS + sb * kBK + g * 64;
                     const KeyConst &c = consts[sc % kConsts];
-                    float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll 1
-                    for (int i0 = 0; i0 < 64; i0 += 32) {
+                    for (int i0 = 0; i0 < kBK; i0 += 32) {
                         uint32_t sr[32];
                         tmem_ld32(s_at + i0, sr);
                         tc_wait_ld();
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
-                            const float4 s4 = *reinterpret_cast<const float4 *>(&c.s[g * 64 + i0 + i]);
-                            const float4 l4 = *reinterpret_cast<const float4 *>(&c.ls[g * 64 + i0 + i]);
-                            mx4[0] = fmaxf(mx4[0], fmaf(__uint_as_float(sr[i]) * rq, s4.x, l4.x));
-                            mx4[1] = fmaxf(mx4[1], fmaf(__uint_as_float(sr[i + 1]) * rq, s4.y, l4.y));
-                            mx4[2] = fmaxf(mx4[2], fmaf(__uint_as_float(sr[i + 2]) * rq, s4.z, l4.z));
-                            mx4[3] = fmaxf(mx4[3], fmaf(__uint_as_float(sr[i + 3]) * rq, s4.w, l4.w));
+                            const ulonglong2 s4 = *reinterpret_cast<const ulonglong2 *>(&c.s[i0 + i]);
+                            const ulonglong2 l4 = *reinterpret_cast<const ulonglong2 *>(&c.ls[i0 + i]);
+                            const float2 a = unpack2(fma2(mul2(pack2(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1])), rq2), s4.x, l4.x));
+                            const float2 b = unpack2(fma2(mul2(pack2(__uint_as_float(sr[i + 2]), __uint_as_float(sr[i + 3])), rq2), s4.y, l4.y));
+                            mx0 = fmaxf(mx0, fmaxf(a.x, a.y));
+                            mx1 = fmaxf(mx1, fmaxf(b.x, b.y));
                         }
                     }
-                    float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-                    mx = fmaxf(mx, exchange(hd->pair, xc, mx));
-                    float alpha = 1.f;
-                    if (j == it.j0) {
-                        m = mx;
-                    } else if (mx > m + kRise) {
-                        alpha = exp2f(m - mx);
-                        l *= alpha;
-                        m = mx;
+                    const float mx = fmaxf(mx0, mx1);
+                    // the maximum so far comes from the other warp's tile and goes on to its next
+                    float mn = mx, alpha = 1.f;
+                    if (sc > 0 && !wait_warp(sy, smem_u32(&hd->m_bar[warp & 3][g ^ 1]), ((sc - 1) >> 1) & 1)) goto done;
+                    if (e > 0) {
+                        const float before = hd->m[g ^ 1][h];
+                        mn = mx > before + kRise ? mx : before;
+                        if (mn != before) alpha = exp2f(before - mn);
+                    }
+                    hd->m[g][h] = mn;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&hd->m_bar[warp & 3][g]));
+                    if (mn != m) {
+                        l *= exp2f(m - mn);  // 0 before the first tile
+                        m = mn;
                     }
                     const float mb = m - (kTop - kRise);
-                    const int ps = sc % kPStages;
-                    if (!wait_warp(sy, smem_u32(&hd->p_empty[ps]), ((sc / kPStages) & 1) ^ 1, true)) goto done;
-                    const uint32_t msg = msg0 + ps * kMsgBytes, pbar = pfull0 + ps * 8, prow = msg + h * 128;
-                    float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+                    const uint64_t mb2 = pack2(-mb, -mb);
+                    // the slot was read by the peer, so its copies have left the staging buffer
+                    if (!wait_warp(sy, smem_u32(&hd->p_empty[g]), (mine & 1) ^ 1, true)) goto done;
+                    uint64_t sum0 = 0, sum1 = 0;
 #pragma unroll 1
-                    for (int i0 = 0; i0 < 64; i0 += 32) {
+                    for (int q = 0; q < kBK / 32; ++q) {
+                        const int i0 = q * 32;
                         uint32_t sr[32], hi[8], lo[8];
                         tmem_ld32(s_at + i0, sr);
                         tc_wait_ld();
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
-                            const float4 s4 = *reinterpret_cast<const float4 *>(&c.s[g * 64 + i0 + i]);
-                            const float4 l4 = *reinterpret_cast<const float4 *>(&c.ls[g * 64 + i0 + i]);
-                            const float4 r4 = *reinterpret_cast<const float4 *>(&c.r[g * 64 + i0 + i]);
-                            const float p0 = ex2_approx(fmaf(__uint_as_float(sr[i]) * rq, s4.x, l4.x) - mb);
-                            const float p1 = ex2_approx(fmaf(__uint_as_float(sr[i + 1]) * rq, s4.y, l4.y) - mb);
-                            const float p2 = ex2_approx(fmaf(__uint_as_float(sr[i + 2]) * rq, s4.z, l4.z) - mb);
-                            const float p3 = ex2_approx(fmaf(__uint_as_float(sr[i + 3]) * rq, s4.w, l4.w) - mb);
-                            sum4[0] = fmaf(p0, r4.x, sum4[0]);
-                            sum4[1] = fmaf(p1, r4.y, sum4[1]);
-                            sum4[2] = fmaf(p2, r4.z, sum4[2]);
-                            sum4[3] = fmaf(p3, r4.w, sum4[3]);
+                            const ulonglong2 s4 = *reinterpret_cast<const ulonglong2 *>(&c.s[i0 + i]);
+                            const ulonglong2 l4 = *reinterpret_cast<const ulonglong2 *>(&c.ls[i0 + i]);
+                            const ulonglong2 r4 = *reinterpret_cast<const ulonglong2 *>(&c.r[i0 + i]);
+                            const float2 a = unpack2(add2(fma2(mul2(pack2(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1])), rq2), s4.x, l4.x), mb2));
+                            const float2 b = unpack2(add2(fma2(mul2(pack2(__uint_as_float(sr[i + 2]), __uint_as_float(sr[i + 3])), rq2), s4.y, l4.y), mb2));
+                            const float p0 = ex2_approx(a.x), p1 = ex2_approx(a.y), p2 = ex2_approx(b.x), p3 = ex2_approx(b.y);
+                            sum0 = fma2(pack2(p0, p1), r4.x, sum0);
+                            sum1 = fma2(pack2(p2, p3), r4.y, sum1);
                             uint32_t h0, l0, h1, l1;
                             split2(p0, p1, h0, l0);
                             split2(p2, p3, h1, l1);
@@ -635,46 +667,64 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
 #pragma unroll
                         for (int v = 0; v < 2; ++v) {
-                            const uint32_t at = prow + (((g * 4 + (i0 >> 4) + v) ^ (h & 7)) << 4);
-                            st_async_v4(at, hi[4 * v], hi[4 * v + 1], hi[4 * v + 2], hi[4 * v + 3], pbar);
-                            st_async_v4(at + kMsgLo, lo[4 * v], lo[4 * v + 1], lo[4 * v + 2], lo[4 * v + 3], pbar);
+                            st_shared_v4(row1 + (((2 * q + v) ^ (h & 7)) << 4), hi[4 * v], hi[4 * v + 1], hi[4 * v + 2], hi[4 * v + 3]);
+                            const uint32_t at = q == 0 ? row1 + (((6 + v) ^ (h & 7)) << 4)
+                                                       : row2 + (((2 * q - 2 + v) ^ ((h >> 1) & 3)) << 4);
+                            st_shared_v4(at, lo[4 * v], lo[4 * v + 1], lo[4 * v + 2], lo[4 * v + 3]);
                         }
                     }
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&hd->s_free[sb]));
-                    l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+                    if (lane == 0) mbar_arrive(smem_u32(&hd->s_free[g]));
+                    const float2 s0 = unpack2(sum0), s1 = unpack2(sum1);
+                    l += (s0.x + s0.y) + (s1.x + s1.y);
                     float fin = 0.f;
-                    if (j == it.j1 - 1) {
-                        const float total = l + exchange(hd->pair, xc, l), own = mb + log2f(total);
+                    if (e == nt - 2) {  // the other warp ends the unit: it needs this one's sum, in the frame it ends with
+                        hd->l[lc & 1][0][h] = l;
+                        hd->l[lc & 1][1][h] = m;
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_u32(&hd->l_bar[warp & 3]));
+                    } else if (e == nt - 1) {
+                        float total = l;
+                        if (nt > 1) {
+                            if (!wait_warp(sy, smem_u32(&hd->l_bar[warp & 3]), lc & 1)) goto done;
+                            const float other = hd->l[lc & 1][0][h], frame = hd->l[lc & 1][1][h];
+                            total += frame == m ? other : other * exp2f(frame - m);
+                        }
+                        const float own = mb + log2f(total);
                         fin = 1.f / total;
                         if (it.np == 1) {
                             const float lse2 = log2_add(own, sink * 1.4426950408889634f);
                             fin *= exp2f(own - lse2);
-                            if (p.lse && head && g == 0) p.lse[(int64_t)it.t * p.N1 + h] = lse2 * 0.6931471805599453f;
-                        } else if (head && g == 0) {
+                            if (p.lse && head) p.lse[(int64_t)it.t * p.N1 + h] = lse2 * 0.6931471805599453f;
+                        } else if (head) {
                             p.part_s[((int64_t)it.t * p.P + it.piece) * p.N1 + h] = own;
                         }
                     }
-                    if (g == 0) st_async_v2(msg + kMsgStats + h * 8, __float_as_uint(head ? alpha : 1.f), __float_as_uint(fin), pbar);
+                    *reinterpret_cast<float2 *>(stage + kMsgStats + h * 8) = make_float2(head ? alpha : 1.f, fin);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        const uint32_t w32 = (warp & 3) * 32, src = smem_u32(stage);
+                        bulk_to_peer(peer_msg + w32 * 128, src + w32 * 128, 32 * 128, peer_full);
+                        bulk_to_peer(peer_msg + kMsgLo + w32 * 64, src + kMsgLo + w32 * 64, 32 * 64, peer_full);
+                        bulk_to_peer(peer_msg + kMsgStats + w32 * 8, src + kMsgStats + w32 * 8, 32 * 8, peer_full);
+                    }
                 }
+                sc0 += nt;
+                if (nt > 1) ++lc;
             }
-            // every P stage must be handed back before this CTA may exit
-            for (int s2 = 0; s2 < kPStages; ++s2) {
-                if ((int)sc > s2) {
-                    const uint32_t n = (sc - s2 + kPStages - 1) / kPStages;
-                    if (!wait_warp(sy, smem_u32(&hd->p_empty[s2]), (n - 1) & 1, true)) goto done;
-                }
-            }
+            // the last message must have been read before this CTA may exit
+            if (mine > 0 && !wait_warp(sy, smem_u32(&hd->p_empty[g]), (mine - 1) & 1, true)) goto done;
         }
     } else {
         // ======================= output CTA =======================
         uint8_t *ring = smem + kOutRing, *msgs = smem + kOutMsgs;
         if (warp >= kProdWarp0) {
-            producer<false>(p, sy, &ori_map, &cmp_map, nullptr, ring, hd, nullptr);
+            producer<false>(p, sy, nullptr, ring, hd, nullptr);
         } else if (warp == kMmaWarp) {
             constexpr uint32_t idesc = idesc_e4m3(128, 128, 1);
-            uint32_t at = 0, phase = 0, pc = 0, oc = 0, pvc = 0, rsc = 0;
+            uint32_t st = 0, phase = 0, pc = 0, oc = 0, rsc = 0;
             for (uint32_t k = 0;; ++k) {
                 int u;
                 if (!tq_read(p, sy, rank, k, u)) goto done;
@@ -684,68 +734,69 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!wait_warp(sy, smem_u32(&hd->o_empty), (oc & 1) ^ 1)) goto done;
                 ++oc;
                 for (int j = it.j0; j < it.j1; ++j, ++pc) {
-                    const int ps = pc % kPStages;
-                    if (!wait_warp(sy, smem_u32(&hd->p_full[ps]), (pc / kPStages) & 1, true)) goto done;
-                    if (lane == 0) mbar_arrive_expect_tx(smem_u32(&hd->p_full[ps]), kMsgTx);  // the next message
+                    const int ps = pc & 1;
+                    if (!wait_warp(sy, smem_u32(&hd->p_full[ps]), (pc >> 1) & 1, true)) goto done;
+                    if (lane == 0) mbar_arrive_expect_tx(smem_u32(&hd->p_full[ps]), kMsgBytes);  // the next message
                     const uint8_t *msg = msgs + ps * kMsgBytes;
                     const float2 *stat = reinterpret_cast<const float2 *>(msg + kMsgStats);
-                    bool need = false;
-                    for (int i = lane; i < 128; i += 32) need |= stat[i].x != 1.f;
-                    if (__any_sync(0xffffffffu, need) && j > it.j0) {
-                        // every PV product so far, then warps 0-7 scale the rows
-                        if (lane == 0) tc_commit(smem_u32(&hd->pv_done));
-                        __syncwarp();
-                        if (!wait_warp(sy, smem_u32(&hd->pv_done), pvc & 1)) goto done;
-                        ++pvc;
-                        if (lane == 0) {
-                            hd->rs_stage = ps;
-                            mbar_arrive(smem_u32(&hd->rs_req));
-                        }
-                        __syncwarp();
-                        if (!wait_warp(sy, smem_u32(&hd->rs_done), rsc & 1)) goto done;
-                        ++rsc;
-                    }
                     const bool last = j == it.j1 - 1;
-                    if (last) {
-                        for (int i = lane; i < 128; i += 32) hd->fin[i] = stat[i].y;
-                        __syncwarp();
-                        if (lane == 0) {
-                            __threadfence_block();
-                            mbar_arrive(smem_u32(&hd->fin_ready));
-                        }
+                    bool rescale = false;
+                    if (j > it.j0) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) rescale |= stat[lane + 32 * i].x != 1.f;
+                        rescale = __any_sync(0xffffffffu, rescale);
                     }
-                    fence_proxy_async_smem();
-                    const uint64_t a = sdesc_sw128(smem_u32(msg), 16, 1024);
+                    if (rescale) {  // warps 0-7 scale the rows, slab by slab
+                        if (lane == 0) {
+                            hd->event_code = (int)(pc & 0x7fffffff);
+                            mbar_arrive(smem_u32(&hd->event));
+                        }
+                        __syncwarp();
+                    }
+                    if (last)
+                        for (int i = lane; i < 128; i += 32) hd->fin[i] = stat[i].y;
+                    if (!wait_warp(sy, smem_u32(&hd->full[st]), phase)) goto done;
+                    fence_proxy_async_smem();  // the rows were written by cp.async
+                    const uint64_t a1 = sdesc_sw128(smem_u32(msg), 16, 1024), a2 = sdesc_sw64(smem_u32(msg) + kMsgLo);
+                    const uint32_t base = smem_u32(ring) + st * kVStage;
+#pragma unroll 1
                     for (int c = 0; c < kVSlabs; ++c) {
-                        if (!wait_warp(sy, smem_u32(&hd->full[at]), phase)) goto done;
+                        if (rescale && !wait_warp(sy, smem_u32(&hd->rs_done[c]), rsc & 1)) goto done;
                         tc_fence_after();
                         if (lane == 0) {
-                            const uint64_t b = sdesc_sw128(smem_u32(ring) + at * kUnit, kUnit, 1024);
+                            const uint64_t b = sdesc_sw128(base + c * kSlab, kSlab, 1024);
                             const uint32_t d = tmem + c * 128;
 #pragma unroll
                             for (int i = 0; i < kBK / 32; ++i) {
-                                mma8_ss(d, a + 2 * i, b + 256 * i, idesc, (j > it.j0 || i > 0) ? 1u : 0u);
-                                mma8_ss(d, a + kMsgLo / 16 + 2 * i, b + 256 * i, idesc, 1u);
+                                mma8_ss(d, a1 + 2 * i, b + 256 * i, idesc, (j > it.j0 || i > 0) ? 1u : 0u);
+                                mma8_ss(d, i == 0 ? a1 + 6 : a2 + 2 * (i - 1), b + 256 * i, idesc, 1u);
                             }
-                            tc_commit(smem_u32(&hd->empty[at]));
-                            if (c == kVSlabs - 1) {
-                                tc_commit_mc(smem_u32(&hd->p_empty[ps]), (uint16_t)1);
-                                if (last) tc_commit(smem_u32(&hd->o_full));
-                            }
+                            tc_commit(smem_u32(&hd->pv_done[c]));
                         }
                         __syncwarp();
-                        if (++at == kVUnits) {
-                            at = 0;
-                            phase ^= 1;
+                    }
+                    if (rescale) ++rsc;
+                    if (lane == 0) {
+                        tc_commit(smem_u32(&hd->empty[st]));
+                        tc_commit_mc(smem_u32(&hd->p_empty[ps]), (uint16_t)1);
+                        if (last) {
+                            tc_commit(smem_u32(&hd->o_full));
+                            hd->event_code = -1;
+                            mbar_arrive(smem_u32(&hd->event));
                         }
+                    }
+                    __syncwarp();
+                    if (++st == kStages) {
+                        st = 0;
+                        phase ^= 1;
                     }
                 }
             }
         } else {
-            const int g = warp >> 2, h = threadIdx.x & 127;  // head row, and which half of the columns
+            const int g = warp >> 2, h = threadIdx.x & 127;  // which half of the columns, head row
             const bool head = h < p.N1;
-            const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16) + g * (kDv / 2);
-            uint32_t ofc = 0, rsc = 0, frc = 0;
+            const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+            uint32_t ofc = 0, ev = 0;
             for (uint32_t k = 0;; ++k) {
                 int u;
                 if (!tq_read(p, sy, rank, k, u)) goto done;
@@ -759,81 +810,67 @@ __global__ void __launch_bounds__(kThreads, 1)
                         for (int d = 0; d < kDv / 2; d += 8) *reinterpret_cast<uint4 *>(orow + d) = make_uint4(0, 0, 0, 0);
                     continue;
                 }
-                // serve rescale requests until the unit's O is complete
-                uint64_t t0 = 0;
-                for (uint32_t spin = 0;; ++spin) {
-                    if (poll_warp(smem_u32(&hd->rs_req), rsc & 1)) {
-                        ++rsc;
-                        tc_fence_after();
-                        const float a = reinterpret_cast<const float2 *>(msgs + hd->rs_stage * kMsgBytes + kMsgStats)[h].x;
-                        if (__any_sync(0xffffffffu, a != 1.f)) {
-                            // two 32-column loads in flight per wait: TMEM latency bounds the loop
+                for (;;) {  // rescale requests, until the unit's last product is issued
+                    if (!wait_warp(sy, smem_u32(&hd->event), ev & 1)) goto done;
+                    ++ev;
+                    const int pc = hd->event_code;
+                    if (pc < 0) break;
+                    const float a = reinterpret_cast<const float2 *>(msgs + (pc & 1) * kMsgBytes + kMsgStats)[h].x;
+                    const bool any = __any_sync(0xffffffffu, a != 1.f);
 #pragma unroll 1
-                            for (int c = 0; c < kDv / 2; c += 64) {
-                                uint32_t r0[32], r1[32];
-                                tmem_ld32(trow + c, r0);
-                                tmem_ld32(trow + c + 32, r1);
-                                tc_wait_ld();
+                    for (int c = 0; c < kVSlabs; ++c) {
+                        // the product of the tile before, of these columns
+                        if (!wait_warp(sy, smem_u32(&hd->pv_done[c]), (pc - 1) & 1)) goto done;
+                        if (any) {
+                            tc_fence_after();
+                            const uint32_t at = trow + c * 128 + g * 64;
+                            uint32_t r0[32], r1[32];
+                            tmem_ld32(at, r0);
+                            tmem_ld32(at + 32, r1);
+                            tc_wait_ld();
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) {
-                                    r0[i] = __float_as_uint(__uint_as_float(r0[i]) * a);
-                                    r1[i] = __float_as_uint(__uint_as_float(r1[i]) * a);
-                                }
-                                tmem_st32(trow + c, r0);
-                                tmem_st32(trow + c + 32, r1);
+                            for (int i = 0; i < 32; ++i) {
+                                r0[i] = __float_as_uint(__uint_as_float(r0[i]) * a);
+                                r1[i] = __float_as_uint(__uint_as_float(r1[i]) * a);
                             }
+                            tmem_st32(at, r0);
+                            tmem_st32(at + 32, r1);
                             tc_wait_st();
+                            tc_fence_before();
                         }
-                        tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(smem_u32(&hd->rs_done));
-                        t0 = 0;
-                        continue;
-                    }
-                    if (poll_warp(smem_u32(&hd->o_full), ofc & 1)) break;
-                    if ((spin & 15u) == 15u) {
-                        if (hd->abort) goto done;
-                        const uint64_t now = globaltimer();
-                        if (t0 == 0) t0 = now;
-                        else if (now - t0 > kTimeoutNs) {
-                            raise_abort(sy, SAS_STATUS_WAIT_TIMEOUT);
-                            goto done;
-                        }
+                        if (lane == 0) mbar_arrive(smem_u32(&hd->rs_done[c]));
                     }
                 }
+                if (!wait_warp(sy, smem_u32(&hd->o_full), ofc & 1)) goto done;
                 ++ofc;
-                if (!wait_warp(sy, smem_u32(&hd->fin_ready), frc & 1)) goto done;
-                ++frc;
                 tc_fence_after();
                 const float fin = hd->fin[h];
+                const uint32_t tcol = trow + g * (kDv / 2);
                 if (it.np == 1 && p.N1 % 32 == 0) {
-                    // 64 columns at a time: each warp stages its 32 head rows (128-byte swizzled) and writes
-                    // them with one TMA store
+                    // 32 columns at a time: each warp stages its 32 head rows (64-byte swizzle) and writes them
+                    // with one TMA store
                     if ((warp & 3) * 32 < p.N1) {
                         const uint32_t buf = smem_u32(smem + kOutStage) + warp * kWarpSlab;
 #pragma unroll 1
-                        for (int sl = 0; sl < kDv / 2 / 64; ++sl) {
-                            uint32_t r0[32], r1[32];
-                            tmem_ld32(trow + sl * 64, r0);
-                            tmem_ld32(trow + sl * 64 + 32, r1);
+                        for (int c = 0; c < kDv / 2; c += 32) {
+                            uint32_t r[32];
+                            tmem_ld32(tcol + c, r);
                             if (lane == 0) bulk_wait_read<0>();  // the last store has read buf
                             __syncwarp();
                             tc_wait_ld();
 #pragma unroll
-                            for (int cc = 0; cc < 8; ++cc) {
+                            for (int cc = 0; cc < 4; ++cc) {
                                 uint32_t w[4];
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    const int i = 8 * (cc & 3) + 2 * e;
-                                    w[e] = pack_bf16(__uint_as_float(cc < 4 ? r0[i] : r1[i]) * fin,
-                                                     __uint_as_float(cc < 4 ? r0[i + 1] : r1[i + 1]) * fin);
-                                }
-                                st_shared_v4(buf + lane * 128 + ((cc ^ (lane & 7)) << 4), w[0], w[1], w[2], w[3]);
+                                for (int e = 0; e < 4; ++e)
+                                    w[e] = pack_bf16(__uint_as_float(r[8 * cc + 2 * e]) * fin, __uint_as_float(r[8 * cc + 2 * e + 1]) * fin);
+                                st_shared_v4(buf + lane * 64 + ((cc ^ ((lane >> 1) & 3)) << 4), w[0], w[1], w[2], w[3]);
                             }
                             fence_proxy_async_smem();
                             __syncwarp();
                             if (lane == 0) {
-                                tma_store_2d(&out_map, buf, g * (kDv / 2) + sl * 64, it.t * p.N1 + (warp & 3) * 32);
+                                tma_store_2d(&out_map, buf, g * (kDv / 2) + c, it.t * p.N1 + (warp & 3) * 32);
                                 bulk_commit();
                             }
                         }
@@ -844,7 +881,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
                     for (int c = 0; c < kDv / 2; c += 32) {
                         uint32_t r[32];
-                        tmem_ld32(trow + c, r);
+                        tmem_ld32(tcol + c, r);
                         tc_wait_ld();
                         float x[32];
 #pragma unroll
@@ -917,24 +954,24 @@ __global__ void __launch_bounds__(kDv / 4) fp8_combine_kernel(const TcArgs p) {
     if (p.lse && tid == 0) p.lse[(int64_t)t * p.N1 + h] = lse2 * 0.6931471805599453f;
 }
 
-// Tensor map over [rows][D] elements with 128-byte swizzle, boxes of 128 bytes x box_rows.
-int make_map(CUtensorMap *map, const void *base, int64_t rows, int D, bool bf16, uint32_t box_rows) {
+// Tensor map over [rows][D] bf16, boxes of 32 rows x 64 columns (128-byte swizzle) or 32 (64-byte).
+int make_map(CUtensorMap *map, const void *base, int64_t rows, int D, uint32_t columns) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return SAS_ERR_CUDA;
     if (rows >= INT32_MAX) return SAS_ERR_UNSUPPORTED;
     cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)rows};
-    cuuint64_t strides[1] = {(cuuint64_t)D * (bf16 ? 2 : 1)};
-    cuuint32_t box[2] = {bf16 ? 64u : 128u, box_rows};
+    cuuint64_t strides[1] = {(cuuint64_t)D * 2};
+    cuuint32_t box[2] = {columns, 32};
     cuuint32_t estr[2] = {1, 1};
-    const CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2,
-                          const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(base), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          columns == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? SAS_OK : SAS_ERR_CUDA;
 }
 
 constexpr int kClusters = 74;  // 148 SMs / 2
-constexpr int kMinPieceTiles = 2;
+constexpr int kMinPieceTiles = 3;
 constexpr int64_t kMaxPartialBytes = int64_t(1) << 30;
 
 struct Plan {
@@ -947,7 +984,7 @@ Plan plan(const SasFp8Args &a) {
     if (a.num_tokens <= 0 || 2 * (int64_t)a.num_tokens > kClusters) return pl;
     const int64_t win = std::min<int64_t>((int64_t)a.ori_win_left + 1 + a.ori_first, (int64_t)a.ori_table_len * a.ori_block_size);
     const int64_t cmp = a.scenario == 3 ? a.topk : a.scenario == 2 ? (int64_t)a.cmp_table_len * a.cmp_block_size : 0;
-    const int64_t est = (win + 3 + cmp + kBK - 1) / kBK;
+    const int64_t est = (win + cmp + kBK - 1) / kBK;
     int64_t P = std::min<int64_t>(kClusters / a.num_tokens, (est + kMinPieceTiles - 1) / kMinPieceTiles);
     P = std::min<int64_t>(P, kMaxPieces);
     if (P <= 1) return pl;
@@ -973,19 +1010,15 @@ int launch_fp8_tc(const SasFp8Args &a, const Args &args, const Layout &L, char *
     static_cast<Args &>(p) = args;
     const Plan pl = plan(a);
     p.status = reinterpret_cast<uint32_t *>(p.rec + TR_STATUS);  // record 0 carries what no token is known for
-    p.ori_rows = a.ori_block_num * a.ori_block_size;
-    p.cmp_rows = a.scenario >= 2 ? a.cmp_block_num * a.cmp_block_size : p.ori_rows;
     p.P = pl.P;
     p.M = pl.M;
     if ((int64_t)a.num_tokens * pl.P >= INT32_MAX) return SAS_ERR_UNSUPPORTED;
     p.U = a.num_tokens * pl.P;
     p.part_o = reinterpret_cast<float *>(ws + L.part_o);
     p.part_s = reinterpret_cast<float *>(ws + L.part_s);
-    CUtensorMap ori_map, cmp_map, q_map, out_map;
-    int rc = make_map(&ori_map, p.ori, p.ori_rows, p.Dq, false, 1);
-    if (!rc) rc = make_map(&cmp_map, a.scenario >= 2 ? p.cmp : p.ori, p.cmp_rows, p.Dq, false, 1);
-    if (!rc) rc = make_map(&q_map, p.q, (int64_t)p.T * p.N1, p.Dq, true, 32);
-    if (!rc) rc = make_map(&out_map, p.out, (int64_t)p.T * p.N1, kDv, true, 32);
+    CUtensorMap q_map, out_map;
+    int rc = make_map(&q_map, p.q, (int64_t)p.T * p.N1, p.Dq, 64);
+    if (!rc) rc = make_map(&out_map, p.out, (int64_t)p.T * p.N1, kDv, 32);
     if (rc) return rc;
     int dev = 0;
     if (check_cuda(cudaGetDevice(&dev))) return SAS_ERR_CUDA;
@@ -1015,7 +1048,7 @@ int launch_fp8_tc(const SasFp8Args &a, const Args &args, const Layout &L, char *
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    if (check_cuda(cudaLaunchKernelEx(&cfg, fp8_tc_kernel, p, ori_map, cmp_map, q_map, out_map))) return SAS_ERR_CUDA;
+    if (check_cuda(cudaLaunchKernelEx(&cfg, fp8_tc_kernel, p, q_map, out_map))) return SAS_ERR_CUDA;
     if (p.P > 1) {
         cudaLaunchConfig_t cc = {};
         cc.gridDim = dim3(a.num_tokens, a.num_heads, 1);
