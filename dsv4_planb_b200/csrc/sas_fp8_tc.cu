@@ -10,9 +10,9 @@
 // of one bf16 MMA, at half the bytes gathered.
 //
 // A key's scale s_j multiplies its score and its value.  With t_ij = scale q_i k_j in log2 units, the
-// weight of value row j (its codes) is 2^(t_ij) s_j, so the running maximum is taken over
-// x_ij = t_ij + log2 s_j, P_ij = 2^(x_ij - m_i + 5.75) goes to the MMA, and the softmax's denominator
-// adds P_ij / s_j.  The sink joins at the end.
+// weight of value row j (its codes) is 2^(t_ij) s_j, so the running maximum m_i is taken over
+// t_ij + log2 s_j.  e_ij = 2^(t_ij - m_i + 5.75) adds to the softmax's denominator and
+// P_ij = e_ij s_j goes to the MMA.  The sink joins at the end.
 //
 // A unit of work (a token, or a piece of one) goes to a cluster of two CTAs on two SMs that split it
 // by role, because O alone (128 heads x 512 fp32) fills one SM's tensor memory:
@@ -22,7 +22,7 @@
 //         S (2 x 96 columns)
 //   4 warps gather 96 key rows per tile          4 warps gather the first 512 bytes of the rows
 //           (cp.async into the MMA's swizzle)
-//   1 warp  S = Q K^T: 2 MMAs (hi, lo) of M 128, 1 warp  O += P V: 2 (hi, lo) per 32 keys and 128
+//   1 warp  S = Q K^T: 2 MMAs (hi, lo) of M 128, 1 warp  O += P V: 2 (hi, lo) per 32 keys and 256
 //           N 96, K 32 per 32 dims                       value dims; V is the N-major B operand, the
 //                                                        same bytes in the same swizzle as K
 //   8 warps split Q; softmax (thread = head;     8 warps rescale O where a maximum rose; epilogue
@@ -41,7 +41,7 @@
 //     same code alone): it reads S twice from TMEM in loops of 32 keys.
 //   - With 128 heads some maximum rises in most tiles.  It is followed only past 2^3 (P <= 2^8.75, the
 //     e4m3 range; the largest weight is then at least 2^5.75, and the 2^-10 that a weight can be off by
-//     where its lo is subnormal are 2^-15.75 of it), and O is rescaled 128 columns at a time, each as
+//     where its lo is subnormal are 2^-15.75 of it), and O is rescaled 256 columns at a time, each as
 //     soon as the last tile's product of these columns is complete.
 //
 // Keys of a token: first positions, then the window, then the compressed rows.  Slots without a key
@@ -89,15 +89,14 @@ constexpr int kMaxPieces = 64;
 constexpr int kMsgLo = 128 * 128, kMsgStats = kMsgLo + 128 * 64, kMsgBytes = kMsgStats + 1024;
 
 struct KeyConst {
-    float s[kBK];   // scale; 0: a zero row or no key
+    float s[kBK];   // scale; 0: a zero row
     float ls[kBK];  // log2 s; -60 for zero rows (their values do not count), -inf: no key
-    float r[kBK];   // 1 / s (2^60 for zero rows, 0: no key)
 };
 
 struct Hdr {
     uint64_t full[kStages], empty[kStages], s_full[2], s_free[2], q_raw, q_full, c_full[kConsts];
     uint64_t x_bar[4][2], m_bar[4][2], l_bar[4];  // of the two warps that share 32 heads
-    uint64_t p_full[2], p_empty[2], o_full, o_empty, event, rs_done[kVSlabs], pv_done[kVSlabs];
+    uint64_t p_full[2], p_empty[2], o_full, o_empty, event, rs_done[2], pv_done[2];
     uint64_t tq_full[kTq], tq_empty[kTq];
     volatile int tq[kTq];
     uint32_t tmem_base;
@@ -266,7 +265,6 @@ __device__ void producer(const TcArgs &p, const Sync &sy, const CUtensorMap *q_m
         int i = it.j0 * kBK + key_at;
         const int32_t f0 = key_fetch(p, it, i);
         int32_t fetched = i + kBK < end ? key_fetch(p, it, i + kBK) : -1;
-        Key key = key_row(p, it, i, f0, bits);
         if constexpr (kScore) {
             // raw Q of the token, three chunks of 64 dims per stage: this warp's 32 head rows, by TMA
             const int chunks = p.Dq / 64;
@@ -284,6 +282,7 @@ __device__ void producer(const TcArgs &p, const Sync &sy, const CUtensorMap *q_m
                 }
             }
         }
+        Key key = key_row(p, it, i, f0, bits);  // behind Q's loads, which need no lookup
         for (int j = it.j0; j < it.j1; ++j, i += kBK, ++tiles, next()) {
             if (key.row >= 0 && !scale_ok(key.s)) {
                 bits |= SAS_STATUS_BAD_SCALE;
@@ -293,9 +292,8 @@ __device__ void producer(const TcArgs &p, const Sync &sy, const CUtensorMap *q_m
                 KeyConst &c = consts[tiles % kConsts];
                 if (holds) {
                     const bool row = key.row >= 0;
-                    c.s[key_at] = row ? key.s : 0.f;
+                    c.s[key_at] = row ? key.s : key.live ? 0.f : 1.f;
                     c.ls[key_at] = row ? log2f(key.s) : key.live ? -60.f : -INFINITY;
-                    c.r[key_at] = row ? 1.f / key.s : key.live ? kScaleMax : 0.f;
                 }
                 __syncwarp();
                 if (lane == 0) {
@@ -469,8 +467,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         init(&hd->o_full, 1, 1);
         init(&hd->o_empty, 1, kSoftWarps);
         init(&hd->event, 1, 1);
-        init(hd->rs_done, kVSlabs, kSoftWarps);
-        init(hd->pv_done, kVSlabs, 1);
+        init(hd->rs_done, 2, kSoftWarps);
+        init(hd->pv_done, 2, 1);
         init(hd->tq_full, kTq, 1);
         init(hd->tq_empty, kTq, kReaders);
         hd->abort = 0;
@@ -643,25 +641,32 @@ __global__ void __launch_bounds__(kThreads, 1)
                     // the slot was read by the peer, so its copies have left the staging buffer
                     if (!wait_warp(sy, smem_u32(&hd->p_empty[g]), (mine & 1) ^ 1, true)) goto done;
                     uint64_t sum0 = 0, sum1 = 0;
+                    const int live = it.rec[TR_NORI] + it.rec[TR_NCMP] - (it.j0 + e) * kBK;
 #pragma unroll 1
                     for (int q = 0; q < kBK / 32; ++q) {
                         const int i0 = q * 32;
                         uint32_t sr[32], hi[8], lo[8];
                         tmem_ld32(s_at + i0, sr);
                         tc_wait_ld();
+                        uint64_t f2 = rq2;
+                        if (live - i0 < 32) {  // slots without a key, in the token's last tile: weight 0
+                            f2 = pack2(1.f, 1.f);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                sr[i] = __float_as_uint(i < live - i0 ? __uint_as_float(sr[i]) * rq : -INFINITY);
+                        }
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
                             const ulonglong2 s4 = *reinterpret_cast<const ulonglong2 *>(&c.s[i0 + i]);
-                            const ulonglong2 l4 = *reinterpret_cast<const ulonglong2 *>(&c.ls[i0 + i]);
-                            const ulonglong2 r4 = *reinterpret_cast<const ulonglong2 *>(&c.r[i0 + i]);
-                            const float2 a = unpack2(add2(fma2(mul2(pack2(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1])), rq2), s4.x, l4.x), mb2));
-                            const float2 b = unpack2(add2(fma2(mul2(pack2(__uint_as_float(sr[i + 2]), __uint_as_float(sr[i + 3])), rq2), s4.y, l4.y), mb2));
-                            const float p0 = ex2_approx(a.x), p1 = ex2_approx(a.y), p2 = ex2_approx(b.x), p3 = ex2_approx(b.y);
-                            sum0 = fma2(pack2(p0, p1), r4.x, sum0);
-                            sum1 = fma2(pack2(p2, p3), r4.y, sum1);
+                            const float2 a = unpack2(fma2(mul2(pack2(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1])), f2), s4.x, mb2));
+                            const float2 b = unpack2(fma2(mul2(pack2(__uint_as_float(sr[i + 2]), __uint_as_float(sr[i + 3])), f2), s4.y, mb2));
+                            const uint64_t e0 = pack2(ex2_approx(a.x), ex2_approx(a.y)), e1 = pack2(ex2_approx(b.x), ex2_approx(b.y));
+                            sum0 = add2(sum0, e0);
+                            sum1 = add2(sum1, e1);
+                            const float2 p0 = unpack2(mul2(e0, s4.x)), p1 = unpack2(mul2(e1, s4.y));
                             uint32_t h0, l0, h1, l1;
-                            split2(p0, p1, h0, l0);
-                            split2(p2, p3, h1, l1);
+                            split2(p0.x, p0.y, h0, l0);
+                            split2(p1.x, p1.y, h1, l1);
                             hi[i >> 2] = h0 | (h1 << 16);
                             lo[i >> 2] = l0 | (l1 << 16);
                         }
@@ -701,7 +706,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                             p.part_s[((int64_t)it.t * p.P + it.piece) * p.N1 + h] = own;
                         }
                     }
-                    *reinterpret_cast<float2 *>(stage + kMsgStats + h * 8) = make_float2(head ? alpha : 1.f, fin);
+                    // the sign of the warp's first alpha: some row of the warp has one
+                    if (!head) alpha = 1.f;
+                    const bool some = __any_sync(0xffffffffu, alpha != 1.f);
+                    *reinterpret_cast<float2 *>(stage + kMsgStats + h * 8) = make_float2(lane == 0 && some ? -alpha : alpha, fin);
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
@@ -723,7 +731,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (warp >= kProdWarp0) {
             producer<false>(p, sy, nullptr, ring, hd, nullptr);
         } else if (warp == kMmaWarp) {
-            constexpr uint32_t idesc = idesc_e4m3(128, 128, 1);
+            constexpr uint32_t idesc = idesc_e4m3(128, 256, 1);
             uint32_t st = 0, phase = 0, pc = 0, oc = 0, rsc = 0;
             for (uint32_t k = 0;; ++k) {
                 int u;
@@ -740,13 +748,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint8_t *msg = msgs + ps * kMsgBytes;
                     const float2 *stat = reinterpret_cast<const float2 *>(msg + kMsgStats);
                     const bool last = j == it.j1 - 1;
-                    bool rescale = false;
-                    if (j > it.j0) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) rescale |= stat[lane + 32 * i].x != 1.f;
-                        rescale = __any_sync(0xffffffffu, rescale);
-                    }
-                    if (rescale) {  // warps 0-7 scale the rows, slab by slab
+                    const bool rescale = j > it.j0 && __any_sync(0xffffffffu, stat[(lane & 3) * 32].x < 0.f);
+                    if (rescale) {  // warps 0-7 scale the rows, 256 columns at a time
                         if (lane == 0) {
                             hd->event_code = (int)(pc & 0x7fffffff);
                             mbar_arrive(smem_u32(&hd->event));
@@ -760,12 +763,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint64_t a1 = sdesc_sw128(smem_u32(msg), 16, 1024), a2 = sdesc_sw64(smem_u32(msg) + kMsgLo);
                     const uint32_t base = smem_u32(ring) + st * kVStage;
 #pragma unroll 1
-                    for (int c = 0; c < kVSlabs; ++c) {
+                    for (int c = 0; c < 2; ++c) {  // 256 value dims each
                         if (rescale && !wait_warp(sy, smem_u32(&hd->rs_done[c]), rsc & 1)) goto done;
                         tc_fence_after();
                         if (lane == 0) {
-                            const uint64_t b = sdesc_sw128(base + c * kSlab, kSlab, 1024);
-                            const uint32_t d = tmem + c * 128;
+                            const uint64_t b = sdesc_sw128(base + c * 2 * kSlab, kSlab, 1024);
+                            const uint32_t d = tmem + c * 256;
 #pragma unroll
                             for (int i = 0; i < kBK / 32; ++i) {
                                 mma8_ss(d, a1 + 2 * i, b + 256 * i, idesc, (j > it.j0 || i > 0) ? 1u : 0u);
@@ -815,26 +818,29 @@ __global__ void __launch_bounds__(kThreads, 1)
                     ++ev;
                     const int pc = hd->event_code;
                     if (pc < 0) break;
-                    const float a = reinterpret_cast<const float2 *>(msgs + (pc & 1) * kMsgBytes + kMsgStats)[h].x;
+                    const float a = fabsf(reinterpret_cast<const float2 *>(msgs + (pc & 1) * kMsgBytes + kMsgStats)[h].x);
                     const bool any = __any_sync(0xffffffffu, a != 1.f);
 #pragma unroll 1
-                    for (int c = 0; c < kVSlabs; ++c) {
+                    for (int c = 0; c < 2; ++c) {
                         // the product of the tile before, of these columns
                         if (!wait_warp(sy, smem_u32(&hd->pv_done[c]), (pc - 1) & 1)) goto done;
                         if (any) {
                             tc_fence_after();
-                            const uint32_t at = trow + c * 128 + g * 64;
-                            uint32_t r0[32], r1[32];
-                            tmem_ld32(at, r0);
-                            tmem_ld32(at + 32, r1);
-                            tc_wait_ld();
+#pragma unroll 1
+                            for (int e = 0; e < 128; e += 64) {
+                                const uint32_t at = trow + c * 256 + g * 128 + e;
+                                uint32_t r0[32], r1[32];
+                                tmem_ld32(at, r0);
+                                tmem_ld32(at + 32, r1);
+                                tc_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                r0[i] = __float_as_uint(__uint_as_float(r0[i]) * a);
-                                r1[i] = __float_as_uint(__uint_as_float(r1[i]) * a);
+                                for (int i = 0; i < 32; ++i) {
+                                    r0[i] = __float_as_uint(__uint_as_float(r0[i]) * a);
+                                    r1[i] = __float_as_uint(__uint_as_float(r1[i]) * a);
+                                }
+                                tmem_st32(at, r0);
+                                tmem_st32(at + 32, r1);
                             }
-                            tmem_st32(at, r0);
-                            tmem_st32(at + 32, r1);
                             tc_wait_st();
                             tc_fence_before();
                         }
