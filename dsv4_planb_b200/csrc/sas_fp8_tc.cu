@@ -20,15 +20,15 @@
 //   CTA 0 ("score")                              CTA 1 ("output")
 //   TMEM: Q hi / lo (D_qk / 2 columns),          TMEM: O (128 x 512 fp32)
 //         S (2 x 96 columns)
-//   4 warps gather 96 key rows per tile          4 warps gather the first 512 bytes of the rows
+//   3 warps gather 96 key rows per tile          3 warps gather the first 512 bytes of the rows
 //           (cp.async into the MMA's swizzle)
 //   1 warp  S = Q K^T: 2 MMAs (hi, lo) of M 128, 1 warp  O += P V: 2 (hi, lo) per 32 keys and 256
 //           N 96, K 32 per 32 dims                       value dims; V is the N-major B operand, the
 //                                                        same bytes in the same swizzle as K
-//   8 warps split Q; softmax (thread = head;     8 warps rescale O where a maximum rose; epilogue
-//           warps 0-3 take the even tiles,
-//           4-7 the odd ones); P and factors
-//           go to CTA 1 by bulk copies
+//   8 warps split Q; softmax (thread = head;     8 warps split P (thread = head; warps 0-3 the even
+//           warps 0-3 take the even tiles,               tiles, 4-7 the odd ones); rescale O where a
+//           4-7 the odd ones); P in fp16 and             maximum rose; epilogue
+//           factors go to CTA 1 by bulk copies
 //
 // What the pieces measured on B200, each alone, and what follows from it:
 //   - An MMA of N 64 takes 58 cycles, as one of N 96; N 128 takes 70-83.  96 keys leave room in TMEM for
@@ -37,8 +37,6 @@
 //     16-byte cp.async reaches 56 bytes per cycle from L2 (110 GB/s), and the HBM's rate over all SMs.
 //   - st.async to the other SM moves 12 bytes per cycle and holds the issuing warps meanwhile; a tile's
 //     P is 24 KiB.  Bulk copies from a staging buffer run beside the next tile's softmax.
-//   - Unrolled over a whole tile the softmax was bound by instruction fetch (3.7 times the cycles of the
-//     same code alone): it reads S twice from TMEM in loops of 32 keys.
 //   - With 128 heads some maximum rises in most tiles.  It is followed only past 2^3 (P <= 2^8.75, the
 //     e4m3 range; the largest weight is then at least 2^5.75, and the 2^-10 that a weight can be off by
 //     where its lo is subnormal are 2^-15.75 of it), and O is rescaled 256 columns at a time, each as
@@ -71,21 +69,22 @@ constexpr int kStages = 3;
 constexpr int kDv = 512, kVSlabs = kDv / 128;
 constexpr int kVStage = kVSlabs * kSlab, kKStage = kVStage + kBK * 64;  // K: dims 512 .. 575 as 64-byte rows behind
 constexpr int kQChunk = 128 * 128, kQPerStage = 3;  // raw Q: 64 bf16 dims of 128 heads; chunks per stage of the K ring
-constexpr int kSoftWarps = 8, kMmaWarp = 8, kProdWarp0 = 9, kProdWarps = 4;
-constexpr int kRowsPerWarp = kBK / kProdWarps;
+constexpr int kSoftWarps = 8, kMmaWarp = 8, kProdWarp0 = 9, kProdWarps = 3;  // 12 warps: 168 registers a thread
+static_assert(kBK == 32 * kProdWarps, "a lane per key slot");
 constexpr int kThreads = 32 * (kProdWarp0 + kProdWarps);
 constexpr uint32_t kReaders = 2 * (kSoftWarps + 1 + kProdWarps) - 1;  // of the unit queue: every warp but its writer
 constexpr int kTmemCols = 512, kTmemS = 320;
 // Ring of per-tile key constants.  Those of tile n are written once the stage of tile n - 1 is free: the
-// scores of tile n - 4 are complete, so those of n - 6 have been read for the last time.
-constexpr int kConsts = 6;
+// scores of tile n - 4 are complete, so those of n - 6 have been taken to registers, by warps that are
+// done with tile n - 8.
+constexpr int kConsts = 8;
 constexpr float kTop = 8.75f;        // log2 of the largest P: 431, within e4m3's 448
 constexpr float kRise = 3.f;         // log2 of the rise of a maximum that is left to P
 constexpr int kMaxPieces = 64;
 
-// P message: per head a 128-byte row (SW128) of 96 hi codes and the first 32 lo codes, then a 64-byte
-// row (SW64) of the other lo codes, then {alpha, the unit's final factor}.  The 32 heads of a warp are
-// contiguous in each part.
+// P message: per head 96 weights in fp16, 64 in a 128-byte row (SW128) and 32 in a 64-byte row (SW64), then
+// {alpha, the unit's final factor}.  The 32 heads of a warp are contiguous in each part.  The output CTA
+// puts the codes in the weights' place: 96 hi and 32 lo in the first row, the other 64 lo in the second.
 constexpr int kMsgLo = 128 * 128, kMsgStats = kMsgLo + 128 * 64, kMsgBytes = kMsgStats + 1024;
 
 struct KeyConst {
@@ -96,16 +95,14 @@ struct KeyConst {
 struct Hdr {
     uint64_t full[kStages], empty[kStages], s_full[2], s_free[2], q_raw, q_full, c_full[kConsts];
     uint64_t x_bar[4][2], m_bar[4][2], l_bar[4];  // of the two warps that share 32 heads
-    uint64_t p_full[2], p_empty[2], o_full, o_empty, event, rs_done[2], pv_done[2];
+    uint64_t p_full[2], p_ready[2], p_empty[2], o_full, o_empty, rs_done[2], pv_done[2];
     uint64_t tq_full[kTq], tq_empty[kTq];
     volatile int tq[kTq];
     uint32_t tmem_base;
     volatile int abort;
-    volatile int event_code;  // output CTA: tile (>= 0) whose alpha the warps apply to O; -1: the unit's last product is issued
-    float fin[128];           // per head: factor of O at the end of the unit
     float amax[2][128], m[2][128], l[2][2][128];
 };
-constexpr int kHdr = 6 * 1024;
+constexpr int kHdr = 5 * 1024;
 static_assert(sizeof(Hdr) <= kHdr, "header");
 constexpr int kConstOff = kHdr;
 constexpr int kScoreMsgs = (kConstOff + kConsts * (int)sizeof(KeyConst) + 1023) / 1024 * 1024;
@@ -121,7 +118,22 @@ static_assert(kScoreMsgs % 1024 == 0 && kScoreRing % 1024 == 0 && kKStage % 1024
               kOutMsgs % 1024 == 0 && kMsgBytes % 1024 == 0 && kOutStage % 1024 == 0, "swizzled tiles are 1 KiB aligned");
 static_assert(kQPerStage * kQChunk <= kKStage && kSmemBytes <= 232448, "shared memory");
 
+// n / d for 0 <= n < 2^31 as a multiplication: 2^(32 + s) <= m d < 2^(32 + s) + 2^(s + 1) with 2^s < d <= 2^(s + 1)
+// makes the quotient exact; d = 1 has no such m.
+struct Div {
+    uint32_t d, m, s;
+};
+__device__ __forceinline__ int div(int n, const Div &v) { return v.d == 1 ? n : (int)(__umulhi((uint32_t)n, v.m) >> v.s); }
+Div make_div(uint32_t d) {
+    Div v{d, 0, 0};
+    if (d == 1) return v;
+    while ((2ull << v.s) < d) ++v.s;
+    v.m = (uint32_t)(((1ull << (32 + v.s)) + d - 1) / d);
+    return v;
+}
+
 struct TcArgs : Args {
+    Div ori_div, cmp_div;    // by the block sizes
     uint32_t *status;
     int U, P, M;             // units; pieces per token, tiles per piece (P = 1: whole tokens)
     float *part_o, *part_s;
@@ -157,6 +169,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
         : "memory");
 }
 
+// Whether some row of O is to be rescaled before the message's product.
+__device__ __forceinline__ bool some_alpha(const uint8_t *msg) {
+    return __any_sync(0xffffffffu, reinterpret_cast<const float2 *>(msg + kMsgStats)[(threadIdx.x & 3) * 32].x < 0.f);
+}
+
 struct Item {
     int32_t rec[TR_INTS];
     int t, piece, np, ntiles, j0, j1;  // tiles [j0, j1) of token t
@@ -186,43 +203,39 @@ __device__ __forceinline__ Item load_unit(const TcArgs &p, int u) {
 // Row lookup of key slot i in three steps, each a tile ahead of the next so that their loads hide
 // behind the copies: the table entry (or the resolved row), the physical row, its block's scale.
 __device__ __forceinline__ int32_t key_fetch(const TcArgs &p, const Item &it, int i) {
-    const int32_t *table = p.ori_bt;
-    int slot = i, bs = p.ori_bs, len = p.ori_table_len;
-    if (i < it.rec[TR_NORI]) {
-        slot = ori_position(it.rec, i);
-    } else {
-        slot = i - it.rec[TR_NORI];
-        if (slot >= it.rec[TR_NCMP]) return -1;
-        if (p.scenario == 3) return __ldg(p.rows + (int64_t)it.t * p.K + slot);
-        table = p.cmp_bt, bs = p.cmp_bs, len = p.cmp_table_len;
-    }
-    const int blk = slot / bs;
-    return blk < len ? __ldg(table + (int64_t)it.rec[TR_B] * len + blk) : -2;
+    const bool win = i < it.rec[TR_NORI];
+    const int slot = win ? ori_position(it.rec, i) : i - it.rec[TR_NORI];
+    if (!win && slot >= it.rec[TR_NCMP]) return -1;
+    if (!win && p.scenario == 3) return __ldg(p.rows + (int64_t)it.t * p.K + slot);
+    const int blk = div(slot, win ? p.ori_div : p.cmp_div), len = win ? p.ori_table_len : p.cmp_table_len;
+    return blk < len ? __ldg((win ? p.ori_bt : p.cmp_bt) + (int64_t)it.rec[TR_B] * len + blk) : -2;
 }
 
 struct Key {
-    int32_t row;  // physical row, or -1: zeros
-    float s;      // its block's scale (loaded), 1 without a row
-    bool live;    // the slot holds a key
+    const uint8_t *row;  // nullptr: zeros
+    float s;             // its block's scale (loaded), 1 without a row
+    bool live;           // the slot holds a key
 };
 
 __device__ __forceinline__ Key key_row(const TcArgs &p, const Item &it, int i, int32_t fetched, uint32_t &bits) {
-    Key key{-1, 1.f, false};
+    Key key{nullptr, 1.f, false};
     const bool win = i < it.rec[TR_NORI];
-    const int slot = win ? i : i - it.rec[TR_NORI];
+    const int slot = win ? ori_position(it.rec, i) : i - it.rec[TR_NORI];
     key.live = win || slot < it.rec[TR_NCMP];
     if (!key.live) return key;
-    const int bs = win ? p.ori_bs : p.cmp_bs;
-    int blk = fetched;
+    const Div &d = win ? p.ori_div : p.cmp_div;
+    int row, blk;
     if (!win && p.scenario == 3) {
-        if (fetched < 0) return key;
-        key.row = fetched;
-        blk = fetched / bs;
+        row = fetched;
+        blk = div(max(row, 0), d);
     } else {
-        if (fetched < -1 || fetched >= (win ? p.ori_block_num : p.cmp_block_num)) bits |= SAS_STATUS_BAD_BLOCK;
-        else if (fetched >= 0) key.row = fetched * bs + (win ? ori_position(it.rec, slot) : slot) % bs;
-        if (key.row < 0) return key;
+        blk = fetched;
+        const bool bad = blk < -1 || blk >= (win ? p.ori_block_num : p.cmp_block_num);
+        if (bad) bits |= SAS_STATUS_BAD_BLOCK;
+        row = bad || blk < 0 ? -1 : blk * (int)d.d + (slot - div(slot, d) * (int)d.d);
     }
+    if (row < 0) return key;
+    key.row = (win ? p.ori : p.cmp) + (int64_t)row * p.Dq;
     key.s = __ldg((win ? p.ori_scale : p.cmp_scale) + blk);
     return key;
 }
@@ -231,22 +244,23 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
-// The gather warps.  Each takes 24 of a tile's 96 key slots (a lane per slot) and copies its rows with
-// 16-byte cp.async: an instruction moves 512 bytes of one row, 32 granules over the four slabs (row r of
-// a slab at r * 128, granule g at g ^ r % 8: the MMA's 128-byte swizzle); dims 512 .. 575 go to 64-byte
-// rows (granule g at g ^ r / 2 % 4: the 64-byte swizzle), 8 rows per instruction.  A stage's full
-// barrier counts the 128 threads; each arrives when its copies have landed.  The warps share nothing else.
+// The gather warps.  Each takes 32 of a tile's 96 key slots (a lane per slot) and copies their rows with
+// 16-byte cp.async: an instruction moves 128 bytes of 4 rows (row r of a slab at r * 128, granule g at
+// g ^ r % 8: the MMA's 128-byte swizzle); dims 512 .. 575 go to 64-byte rows (granule g at g ^ r / 2 % 4:
+// the 64-byte swizzle), 8 rows per instruction.  Row addresses go from lane to lane once per 4 rows.  A
+// stage's full barrier counts the threads; each arrives when its copies have landed.  The warps share
+// nothing else.
 template <bool kScore>
 __device__ void producer(const TcArgs &p, const Sync &sy, const CUtensorMap *q_map, uint8_t *ring, Hdr *hd,
                          KeyConst *consts) {
     constexpr uint32_t kStageBytes = kScore ? kKStage : kVStage;
-    const int w = (threadIdx.x >> 5) - kProdWarp0, lane = threadIdx.x & 31;
-    const bool holds = lane < kRowsPerWarp;  // this lane looks a key up
-    const int key_at = w * kRowsPerWarp + (holds ? lane : 0);
+    const int w = (threadIdx.x >> 5) - kProdWarp0, lane = threadIdx.x & 31, key_at = w * 32 + lane;
     const bool writer = kScore && w == 0;
     const bool tail = kScore && p.Dq > 512;
     const uint32_t ring_at = smem_u32(ring);
-    const uint32_t dst_lane = (lane >> 3) * kSlab + w * kRowsPerWarp * 128, gran = (lane & 7) << 4;
+    // this lane's granule lane % 8 of row 4 k + lane / 8: offsets for even k, and what odd k change
+    const uint32_t dst0 = key_at / 32 * 4096 + (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4);
+    const uint32_t src_off = (lane & 7) * 16;
     uint32_t st = 0, phase = 1, tiles = 0, bits = 0;  // stage, and the parity its empty barrier is waited on
     int pend = -1;
     auto next = [&] {
@@ -266,17 +280,18 @@ __device__ void producer(const TcArgs &p, const Sync &sy, const CUtensorMap *q_m
         const int32_t f0 = key_fetch(p, it, i);
         int32_t fetched = i + kBK < end ? key_fetch(p, it, i + kBK) : -1;
         if constexpr (kScore) {
-            // raw Q of the token, three chunks of 64 dims per stage: this warp's 32 head rows, by TMA
+            // raw Q of the token, three chunks of 64 dims per stage, 32 head rows at a time by TMA
             const int chunks = p.Dq / 64;
             for (int c = 0; c < chunks; c += kQPerStage, next()) {
                 if (!wait_warp(sy, smem_u32(&hd->empty[st]), phase)) return;
                 const uint32_t fb = smem_u32(&hd->full[st]);
-                if (lane == 0 && w * 32 < p.N1) {
-                    const int n = min(kQPerStage, chunks - c);
-                    mbar_arrive_expect_tx(fb, n * 4096);
-                    for (int e = 0; e < n; ++e)
-                        tma_load_2d(ring_at + st * kStageBytes + e * kQChunk + w * 4096, q_map, (c + e) * 64,
-                                    it.t * p.N1 + w * 32, fb);
+                if (lane == 0 && w * 32 < p.N1) {  // warp 0 takes the fourth 32 rows too
+                    const int n = min(kQPerStage, chunks - c), groups = w == 0 && p.N1 > 96 ? 2 : 1;
+                    mbar_arrive_expect_tx(fb, n * groups * 4096);
+                    for (int g = w; g < w + 3 * groups; g += 3)
+                        for (int e = 0; e < n; ++e)
+                            tma_load_2d(ring_at + st * kStageBytes + e * kQChunk + g * 4096, q_map, (c + e) * 64,
+                                        it.t * p.N1 + g * 32, fb);
                 } else {
                     mbar_arrive(fb);  // rows of no head: whatever lies there
                 }
@@ -284,17 +299,15 @@ __device__ void producer(const TcArgs &p, const Sync &sy, const CUtensorMap *q_m
         }
         Key key = key_row(p, it, i, f0, bits);  // behind Q's loads, which need no lookup
         for (int j = it.j0; j < it.j1; ++j, i += kBK, ++tiles, next()) {
-            if (key.row >= 0 && !scale_ok(key.s)) {
+            if (key.row != nullptr && !scale_ok(key.s)) {
                 bits |= SAS_STATUS_BAD_SCALE;
-                key.row = -1;
+                key.row = nullptr;
             }
             if constexpr (kScore) {
                 KeyConst &c = consts[tiles % kConsts];
-                if (holds) {
-                    const bool row = key.row >= 0;
-                    c.s[key_at] = row ? key.s : key.live ? 0.f : 1.f;
-                    c.ls[key_at] = row ? log2f(key.s) : key.live ? -60.f : -INFINITY;
-                }
+                const bool row = key.row != nullptr;
+                c.s[key_at] = row ? key.s : key.live ? 0.f : 1.f;
+                c.ls[key_at] = row ? log2f(key.s) : key.live ? -60.f : -INFINITY;
                 __syncwarp();
                 if (lane == 0) {
                     mbar_arrive(smem_u32(&hd->c_full[tiles % kConsts]));
@@ -304,26 +317,26 @@ __device__ void producer(const TcArgs &p, const Sync &sy, const CUtensorMap *q_m
             }
             if (!wait_warp(sy, smem_u32(&hd->empty[st]), phase)) return;
             const uint32_t base = ring_at + st * kStageBytes;
-            const uint8_t *src = key.row < 0 ? nullptr
-                                             : (i < it.rec[TR_NORI] ? p.ori : p.cmp) + (int64_t)key.row * p.Dq;
-            const uint64_t src64 = reinterpret_cast<uint64_t>(src);
-#pragma unroll 8
-            for (int r = 0; r < kRowsPerWarp; ++r) {
-                const uint64_t a = __shfl_sync(0xffffffffu, src64, r);
-                cp_async16(base + dst_lane + r * 128 + (gran ^ ((r & 7) << 4)),
-                           reinterpret_cast<const uint8_t *>(a ? a : reinterpret_cast<uint64_t>(p.ori)) + lane * 16, a ? 16 : 0);
+            const uint64_t mine = reinterpret_cast<uint64_t>(key.row);
+#pragma unroll
+            for (int k4 = 0; k4 < 8; ++k4) {
+                const uint64_t a = __shfl_sync(0xffffffffu, mine, 4 * k4 + (lane >> 3));
+                const uint8_t *src = reinterpret_cast<const uint8_t *>(a ? a : reinterpret_cast<uint64_t>(p.ori)) + src_off;
+                const uint32_t n = a ? 16 : 0, dst = base + (dst0 ^ ((k4 & 1) << 6)) + k4 * 512;
+#pragma unroll
+                for (int c = 0; c < kVSlabs; ++c) cp_async16(dst + c * kSlab, src + c * 128, n);
             }
             if (tail) {
 #pragma unroll
-                for (int r0 = 0; r0 < kRowsPerWarp; r0 += 8) {
-                    const int r = r0 + (lane >> 2), row = w * kRowsPerWarp + r;
-                    const uint64_t a = __shfl_sync(0xffffffffu, src64, r);
-                    cp_async16(base + kVStage + row * 64 + (((lane & 3) ^ ((row >> 1) & 3)) << 4),
+                for (int r0 = 0; r0 < 32; r0 += 8) {
+                    const int r = r0 + (lane >> 2);
+                    const uint64_t a = __shfl_sync(0xffffffffu, mine, r);
+                    cp_async16(base + kVStage + (w * 32 + r) * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4),
                                a ? reinterpret_cast<const uint8_t *>(a) + 512 + (lane & 3) * 16 : p.ori, a ? 16 : 0);
                 }
             }
             asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&hd->full[st])) : "memory");
-            key = Key{-1, 1.f, false};  // the next tile's lookups, behind the copies
+            key = Key{nullptr, 1.f, false};  // the next tile's lookups, behind the copies
             if (i + kBK < end) key = key_row(p, it, i + kBK, fetched, bits);
             fetched = i + 2 * kBK < end ? key_fetch(p, it, i + 2 * kBK) : -1;
         }
@@ -333,32 +346,43 @@ __device__ void producer(const TcArgs &p, const Sync &sy, const CUtensorMap *q_m
     if (bits) sas::set_status(p.status, bits);
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack_half(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&v);
 }
 
-// Two fp32 values (at most 448) as two pairs of e4m3 codes, hi + lo.  fp16 holds hi and the difference
-// exactly; the value itself is first rounded to fp16 (2^-12 relative).
-__device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t &lo) {
-    const __half2 x = __floats2half2_rn(a, b);
+// Two fp16 values (at most 448) as two pairs of e4m3 codes, hi + lo.  The difference is exact in fp16.
+__device__ __forceinline__ void split2(uint32_t x, uint32_t &hi, uint32_t &lo) {
     uint16_t h, l;
-    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(h) : "r"(*reinterpret_cast<const uint32_t *>(&x)));
+    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(h) : "r"(x));
     const uint32_t back = e4m3x2_to_half2(h);
-    const __half2 d = __hsub2(x, *reinterpret_cast<const __half2 *>(&back));
+    const __half2 d = __hsub2(*reinterpret_cast<const __half2 *>(&x), *reinterpret_cast<const __half2 *>(&back));
     asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(l) : "r"(*reinterpret_cast<const uint32_t *>(&d)));
     hi = h;
     lo = l;
+}
+// Four fp16 values into four hi and four lo codes.
+__device__ __forceinline__ void split4h(uint32_t a, uint32_t b, uint32_t &hi, uint32_t &lo) {
+    uint32_t h0, l0, h1, l1;
+    split2(a, h0, l0);
+    split2(b, h1, l1);
+    hi = h0 | (h1 << 16);
+    lo = l0 | (l1 << 16);
 }
 
 // Four bf16 values times f into four hi and four lo codes.
 __device__ __forceinline__ void split4(uint32_t a, uint32_t b, float f, uint32_t &hi, uint32_t &lo) {
     const float2 x = sas::DT<__nv_bfloat16>::to_f2(a), y = sas::DT<__nv_bfloat16>::to_f2(b);
-    uint32_t h0, l0, h1, l1;
-    split2(x.x * f, x.y * f, h0, l0);
-    split2(y.x * f, y.y * f, h1, l1);
-    hi = h0 | (h1 << 16);
-    lo = l0 | (l1 << 16);
+    split4h(pack_half(x.x * f, x.y * f), pack_half(y.x * f, y.y * f), hi, lo);
 }
 
 // Q of head row h, raw bf16 in TMEM columns [0, D_qk / 2), into hi and lo codes in place: chunk c of 64
@@ -464,15 +488,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         init(hd->l_bar, 4, 1);
         init(hd->p_full, 2, 1);
         init(hd->p_empty, 2, 1);
+        init(hd->p_ready, 2, kSoftWarps);
         init(&hd->o_full, 1, 1);
         init(&hd->o_empty, 1, kSoftWarps);
-        init(&hd->event, 1, 1);
         init(hd->rs_done, 2, kSoftWarps);
         init(hd->pv_done, 2, 1);
         init(hd->tq_full, kTq, 1);
         init(hd->tq_empty, kTq, kReaders);
         hd->abort = 0;
-        hd->event_code = 0;
         // the output CTA expects the first message of each P slot (bulk copies complete it)
         if (rank == 1)
             for (int i = 0; i < 2; ++i) mbar_arrive_expect_tx(smem_u32(&hd->p_full[i]), kMsgBytes);
@@ -572,6 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t s_at = trow + kTmemS + g * kBK;
             uint8_t *stage = smem + kScoreMsgs + g * kMsgBytes;
             const uint32_t row1 = smem_u32(stage) + h * 128, row2 = smem_u32(stage) + kMsgLo + h * 64;
+            const uint32_t sw1 = (h & 7) << 4, sw2 = ((h >> 1) & 3) << 4;
             const uint32_t peer_msg = map_to_cta(smem_u32(smem + kOutMsgs), 1) + g * kMsgBytes;
             const uint32_t peer_full = map_to_cta(smem_u32(&hd->p_full[g]), 1);
             const float sink = head && p.sinks ? p.sinks[h] : -INFINITY;
@@ -616,8 +640,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                             const ulonglong2 l4 = *reinterpret_cast<const ulonglong2 *>(&c.ls[i0 + i]);
                             const float2 a = unpack2(fma2(mul2(pack2(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1])), rq2), s4.x, l4.x));
                             const float2 b = unpack2(fma2(mul2(pack2(__uint_as_float(sr[i + 2]), __uint_as_float(sr[i + 3])), rq2), s4.y, l4.y));
-                            mx0 = fmaxf(mx0, fmaxf(a.x, a.y));
-                            mx1 = fmaxf(mx1, fmaxf(b.x, b.y));
+                            mx0 = max3(mx0, a.x, a.y);
+                            mx1 = max3(mx1, b.x, b.y);
                         }
                     }
                     const float mx = fmaxf(mx0, mx1);
@@ -643,9 +667,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     uint64_t sum0 = 0, sum1 = 0;
                     const int live = it.rec[TR_NORI] + it.rec[TR_NCMP] - (it.j0 + e) * kBK;
 #pragma unroll 1
-                    for (int q = 0; q < kBK / 32; ++q) {
-                        const int i0 = q * 32;
-                        uint32_t sr[32], hi[8], lo[8];
+                    for (int i0 = 0; i0 < kBK; i0 += 32) {
+                        uint32_t sr[32], hp[16];
                         tmem_ld32(s_at + i0, sr);
                         tc_wait_ld();
                         uint64_t f2 = rq2;
@@ -664,19 +687,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                             sum0 = add2(sum0, e0);
                             sum1 = add2(sum1, e1);
                             const float2 p0 = unpack2(mul2(e0, s4.x)), p1 = unpack2(mul2(e1, s4.y));
-                            uint32_t h0, l0, h1, l1;
-                            split2(p0.x, p0.y, h0, l0);
-                            split2(p1.x, p1.y, h1, l1);
-                            hi[i >> 2] = h0 | (h1 << 16);
-                            lo[i >> 2] = l0 | (l1 << 16);
+                            hp[i >> 1] = pack_half(p0.x, p0.y);
+                            hp[(i >> 1) + 1] = pack_half(p1.x, p1.y);
                         }
+                        // keys 0 .. 63 in the 128-byte row, 64 .. 95 in the 64-byte row, 8 keys a granule
+                        const uint32_t row = i0 == 64 ? row2 : row1 + ((i0 << 1) ^ (sw1 & 0x40)), sw = i0 == 64 ? sw2 : sw1 & 0x30;
 #pragma unroll
-                        for (int v = 0; v < 2; ++v) {
-                            st_shared_v4(row1 + (((2 * q + v) ^ (h & 7)) << 4), hi[4 * v], hi[4 * v + 1], hi[4 * v + 2], hi[4 * v + 3]);
-                            const uint32_t at = q == 0 ? row1 + (((6 + v) ^ (h & 7)) << 4)
-                                                       : row2 + (((2 * q - 2 + v) ^ ((h >> 1) & 3)) << 4);
-                            st_shared_v4(at, lo[4 * v], lo[4 * v + 1], lo[4 * v + 2], lo[4 * v + 3]);
-                        }
+                        for (int v = 0; v < 4; ++v)
+                            st_shared_v4(row + ((v << 4) ^ sw), hp[4 * v], hp[4 * v + 1], hp[4 * v + 2], hp[4 * v + 3]);
                     }
                     tc_fence_before();
                     __syncwarp();
@@ -743,21 +761,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ++oc;
                 for (int j = it.j0; j < it.j1; ++j, ++pc) {
                     const int ps = pc & 1;
-                    if (!wait_warp(sy, smem_u32(&hd->p_full[ps]), (pc >> 1) & 1, true)) goto done;
-                    if (lane == 0) mbar_arrive_expect_tx(smem_u32(&hd->p_full[ps]), kMsgBytes);  // the next message
+                    if (!wait_warp(sy, smem_u32(&hd->p_ready[ps]), (pc >> 1) & 1)) goto done;
                     const uint8_t *msg = msgs + ps * kMsgBytes;
-                    const float2 *stat = reinterpret_cast<const float2 *>(msg + kMsgStats);
-                    const bool last = j == it.j1 - 1;
-                    const bool rescale = j > it.j0 && __any_sync(0xffffffffu, stat[(lane & 3) * 32].x < 0.f);
-                    if (rescale) {  // warps 0-7 scale the rows, 256 columns at a time
-                        if (lane == 0) {
-                            hd->event_code = (int)(pc & 0x7fffffff);
-                            mbar_arrive(smem_u32(&hd->event));
-                        }
-                        __syncwarp();
-                    }
-                    if (last)
-                        for (int i = lane; i < 128; i += 32) hd->fin[i] = stat[i].y;
+                    const bool last = j == it.j1 - 1, rescale = j > it.j0 && some_alpha(msg);
                     if (!wait_warp(sy, smem_u32(&hd->full[st]), phase)) goto done;
                     fence_proxy_async_smem();  // the rows were written by cp.async
                     const uint64_t a1 = sdesc_sw128(smem_u32(msg), 16, 1024), a2 = sdesc_sw64(smem_u32(msg) + kMsgLo);
@@ -782,11 +788,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (lane == 0) {
                         tc_commit(smem_u32(&hd->empty[st]));
                         tc_commit_mc(smem_u32(&hd->p_empty[ps]), (uint16_t)1);
-                        if (last) {
-                            tc_commit(smem_u32(&hd->o_full));
-                            hd->event_code = -1;
-                            mbar_arrive(smem_u32(&hd->event));
-                        }
+                        if (last) tc_commit(smem_u32(&hd->o_full));
                     }
                     __syncwarp();
                     if (++st == kStages) {
@@ -799,7 +801,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int g = warp >> 2, h = threadIdx.x & 127;  // which half of the columns, head row
             const bool head = h < p.N1;
             const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-            uint32_t ofc = 0, ev = 0;
+            const uint32_t sw1 = (h & 7) << 4, sw2 = ((h >> 1) & 3) << 4;
+            uint32_t ofc = 0, pc = 0;
             for (uint32_t k = 0;; ++k) {
                 int u;
                 if (!tq_read(p, sy, rank, k, u)) goto done;
@@ -813,12 +816,40 @@ __global__ void __launch_bounds__(kThreads, 1)
                         for (int d = 0; d < kDv / 2; d += 8) *reinterpret_cast<uint4 *>(orow + d) = make_uint4(0, 0, 0, 0);
                     continue;
                 }
-                for (;;) {  // rescale requests, until the unit's last product is issued
-                    if (!wait_warp(sy, smem_u32(&hd->event), ev & 1)) goto done;
-                    ++ev;
-                    const int pc = hd->event_code;
-                    if (pc < 0) break;
-                    const float a = fabsf(reinterpret_cast<const float2 *>(msgs + (pc & 1) * kMsgBytes + kMsgStats)[h].x);
+                float fin = 1.f;
+                for (int j = it.j0; j < it.j1; ++j, ++pc) {
+                    const int ps = pc & 1;
+                    uint8_t *msg = msgs + ps * kMsgBytes;
+                    if (!wait_warp(sy, smem_u32(&hd->p_full[ps]), (pc >> 1) & 1, true)) goto done;
+                    const float2 stat = reinterpret_cast<const float2 *>(msg + kMsgStats)[h];
+                    const bool rescale = j > it.j0 && some_alpha(msg);
+                    fin = stat.y;
+                    if (g == ps) {  // this warp's tile: its 32 heads' weights into hi and lo codes, in place
+                        if (threadIdx.x == g * 128) mbar_arrive_expect_tx(smem_u32(&hd->p_full[ps]), kMsgBytes);  // the next message
+                        uint8_t *row1 = msg + h * 128, *row2 = msg + kMsgLo + h * 64;
+                        uint4 x[12], y[12];
+#pragma unroll
+                        for (int v = 0; v < 8; ++v) x[v] = *reinterpret_cast<const uint4 *>(row1 + ((v << 4) ^ sw1));
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) x[8 + v] = *reinterpret_cast<const uint4 *>(row2 + ((v << 4) ^ sw2));
+#pragma unroll
+                        for (int v = 0; v < 6; ++v) {
+                            split4h(x[2 * v].x, x[2 * v].y, y[v].x, y[6 + v].x);
+                            split4h(x[2 * v].z, x[2 * v].w, y[v].y, y[6 + v].y);
+                            split4h(x[2 * v + 1].x, x[2 * v + 1].y, y[v].z, y[6 + v].z);
+                            split4h(x[2 * v + 1].z, x[2 * v + 1].w, y[v].w, y[6 + v].w);
+                        }
+#pragma unroll
+                        for (int v = 0; v < 8; ++v) *reinterpret_cast<uint4 *>(row1 + ((v << 4) ^ sw1)) = y[v];
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) *reinterpret_cast<uint4 *>(row2 + ((v << 4) ^ sw2)) = y[8 + v];
+                        fence_proxy_async_smem();
+                    }
+                    // every warp, so that none reads the factors of a message that has been overwritten
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&hd->p_ready[ps]));
+                    if (!rescale) continue;
+                    const float a = fabsf(stat.x);
                     const bool any = __any_sync(0xffffffffu, a != 1.f);
 #pragma unroll 1
                     for (int c = 0; c < 2; ++c) {
@@ -851,7 +882,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!wait_warp(sy, smem_u32(&hd->o_full), ofc & 1)) goto done;
                 ++ofc;
                 tc_fence_after();
-                const float fin = hd->fin[h];
                 const uint32_t tcol = trow + g * (kDv / 2);
                 if (it.np == 1 && p.N1 % 32 == 0) {
                     // 32 columns at a time: each warp stages its 32 head rows (64-byte swizzle) and writes them
@@ -1014,6 +1044,8 @@ size_t fp8_tc_pieces(const SasFp8Args &a) { return (size_t)plan(a).P; }
 int launch_fp8_tc(const SasFp8Args &a, const Args &args, const Layout &L, char *ws, cudaStream_t s) {
     TcArgs p;
     static_cast<Args &>(p) = args;
+    p.ori_div = make_div((uint32_t)p.ori_bs);
+    p.cmp_div = make_div((uint32_t)p.cmp_bs);
     const Plan pl = plan(a);
     p.status = reinterpret_cast<uint32_t *>(p.rec + TR_STATUS);  // record 0 carries what no token is known for
     p.P = pl.P;
