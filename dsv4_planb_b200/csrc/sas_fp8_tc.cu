@@ -95,7 +95,7 @@ struct KeyConst {
 struct Hdr {
     uint64_t full[kStages], empty[kStages], s_full[2], s_free[2], q_raw, q_full, c_full[kConsts];
     uint64_t x_bar[4][2], m_bar[4][2], l_bar[4];  // of the two warps that share 32 heads
-    uint64_t p_full[2], p_ready[2], p_empty[2], o_full, o_empty, rs_done[2], pv_done[2];
+    uint64_t p_full[2], p_ready[2], p_empty[2], p_sent[2], o_full, o_empty, rs_done[2], pv_done[2];
     uint64_t tq_full[kTq], tq_empty[kTq];
     volatile int tq[kTq];
     uint32_t tmem_base;
@@ -143,22 +143,30 @@ __device__ __forceinline__ void mma8_ts(uint32_t d, uint32_t a_tmem, uint64_t b,
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d),
-        "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
 __device__ __forceinline__ void mma8_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
 // Instruction descriptor of kind::f8f6f4, both operands e4m3 (format 0), fp32 accumulation; b_mn: B is
 // N-major.
 __host__ __device__ constexpr uint32_t idesc_e4m3(uint32_t m, uint32_t n, uint32_t b_mn) {
     return (1u << 4) | (b_mn << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+        "[%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
@@ -169,9 +177,27 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
         : "memory");
 }
 
+// wait_warp with its polling loop out of line: the roles' loops share the instruction caches, and the
+// first try (which suspends the warp for a while) mostly succeeds.
+__device__ __noinline__ bool wait_long(const Sync &s, uint32_t bar, uint32_t parity, bool cluster_scope) {
+    return wait_warp(s, bar, parity, cluster_scope);
+}
+__device__ __forceinline__ bool wait_on(const Sync &s, uint32_t bar, uint32_t parity, bool cluster_scope = false) {
+    const bool done = cluster_scope ? mbar_try_cluster(bar, parity) : mbar_try(bar, parity);
+    return __all_sync(0xffffffffu, done) || wait_long(s, bar, parity, cluster_scope);
+}
+
 // Whether some row of O is to be rescaled before the message's product.
 __device__ __forceinline__ bool some_alpha(const uint8_t *msg) {
     return __any_sync(0xffffffffu, reinterpret_cast<const float2 *>(msg + kMsgStats)[(threadIdx.x & 3) * 32].x < 0.f);
+}
+
+// One lane of the warp, the same one each time.  The compiler takes what it runs as warp-uniform: with
+// `lane == 0` in its place an MMA of N 96 issued every 53 cycles instead of 48.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
 }
 
 struct Item {
@@ -283,7 +309,7 @@ __device__ void producer(const TcArgs &p, const Sync &sy, const CUtensorMap *q_m
             // raw Q of the token, three chunks of 64 dims per stage, 32 head rows at a time by TMA
             const int chunks = p.Dq / 64;
             for (int c = 0; c < chunks; c += kQPerStage, next()) {
-                if (!wait_warp(sy, smem_u32(&hd->empty[st]), phase)) return;
+                if (!wait_on(sy, smem_u32(&hd->empty[st]), phase)) return;
                 const uint32_t fb = smem_u32(&hd->full[st]);
                 if (lane == 0 && w * 32 < p.N1) {  // warp 0 takes the fourth 32 rows too
                     const int n = min(kQPerStage, chunks - c), groups = w == 0 && p.N1 > 96 ? 2 : 1;
@@ -315,10 +341,10 @@ __device__ void producer(const TcArgs &p, const Sync &sy, const CUtensorMap *q_m
                         pend = (int)ncluster_x() + atomicAdd(p.counter, 1);
                 }
             }
-            if (!wait_warp(sy, smem_u32(&hd->empty[st]), phase)) return;
+            if (!wait_on(sy, smem_u32(&hd->empty[st]), phase)) return;
             const uint32_t base = ring_at + st * kStageBytes;
             const uint64_t mine = reinterpret_cast<uint64_t>(key.row);
-#pragma unroll
+#pragma unroll 1  // short code: the roles of an SM share its instruction caches
             for (int k4 = 0; k4 < 8; ++k4) {
                 const uint64_t a = __shfl_sync(0xffffffffu, mine, 4 * k4 + (lane >> 3));
                 const uint8_t *src = reinterpret_cast<const uint8_t *>(a ? a : reinterpret_cast<uint64_t>(p.ori)) + src_off;
@@ -327,7 +353,7 @@ __device__ void producer(const TcArgs &p, const Sync &sy, const CUtensorMap *q_m
                 for (int c = 0; c < kVSlabs; ++c) cp_async16(dst + c * kSlab, src + c * 128, n);
             }
             if (tail) {
-#pragma unroll
+#pragma unroll 1
                 for (int r0 = 0; r0 < 32; r0 += 8) {
                     const int r = r0 + (lane >> 2);
                     const uint64_t a = __shfl_sync(0xffffffffu, mine, r);
@@ -406,7 +432,7 @@ __device__ float split_q(const Sync &sy, Hdr *hd, uint32_t trow, int chunks, uin
     hd->amax[g][h] = amax;
     __syncwarp();
     if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(&hd->x_bar[warp & 3][g]));
-    ok = wait_warp(sy, smem_u32(&hd->x_bar[warp & 3][g ^ 1]), parity);
+    ok = wait_on(sy, smem_u32(&hd->x_bar[warp & 3][g ^ 1]), parity);
     amax = fmaxf(amax, hd->amax[g ^ 1][h]);
     // largest element to [128, 256); rows of zeros and of the smallest subnormals: f = 2^126
     const int e = (int)(__float_as_uint(amax) >> 23) - 127;
@@ -488,6 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         init(hd->l_bar, 4, 1);
         init(hd->p_full, 2, 1);
         init(hd->p_empty, 2, 1);
+        init(hd->p_sent, 2, 1);
         init(hd->p_ready, 2, kSoftWarps);
         init(&hd->o_full, 1, 1);
         init(&hd->o_empty, 1, kSoftWarps);
@@ -509,7 +536,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     cluster_sync();  // both CTAs' barriers are initialised before any remote arrive
     tc_fence_after();
-    // a programmatic dependent of the resolve kernel: its records are visible after this wait
+    // a programmatic dependent of the resolve kernel: its records are visible after this wait.  q is older
+    // than that kernel: the first unit's comes into L2 meanwhile
+    if (rank == 0 && threadIdx.x == 32 * kProdWarp0 && first_unit(p) >= 0)
+        prefetch_l2_bulk(reinterpret_cast<const uint16_t *>(p.q) + (int64_t)(first_unit(p) % p.T) * p.N1 * p.Dq,
+                         (uint32_t)p.N1 * p.Dq * 2);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (p.P > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem = hd->tmem_base;
@@ -539,11 +570,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const Item it = load_unit(p, u);
                 if (it.skip || it.j1 <= it.j0) continue;
                 // raw Q -> TMEM, once the previous unit's last product has read the old one
-                if (sc > 0 && !wait_warp(sy, smem_u32(&hd->s_full[(sc - 1) & 1]), ((sc - 1) >> 1) & 1)) goto done;
+                if (sc > 0 && !wait_on(sy, smem_u32(&hd->s_full[(sc - 1) & 1]), ((sc - 1) >> 1) & 1)) goto done;
                 for (int c = 0; c < chunks; c += kQPerStage, next()) {
-                    if (!wait_warp(sy, smem_u32(&hd->full[st]), phase)) goto done;
+                    if (!wait_on(sy, smem_u32(&hd->full[st]), phase)) goto done;
                     tc_fence_after();
-                    if (lane == 0) {
+                    if (elect_one()) {
                         for (int e = 0; e < kQPerStage && c + e < chunks; ++e) {
                             const uint64_t d = sdesc_sw128(smem_u32(ring) + st * kKStage + e * kQChunk, 16, 1024);
                             for (int kq = 0; kq < 4; ++kq) tmem_cp_128x256b(tmem + ((c + e) * 4 + kq) * 8, d + 2 * kq);
@@ -553,20 +584,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     __syncwarp();
                 }
-                if (!wait_warp(sy, smem_u32(&hd->q_full), qc & 1)) goto done;
+                if (!wait_on(sy, smem_u32(&hd->q_full), qc & 1)) goto done;
                 ++qc;
                 for (int j = it.j0; j < it.j1; ++j, ++sc, next()) {
                     const int sb = sc & 1;
                     const uint32_t d = tmem + kTmemS + sb * kBK;
-                    if (!wait_warp(sy, smem_u32(&hd->s_free[sb]), ((sc >> 1) & 1) ^ 1)) goto done;
-                    if (!wait_warp(sy, smem_u32(&hd->full[st]), phase)) goto done;
+                    if (!wait_on(sy, smem_u32(&hd->s_free[sb]), ((sc >> 1) & 1) ^ 1)) goto done;
+                    if (!wait_on(sy, smem_u32(&hd->full[st]), phase)) goto done;
                     tc_fence_after();
                     fence_proxy_async_smem();  // the rows were written by cp.async
-                    if (lane == 0) {
+                    if (elect_one()) {
                         const uint32_t base = smem_u32(ring) + st * kKStage;
-#pragma unroll 1
+                        const uint64_t b0 = sdesc_sw128(base, 16, 1024);
+#pragma unroll
                         for (int c = 0; c < kVSlabs; ++c) {
-                            const uint64_t b = sdesc_sw128(base + c * kSlab, 16, 1024);
+                            const uint64_t b = b0 + c * (kSlab / 16);
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 const uint32_t a = tmem + c * 64 + (i >> 1) * 32 + (i & 1) * 8;
@@ -611,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     continue;
                 }
                 const int nt = it.j1 - it.j0;
-                if (!wait_warp(sy, smem_u32(&hd->q_raw), qc & 1)) goto done;
+                if (!wait_on(sy, smem_u32(&hd->q_raw), qc & 1)) goto done;
                 tc_fence_after();
                 bool ok;
                 const float rq = p.scale_log2 / split_q(sy, hd, trow, p.Dq / 64, qc & 1, ok);
@@ -624,18 +656,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                 float m = -INFINITY, l = 0.f;  // of this thread's tiles, l in the frame of m
                 for (int e = (sc0 & 1) == (uint32_t)g ? 0 : 1; e < nt; e += 2, ++mine) {
                     const uint32_t sc = sc0 + e;
-                    if (!wait_warp(sy, smem_u32(&hd->c_full[sc % kConsts]), (sc / kConsts) & 1)) goto done;
-                    if (!wait_warp(sy, smem_u32(&hd->s_full[g]), mine & 1)) goto done;
+                    if (!wait_on(sy, smem_u32(&hd->c_full[sc % kConsts]), (sc / kConsts) & 1)) goto done;
+                    if (!wait_on(sy, smem_u32(&hd->s_full[g]), mine & 1)) goto done;
                     tc_fence_after();
                     const KeyConst &c = consts[sc % kConsts];
                     float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll 1
-                    for (int i0 = 0; i0 < kBK; i0 += 32) {
-                        uint32_t sr[32];
-                        tmem_ld32(s_at + i0, sr);
+                    for (int i0 = 0; i0 < kBK; i0 += 16) {
+                        uint32_t sr[16];
+                        tmem_ld16(s_at + i0, sr);
                         tc_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
+                        for (int i = 0; i < 16; i += 4) {
                             const ulonglong2 s4 = *reinterpret_cast<const ulonglong2 *>(&c.s[i0 + i]);
                             const ulonglong2 l4 = *reinterpret_cast<const ulonglong2 *>(&c.ls[i0 + i]);
                             const float2 a = unpack2(fma2(mul2(pack2(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1])), rq2), s4.x, l4.x));
@@ -647,7 +679,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const float mx = fmaxf(mx0, mx1);
                     // the maximum so far comes from the other warp's tile and goes on to its next
                     float mn = mx, alpha = 1.f;
-                    if (sc > 0 && !wait_warp(sy, smem_u32(&hd->m_bar[warp & 3][g ^ 1]), ((sc - 1) >> 1) & 1)) goto done;
+                    if (sc > 0 && !wait_on(sy, smem_u32(&hd->m_bar[warp & 3][g ^ 1]), ((sc - 1) >> 1) & 1)) goto done;
                     if (e > 0) {
                         const float before = hd->m[g ^ 1][h];
                         mn = mx > before + kRise ? mx : before;
@@ -662,24 +694,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     const float mb = m - (kTop - kRise);
                     const uint64_t mb2 = pack2(-mb, -mb);
-                    // the slot was read by the peer, so its copies have left the staging buffer
-                    if (!wait_warp(sy, smem_u32(&hd->p_empty[g]), (mine & 1) ^ 1, true)) goto done;
+                    // the last message has arrived, so its copies have left the staging buffer
+                    if (!wait_on(sy, smem_u32(&hd->p_sent[g]), (mine & 1) ^ 1, true)) goto done;
                     uint64_t sum0 = 0, sum1 = 0;
                     const int live = it.rec[TR_NORI] + it.rec[TR_NCMP] - (it.j0 + e) * kBK;
 #pragma unroll 1
-                    for (int i0 = 0; i0 < kBK; i0 += 32) {
-                        uint32_t sr[32], hp[16];
-                        tmem_ld32(s_at + i0, sr);
+                    for (int i0 = 0; i0 < kBK; i0 += 16) {
+                        uint32_t sr[16], hp[8];
+                        tmem_ld16(s_at + i0, sr);
                         tc_wait_ld();
                         uint64_t f2 = rq2;
-                        if (live - i0 < 32) {  // slots without a key, in the token's last tile: weight 0
+                        if (live - i0 < 16) {  // slots without a key, in the token's last tile: weight 0
                             f2 = pack2(1.f, 1.f);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i)
+                            for (int i = 0; i < 16; ++i)
                                 sr[i] = __float_as_uint(i < live - i0 ? __uint_as_float(sr[i]) * rq : -INFINITY);
                         }
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
+                        for (int i = 0; i < 16; i += 4) {
                             const ulonglong2 s4 = *reinterpret_cast<const ulonglong2 *>(&c.s[i0 + i]);
                             const float2 a = unpack2(fma2(mul2(pack2(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1])), f2), s4.x, mb2));
                             const float2 b = unpack2(fma2(mul2(pack2(__uint_as_float(sr[i + 2]), __uint_as_float(sr[i + 3])), f2), s4.y, mb2));
@@ -690,10 +722,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                             hp[i >> 1] = pack_half(p0.x, p0.y);
                             hp[(i >> 1) + 1] = pack_half(p1.x, p1.y);
                         }
-                        // keys 0 .. 63 in the 128-byte row, 64 .. 95 in the 64-byte row, 8 keys a granule
-                        const uint32_t row = i0 == 64 ? row2 : row1 + ((i0 << 1) ^ (sw1 & 0x40)), sw = i0 == 64 ? sw2 : sw1 & 0x30;
+                        // 8 keys a granule; keys 0 .. 63 in the 128-byte row, 64 .. 95 in the 64-byte row
+                        const uint32_t row = i0 < 64 ? row1 + ((2 * i0) ^ (sw1 & 0x60)) : row2 + ((2 * i0 - 128) ^ (sw2 & 0x20));
+                        const uint32_t sw = (i0 < 64 ? sw1 : sw2) & 0x10;
 #pragma unroll
-                        for (int v = 0; v < 4; ++v)
+                        for (int v = 0; v < 2; ++v)
                             st_shared_v4(row + ((v << 4) ^ sw), hp[4 * v], hp[4 * v + 1], hp[4 * v + 2], hp[4 * v + 3]);
                     }
                     tc_fence_before();
@@ -710,7 +743,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     } else if (e == nt - 1) {
                         float total = l;
                         if (nt > 1) {
-                            if (!wait_warp(sy, smem_u32(&hd->l_bar[warp & 3]), lc & 1)) goto done;
+                            if (!wait_on(sy, smem_u32(&hd->l_bar[warp & 3]), lc & 1)) goto done;
                             const float other = hd->l[lc & 1][0][h], frame = hd->l[lc & 1][1][h];
                             total += frame == m ? other : other * exp2f(frame - m);
                         }
@@ -729,7 +762,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const bool some = __any_sync(0xffffffffu, alpha != 1.f);
                     *reinterpret_cast<float2 *>(stage + kMsgStats + h * 8) = make_float2(lane == 0 && some ? -alpha : alpha, fin);
                     fence_proxy_async_smem();
-                    __syncwarp();
+                    // only now must the peer be done with the slot: S has been free since the second pass
+                    if (!wait_on(sy, smem_u32(&hd->p_empty[g]), (mine & 1) ^ 1, true)) goto done;
                     if (lane == 0) {
                         const uint32_t w32 = (warp & 3) * 32, src = smem_u32(stage);
                         bulk_to_peer(peer_msg + w32 * 128, src + w32 * 128, 32 * 128, peer_full);
@@ -741,7 +775,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (nt > 1) ++lc;
             }
             // the last message must have been read before this CTA may exit
-            if (mine > 0 && !wait_warp(sy, smem_u32(&hd->p_empty[g]), (mine - 1) & 1, true)) goto done;
+            if (mine > 0 && !wait_on(sy, smem_u32(&hd->p_empty[g]), (mine - 1) & 1, true)) goto done;
         }
     } else {
         // ======================= output CTA =======================
@@ -757,22 +791,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (u < 0) break;
                 const Item it = load_unit(p, u);
                 if (it.skip || it.j1 <= it.j0) continue;
-                if (!wait_warp(sy, smem_u32(&hd->o_empty), (oc & 1) ^ 1)) goto done;
+                if (!wait_on(sy, smem_u32(&hd->o_empty), (oc & 1) ^ 1)) goto done;
                 ++oc;
                 for (int j = it.j0; j < it.j1; ++j, ++pc) {
                     const int ps = pc & 1;
-                    if (!wait_warp(sy, smem_u32(&hd->p_ready[ps]), (pc >> 1) & 1)) goto done;
+                    if (!wait_on(sy, smem_u32(&hd->p_ready[ps]), (pc >> 1) & 1)) goto done;
                     const uint8_t *msg = msgs + ps * kMsgBytes;
                     const bool last = j == it.j1 - 1, rescale = j > it.j0 && some_alpha(msg);
-                    if (!wait_warp(sy, smem_u32(&hd->full[st]), phase)) goto done;
+                    if (!wait_on(sy, smem_u32(&hd->full[st]), phase)) goto done;
                     fence_proxy_async_smem();  // the rows were written by cp.async
                     const uint64_t a1 = sdesc_sw128(smem_u32(msg), 16, 1024), a2 = sdesc_sw64(smem_u32(msg) + kMsgLo);
                     const uint32_t base = smem_u32(ring) + st * kVStage;
 #pragma unroll 1
                     for (int c = 0; c < 2; ++c) {  // 256 value dims each
-                        if (rescale && !wait_warp(sy, smem_u32(&hd->rs_done[c]), rsc & 1)) goto done;
+                        if (rescale && !wait_on(sy, smem_u32(&hd->rs_done[c]), rsc & 1)) goto done;
                         tc_fence_after();
-                        if (lane == 0) {
+                        if (elect_one()) {
                             const uint64_t b = sdesc_sw128(base + c * 2 * kSlab, kSlab, 1024);
                             const uint32_t d = tmem + c * 256;
 #pragma unroll
@@ -785,7 +819,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         __syncwarp();
                     }
                     if (rescale) ++rsc;
-                    if (lane == 0) {
+                    if (elect_one()) {
                         tc_commit(smem_u32(&hd->empty[st]));
                         tc_commit_mc(smem_u32(&hd->p_empty[ps]), (uint16_t)1);
                         if (last) tc_commit(smem_u32(&hd->o_full));
@@ -820,12 +854,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int j = it.j0; j < it.j1; ++j, ++pc) {
                     const int ps = pc & 1;
                     uint8_t *msg = msgs + ps * kMsgBytes;
-                    if (!wait_warp(sy, smem_u32(&hd->p_full[ps]), (pc >> 1) & 1, true)) goto done;
+                    if (!wait_on(sy, smem_u32(&hd->p_full[ps]), (pc >> 1) & 1, true)) goto done;
                     const float2 stat = reinterpret_cast<const float2 *>(msg + kMsgStats)[h];
                     const bool rescale = j > it.j0 && some_alpha(msg);
                     fin = stat.y;
                     if (g == ps) {  // this warp's tile: its 32 heads' weights into hi and lo codes, in place
-                        if (threadIdx.x == g * 128) mbar_arrive_expect_tx(smem_u32(&hd->p_full[ps]), kMsgBytes);  // the next message
+                        if (threadIdx.x == g * 128) {
+                            mbar_arrive_expect_tx(smem_u32(&hd->p_full[ps]), kMsgBytes);  // the next message
+                            mbar_arrive_remote(map_to_cta(smem_u32(&hd->p_sent[ps]), 0));
+                        }
                         uint8_t *row1 = msg + h * 128, *row2 = msg + kMsgLo + h * 64;
                         uint4 x[12], y[12];
 #pragma unroll
@@ -854,7 +891,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
                     for (int c = 0; c < 2; ++c) {
                         // the product of the tile before, of these columns
-                        if (!wait_warp(sy, smem_u32(&hd->pv_done[c]), (pc - 1) & 1)) goto done;
+                        if (!wait_on(sy, smem_u32(&hd->pv_done[c]), (pc - 1) & 1)) goto done;
                         if (any) {
                             tc_fence_after();
 #pragma unroll 1
@@ -879,7 +916,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (lane == 0) mbar_arrive(smem_u32(&hd->rs_done[c]));
                     }
                 }
-                if (!wait_warp(sy, smem_u32(&hd->o_full), ofc & 1)) goto done;
+                if (!wait_on(sy, smem_u32(&hd->o_full), ofc & 1)) goto done;
                 ++ofc;
                 tc_fence_after();
                 const uint32_t tcol = trow + g * (kDv / 2);
@@ -960,31 +997,49 @@ done:
 
 // Pieces of split tokens, and the sink: out = sum_i 2^(own_i - lse2) o_i with o_i normalised within its
 // piece and own_i the log2 of the piece's weight sum; lse2 = log2 (sum_i 2^own_i + 2^sink2).
-// Block (t, h), thread = 4 columns.
+// Block (t, h), thread = 4 columns.  Latency bound: the record, the sums and the first pieces' columns
+// are loaded together, before the number of pieces is known (the slots of all P exist).
 __global__ void __launch_bounds__(kDv / 4) fp8_combine_kernel(const TcArgs p) {
-    __shared__ float w_s[kMaxPieces];
+    constexpr int kAhead = 8;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
-    const int np = load_unit(p, t).np;
-    if (np == 1) return;  // written by the attention kernel
+    const int t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
     const int64_t s0 = (int64_t)t * p.P;
-    const float own = tid < np ? __ldcg(p.part_s + (s0 + tid) * p.N1 + h) : -INFINITY;
-    if (tid < kMaxPieces) w_s[tid] = own;
-    __syncthreads();
-    float lse2 = p.sinks ? p.sinks[h] * 1.4426950408889634f : -INFINITY;
-    for (int i = 0; i < np; ++i) lse2 = log2_add(lse2, w_s[i]);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     const float4 *po = reinterpret_cast<const float4 *>(p.part_o + (s0 * p.N1 + h) * kDv) + tid;
     const int64_t stride = (int64_t)p.N1 * kDv / 4;
-#pragma unroll 8
-    for (int i = 0; i < np; ++i) {
-        const float4 o = __ldcg(po + i * stride);
-        const float w = exp2f(w_s[i] - lse2);
-        acc.x = fmaf(w, o.x, acc.x);
-        acc.y = fmaf(w, o.y, acc.y);
-        acc.z = fmaf(w, o.z, acc.z);
-        acc.w = fmaf(w, o.w, acc.w);
-    }
+    float4 o[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+        if (i < p.P) o[i] = __ldcg(po + i * stride);
+    // every warp holds the sums of all pieces, two a lane
+    const float r0 = lane < p.P ? __ldcg(p.part_s + (s0 + lane) * p.N1 + h) : -INFINITY;
+    const float r1 = lane + 32 < p.P ? __ldcg(p.part_s + (s0 + lane + 32) * p.N1 + h) : -INFINITY;
+    const float sink = p.sinks ? __ldg(p.sinks + h) * 1.4426950408889634f : -INFINITY;
+    const int np = load_unit(p, t).np;
+    if (np == 1) return;  // written by the attention kernel
+    const float own0 = lane < np ? r0 : -INFINITY, own1 = lane + 32 < np ? r1 : -INFINITY;
+    const bool bad = __any_sync(0xffffffffu, own0 != own0 || own1 != own1);
+    float top = fmaxf(fmaxf(own0, own1), sink);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    // pieces always hold a key, so that their sums are finite unless something is NaN
+    float sum = exp2f(own0 - top) + exp2f(own1 - top);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    const float lse2 = bad ? NAN : top == INFINITY ? top : top + log2f(sum + exp2f(sink - top));
+    const float w0 = exp2f(own0 - lse2), w1 = exp2f(own1 - lse2);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](int i, const float4 &v) {
+        const float w = __shfl_sync(0xffffffffu, i < 32 ? w0 : w1, i & 31);
+        acc.x = fmaf(w, v.x, acc.x);
+        acc.y = fmaf(w, v.y, acc.y);
+        acc.z = fmaf(w, v.z, acc.z);
+        acc.w = fmaf(w, v.w, acc.w);
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+        if (i < np) add(i, o[i]);
+#pragma unroll 4
+    for (int i = kAhead; i < np; ++i) add(i, __ldcg(po + i * stride));
     uint2 *out = reinterpret_cast<uint2 *>(reinterpret_cast<__nv_bfloat16 *>(p.out) + ((int64_t)t * p.N1 + h) * kDv) + tid;
     *out = make_uint2(pack_bf16(acc.x, acc.y), pack_bf16(acc.z, acc.w));
     if (p.lse && tid == 0) p.lse[(int64_t)t * p.N1 + h] = lse2 * 0.6931471805599453f;
@@ -1007,7 +1062,7 @@ int make_map(CUtensorMap *map, const void *base, int64_t rows, int D, uint32_t c
 }
 
 constexpr int kClusters = 74;  // 148 SMs / 2
-constexpr int kMinPieceTiles = 3;
+constexpr int kMinPieceTiles = 1;
 constexpr int64_t kMaxPartialBytes = int64_t(1) << 30;
 
 struct Plan {
