@@ -20,7 +20,7 @@
 //   CTA 0 ("score")                              CTA 1 ("output")
 //   TMEM: Q hi / lo (D_qk / 2 columns),          TMEM: O (128 x 512 fp32)
 //         S (2 x 96 columns)
-//   3 warps gather 96 key rows per tile          3 warps gather the first 512 bytes of the rows
+//   4 warps gather 96 key rows per tile          4 warps gather the first 512 bytes of the rows
 //           (cp.async into the MMA's swizzle)
 //   1 warp  S = Q K^T: 2 MMAs (hi, lo) of M 128, 1 warp  O += P V: 2 (hi, lo) per 32 keys and 256
 //           N 96, K 32 per 32 dims                       value dims; V is the N-major B operand, the
@@ -69,8 +69,9 @@ constexpr int kStages = 3;
 constexpr int kDv = 512, kVSlabs = kDv / 128;
 constexpr int kVStage = kVSlabs * kSlab, kKStage = kVStage + kBK * 64;  // K: dims 512 .. 575 as 64-byte rows behind
 constexpr int kQChunk = 128 * 128, kQPerStage = 3;  // raw Q: 64 bf16 dims of 128 heads; chunks per stage of the K ring
-constexpr int kSoftWarps = 8, kMmaWarp = 8, kProdWarp0 = 9, kProdWarps = 3;  // 12 warps: 168 registers a thread
-static_assert(kBK == 32 * kProdWarps, "a lane per key slot");
+constexpr int kSoftWarps = 8, kMmaWarp = 8, kProdWarp0 = 9, kProdWarps = 4;
+constexpr int kRows = kBK / kProdWarps;
+static_assert(kRows % 8 == 0 && kProdWarps == 4, "whole swizzle periods, 32 heads of Q a warp");
 constexpr int kThreads = 32 * (kProdWarp0 + kProdWarps);
 constexpr uint32_t kReaders = 2 * (kSoftWarps + 1 + kProdWarps) - 1;  // of the unit queue: every warp but its writer
 constexpr int kTmemCols = 512, kTmemS = 320;
@@ -266,11 +267,14 @@ __device__ __forceinline__ Key key_row(const TcArgs &p, const Item &it, int i, i
     return key;
 }
 
+// The kernel is a programmatic dependent of the resolve kernel: its records are visible after this wait.
+__device__ __forceinline__ void wait_resolved() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32_t bytes) {  // bytes 0: zeros
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
-// The gather warps.  Each takes 32 of a tile's 96 key slots (a lane per slot) and copies their rows with
+// The gather warps.  Each takes 24 of a tile's 96 key slots (a lane per slot) and copies their rows with
 // 16-byte cp.async: an instruction moves 128 bytes of 4 rows (row r of a slab at r * 128, granule g at
 // g ^ r % 8: the MMA's 128-byte swizzle); dims 512 .. 575 go to 64-byte rows (granule g at g ^ r / 2 % 4:
 // the 64-byte swizzle), 8 rows per instruction.  Row addresses go from lane to lane once per 4 rows.  A
@@ -280,12 +284,14 @@ template <bool kScore>
 __device__ void producer(const TcArgs &p, const Sync &sy, const CUtensorMap *q_map, uint8_t *ring, Hdr *hd,
                          KeyConst *consts) {
     constexpr uint32_t kStageBytes = kScore ? kKStage : kVStage;
-    const int w = (threadIdx.x >> 5) - kProdWarp0, lane = threadIdx.x & 31, key_at = w * 32 + lane;
+    const int w = (threadIdx.x >> 5) - kProdWarp0, lane = threadIdx.x & 31;
+    const bool holds = lane < kRows;
+    const int key_at = w * kRows + (holds ? lane : 0);
     const bool writer = kScore && w == 0;
     const bool tail = kScore && p.Dq > 512;
     const uint32_t ring_at = smem_u32(ring);
     // this lane's granule lane % 8 of row 4 k + lane / 8: offsets for even k, and what odd k change
-    const uint32_t dst0 = key_at / 32 * 4096 + (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4);
+    const uint32_t dst0 = w * kRows * 128 + (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4);
     const uint32_t src_off = (lane & 7) * 16;
     uint32_t st = 0, phase = 1, tiles = 0, bits = 0;  // stage, and the parity its empty barrier is waited on
     int pend = -1;
@@ -295,57 +301,49 @@ __device__ void producer(const TcArgs &p, const Sync &sy, const CUtensorMap *q_m
             phase ^= 1;
         }
     };
+    // raw Q of a token, three chunks of 64 dims per stage, 32 head rows per warp by TMA
+    auto load_q = [&](int t) {
+        const int chunks = p.Dq / 64;
+        for (int c = 0; c < chunks; c += kQPerStage, next()) {
+            if (!wait_on(sy, smem_u32(&hd->empty[st]), phase)) return false;
+            const uint32_t fb = smem_u32(&hd->full[st]);
+            if (lane == 0 && w * 32 < p.N1) {
+                const int n = min(kQPerStage, chunks - c);
+                mbar_arrive_expect_tx(fb, n * 4096);
+                for (int e = 0; e < n; ++e)
+                    tma_load_2d(ring_at + st * kStageBytes + e * kQChunk + w * 4096, q_map, (c + e) * 64, t * p.N1 + w * 32,
+                                fb);
+            } else {
+                mbar_arrive(fb);  // rows of no head: whatever lies there
+            }
+        }
+        return true;
+    };
     for (uint32_t k = 0;; ++k) {
         int u = -1;
         if (!(writer ? tq_publish(p, sy, k, pend, u) : tq_read(p, sy, kScore ? 0 : 1, k, u))) return;
         if (u < 0) break;
+        // q is older than the resolve kernel: the first unit's is loaded beside it, whatever the unit holds
+        if (kScore && k == 0 && !load_q(u % p.T)) return;
+        if (k == 0) wait_resolved();
         const Item it = load_unit(p, u);
         if (it.skip || it.j1 <= it.j0) continue;
         const int end = it.j1 * kBK;
         int i = it.j0 * kBK + key_at;
         const int32_t f0 = key_fetch(p, it, i);
         int32_t fetched = i + kBK < end ? key_fetch(p, it, i + kBK) : -1;
-        if constexpr (kScore) {
-            // raw Q of the token, three chunks of 64 dims per stage, 32 head rows at a time by TMA
-            const int chunks = p.Dq / 64;
-            for (int c = 0; c < chunks; c += kQPerStage, next()) {
-                if (!wait_on(sy, smem_u32(&hd->empty[st]), phase)) return;
-                const uint32_t fb = smem_u32(&hd->full[st]);
-                if (lane == 0 && w * 32 < p.N1) {  // warp 0 takes the fourth 32 rows too
-                    const int n = min(kQPerStage, chunks - c), groups = w == 0 && p.N1 > 96 ? 2 : 1;
-                    mbar_arrive_expect_tx(fb, n * groups * 4096);
-                    for (int g = w; g < w + 3 * groups; g += 3)
-                        for (int e = 0; e < n; ++e)
-                            tma_load_2d(ring_at + st * kStageBytes + e * kQChunk + g * 4096, q_map, (c + e) * 64,
-                                        it.t * p.N1 + g * 32, fb);
-                } else {
-                    mbar_arrive(fb);  // rows of no head: whatever lies there
-                }
-            }
-        }
+        if (kScore && k > 0 && !load_q(it.t)) return;
         Key key = key_row(p, it, i, f0, bits);  // behind Q's loads, which need no lookup
         for (int j = it.j0; j < it.j1; ++j, i += kBK, ++tiles, next()) {
             if (key.row != nullptr && !scale_ok(key.s)) {
                 bits |= SAS_STATUS_BAD_SCALE;
                 key.row = nullptr;
             }
-            if constexpr (kScore) {
-                KeyConst &c = consts[tiles % kConsts];
-                const bool row = key.row != nullptr;
-                c.s[key_at] = row ? key.s : key.live ? 0.f : 1.f;
-                c.ls[key_at] = row ? log2f(key.s) : key.live ? -60.f : -INFINITY;
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(smem_u32(&hd->c_full[tiles % kConsts]));
-                    if (writer && j == (it.j1 - it.j0 > 1 ? it.j1 - 2 : it.j0))
-                        pend = (int)ncluster_x() + atomicAdd(p.counter, 1);
-                }
-            }
             if (!wait_on(sy, smem_u32(&hd->empty[st]), phase)) return;
             const uint32_t base = ring_at + st * kStageBytes;
             const uint64_t mine = reinterpret_cast<uint64_t>(key.row);
 #pragma unroll 1  // short code: the roles of an SM share its instruction caches
-            for (int k4 = 0; k4 < 8; ++k4) {
+            for (int k4 = 0; k4 < kRows / 4; ++k4) {
                 const uint64_t a = __shfl_sync(0xffffffffu, mine, 4 * k4 + (lane >> 3));
                 const uint8_t *src = reinterpret_cast<const uint8_t *>(a ? a : reinterpret_cast<uint64_t>(p.ori)) + src_off;
                 const uint32_t n = a ? 16 : 0, dst = base + (dst0 ^ ((k4 & 1) << 6)) + k4 * 512;
@@ -354,14 +352,28 @@ __device__ void producer(const TcArgs &p, const Sync &sy, const CUtensorMap *q_m
             }
             if (tail) {
 #pragma unroll 1
-                for (int r0 = 0; r0 < 32; r0 += 8) {
+                for (int r0 = 0; r0 < kRows; r0 += 8) {
                     const int r = r0 + (lane >> 2);
                     const uint64_t a = __shfl_sync(0xffffffffu, mine, r);
-                    cp_async16(base + kVStage + (w * 32 + r) * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4),
+                    cp_async16(base + kVStage + (w * kRows + r) * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4),
                                a ? reinterpret_cast<const uint8_t *>(a) + 512 + (lane & 3) * 16 : p.ori, a ? 16 : 0);
                 }
             }
             asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&hd->full[st])) : "memory");
+            if constexpr (kScore) {
+                KeyConst &c = consts[tiles % kConsts];
+                const bool row = key.row != nullptr;
+                if (holds) {  // ls decides on the frame only, so that an approximation does
+                    c.s[key_at] = row ? key.s : key.live ? 0.f : 1.f;
+                    c.ls[key_at] = row ? __log2f(key.s) : key.live ? -60.f : -INFINITY;
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(smem_u32(&hd->c_full[tiles % kConsts]));
+                    if (writer && j == (it.j1 - it.j0 > 1 ? it.j1 - 2 : it.j0))
+                        pend = (int)ncluster_x() + atomicAdd(p.counter, 1);
+                }
+            }
             key = Key{nullptr, 1.f, false};  // the next tile's lookups, behind the copies
             if (i + kBK < end) key = key_row(p, it, i + kBK, fetched, bits);
             fetched = i + 2 * kBK < end ? key_fetch(p, it, i + 2 * kBK) : -1;
@@ -536,12 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     cluster_sync();  // both CTAs' barriers are initialised before any remote arrive
     tc_fence_after();
-    // a programmatic dependent of the resolve kernel: its records are visible after this wait.  q is older
-    // than that kernel: the first unit's comes into L2 meanwhile
-    if (rank == 0 && threadIdx.x == 32 * kProdWarp0 && first_unit(p) >= 0)
-        prefetch_l2_bulk(reinterpret_cast<const uint16_t *>(p.q) + (int64_t)(first_unit(p) % p.T) * p.N1 * p.Dq,
-                         (uint32_t)p.N1 * p.Dq * 2);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (warp < kProdWarp0) wait_resolved();  // the gather warps wait later
     if (p.P > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem = hd->tmem_base;
     Sync sy{&hd->abort, p.status, map_to_cta(smem_u32((const void *)&hd->abort), rank ^ 1u), hd->tq_full, hd->tq_empty,
@@ -568,7 +575,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!tq_read(p, sy, rank, k, u)) goto done;
                 if (u < 0) break;
                 const Item it = load_unit(p, u);
-                if (it.skip || it.j1 <= it.j0) continue;
+                if (it.skip || it.j1 <= it.j0) {
+                    // the first unit's Q has been loaded all the same
+                    for (int c = 0; k == 0 && c < chunks; c += kQPerStage, next()) {
+                        if (!wait_on(sy, smem_u32(&hd->full[st]), phase)) goto done;
+                        if (elect_one()) mbar_arrive(smem_u32(&hd->empty[st]));
+                        __syncwarp();
+                    }
+                    continue;
+                }
                 // raw Q -> TMEM, once the previous unit's last product has read the old one
                 if (sc > 0 && !wait_on(sy, smem_u32(&hd->s_full[(sc - 1) & 1]), ((sc - 1) >> 1) & 1)) goto done;
                 for (int c = 0; c < chunks; c += kQPerStage, next()) {
