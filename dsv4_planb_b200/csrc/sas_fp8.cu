@@ -192,9 +192,9 @@ Layout layout_of(const SasFp8Args &a) {
     L.rec = take(sizeof(int32_t) * TR_INTS * T);
     L.rows = take(a.scenario == 3 ? sizeof(int32_t) * (size_t)a.topk * T : 0);
     const size_t P = use_tc(a) ? sas_host::fp8_tc_pieces(a) : 1;
-    const size_t slots = P > 1 ? T * P * (size_t)a.num_heads : 0;
-    L.part_o = take(slots * (size_t)a.v_head_dim * sizeof(float));
-    L.part_s = take(slots * sizeof(float));
+    const size_t slots = P > 1 ? T * P : 0, N1 = (size_t)a.num_heads;
+    L.part_o = take(slots * ((N1 + 31) / 32 * 32) * (size_t)a.v_head_dim * sizeof(float));
+    L.part_s = take(slots * N1 * sizeof(float));
     L.total = off;
     return L;
 }

@@ -25,7 +25,7 @@ struct Layout {
     size_t head;   // status word (for sas_kvq_read_status) and the unit counter
     size_t rec;    // int32 [T][TR_INTS]
     size_t rows;   // int32 [T][topk]: physical compressed rows (scenario 3), -1: a zero row
-    size_t part_o; // split tokens: fp32 [T][P][N1][Dv]
+    size_t part_o; // split tokens: fp32 [T][P][N1 rounded up to 32][Dv]
     size_t part_s; // split tokens: fp32 [T][P][N1]: log2 of the piece's weight sum
     size_t total;
 };

@@ -111,7 +111,7 @@ constexpr int kScoreRing = kScoreMsgs + 2 * kMsgBytes;
 constexpr int kScoreSmem = kScoreRing + kStages * kKStage;
 constexpr int kOutRing = kHdr;
 constexpr int kOutMsgs = kOutRing + kStages * kVStage;
-constexpr int kOutStage = kOutMsgs + 2 * kMsgBytes;  // epilogue staging: 32 columns of 32 heads per warp
+constexpr int kOutStage = kOutMsgs + 2 * kMsgBytes;  // epilogue staging: 64 bytes of 32 heads per warp
 constexpr int kWarpSlab = 32 * 64;
 constexpr int kOutSmem = kOutStage + kSoftWarps * kWarpSlab;
 constexpr int kSmemBytes = (kScoreSmem > kOutSmem ? kScoreSmem : kOutSmem) + 1024;  // + alignment slack
@@ -137,6 +137,7 @@ struct TcArgs : Args {
     Div ori_div, cmp_div;    // by the block sizes
     uint32_t *status;
     int U, P, M;             // units; pieces per token, tiles per piece (P = 1: whole tokens)
+    int NP;                  // rows of a slot of part_o: N1 rounded up to 32
     float *part_o, *part_s;
 };
 
@@ -503,7 +504,8 @@ __device__ __forceinline__ uint64_t sdesc_sw64(uint32_t saddr) {
 }
 
 __global__ void __launch_bounds__(kThreads, 1)
-    fp8_tc_kernel(const TcArgs p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap out_map) {
+    fp8_tc_kernel(const TcArgs p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap out_map,
+                  const __grid_constant__ CUtensorMap part_map) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
     Hdr *hd = reinterpret_cast<Hdr *>(smem);
@@ -935,57 +937,55 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ++ofc;
                 tc_fence_after();
                 const uint32_t tcol = trow + g * (kDv / 2);
-                if (it.np == 1 && p.N1 % 32 == 0) {
-                    // 32 columns at a time: each warp stages its 32 head rows (64-byte swizzle) and writes them
-                    // with one TMA store
-                    if ((warp & 3) * 32 < p.N1) {
-                        const uint32_t buf = smem_u32(smem + kOutStage) + warp * kWarpSlab;
+                // Each warp stages 64 bytes of its 32 head rows (64-byte swizzle) and writes them out: one TMA
+                // store, or 64-byte pieces of rows where a box would reach into the next token's heads.  Whole
+                // tokens in bf16, pieces in fp32, normalised within the piece.  (Direct stores, 16 bytes a lane
+                // to 32 rows, took 9.5 us for a piece.)
+                if ((warp & 3) * 32 < p.N1) {
+                    const uint32_t buf = smem_u32(smem + kOutStage) + warp * kWarpSlab;
+                    const bool piece = it.np > 1;
+                    const int row = piece ? ((it.t * p.P + it.piece) * p.NP + (warp & 3) * 32) : it.t * p.N1 + (warp & 3) * 32;
+                    const int step = piece ? 16 : 32;
 #pragma unroll 1
-                        for (int c = 0; c < kDv / 2; c += 32) {
-                            uint32_t r[32];
-                            tmem_ld32(tcol + c, r);
-                            if (lane == 0) bulk_wait_read<0>();  // the last store has read buf
-                            __syncwarp();
-                            tc_wait_ld();
+                    for (int c = 0; c < kDv / 2; c += step) {
+                        uint32_t r[32], w[16];
+                        tmem_ld32(tcol + (c & ~31), r);
+                        if (lane == 0) bulk_wait_read<0>();  // the last store has read buf
+                        __syncwarp();
+                        tc_wait_ld();
+                        if (piece) {
 #pragma unroll
-                            for (int cc = 0; cc < 4; ++cc) {
-                                uint32_t w[4];
+                            for (int i = 0; i < 16; ++i)
+                                w[i] = __float_as_uint(__uint_as_float(c & 16 ? r[16 + i] : r[i]) * fin);
+                        } else {
 #pragma unroll
-                                for (int e = 0; e < 4; ++e)
-                                    w[e] = pack_bf16(__uint_as_float(r[8 * cc + 2 * e]) * fin, __uint_as_float(r[8 * cc + 2 * e + 1]) * fin);
-                                st_shared_v4(buf + lane * 64 + ((cc ^ ((lane >> 1) & 3)) << 4), w[0], w[1], w[2], w[3]);
-                            }
+                            for (int i = 0; i < 16; ++i)
+                                w[i] = pack_bf16(__uint_as_float(r[2 * i]) * fin, __uint_as_float(r[2 * i + 1]) * fin);
+                        }
+#pragma unroll
+                        for (int cc = 0; cc < 4; ++cc)
+                            st_shared_v4(buf + lane * 64 + ((cc ^ ((lane >> 1) & 3)) << 4), w[4 * cc], w[4 * cc + 1], w[4 * cc + 2],
+                                         w[4 * cc + 3]);
+                        if (piece || p.N1 % 32 == 0) {
                             fence_proxy_async_smem();
                             __syncwarp();
                             if (lane == 0) {
-                                tma_store_2d(&out_map, buf, g * (kDv / 2) + c, it.t * p.N1 + (warp & 3) * 32);
+                                tma_store_2d(piece ? &part_map : &out_map, buf, g * (kDv / 2) + c, row);
                                 bulk_commit();
                             }
+                        } else {
+                            __syncwarp();
+#pragma unroll
+                            for (int i = 0; i < 32; i += 8) {
+                                const int e = i + (lane >> 2), q = lane & 3;
+                                const uint4 v = *reinterpret_cast<const uint4 *>(smem + kOutStage + warp * kWarpSlab + e * 64 +
+                                                                                 ((q ^ ((e >> 1) & 3)) << 4));
+                                if ((warp & 3) * 32 + e < p.N1)
+                                    *reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(p.out) + (int64_t)(row + e) * kDv +
+                                                               g * (kDv / 2) + c + q * 8) = v;
+                            }
+                            __syncwarp();  // buf is written again
                         }
-                    }
-                } else {
-                    // other head counts, and pieces (fp32, normalised within the piece)
-                    float *po = p.part_o + (((int64_t)it.t * p.P + it.piece) * p.N1 + (head ? h : 0)) * kDv + g * (kDv / 2);
-#pragma unroll 1
-                    for (int c = 0; c < kDv / 2; c += 32) {
-                        uint32_t r[32];
-                        tmem_ld32(tcol + c, r);
-                        tc_wait_ld();
-                        float x[32];
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]) * fin;
-                        if (head && it.np > 1) {
-                            float4 *d = reinterpret_cast<float4 *>(po + c);
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) d[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-                        } else if (head) {
-                            uint4 *d = reinterpret_cast<uint4 *>(orow + c);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                d[i] = make_uint4(pack_bf16(x[8 * i], x[8 * i + 1]), pack_bf16(x[8 * i + 2], x[8 * i + 3]),
-                                                  pack_bf16(x[8 * i + 4], x[8 * i + 5]), pack_bf16(x[8 * i + 6], x[8 * i + 7]));
-                        }
-                        __syncwarp();  // the next load is warp-wide
                     }
                 }
                 tc_fence_before();
@@ -1019,8 +1019,8 @@ __global__ void __launch_bounds__(kDv / 4) fp8_combine_kernel(const TcArgs p) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
     const int64_t s0 = (int64_t)t * p.P;
-    const float4 *po = reinterpret_cast<const float4 *>(p.part_o + (s0 * p.N1 + h) * kDv) + tid;
-    const int64_t stride = (int64_t)p.N1 * kDv / 4;
+    const float4 *po = reinterpret_cast<const float4 *>(p.part_o + (s0 * p.NP + h) * kDv) + tid;
+    const int64_t stride = (int64_t)p.NP * kDv / 4;
     float4 o[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
@@ -1060,18 +1060,19 @@ __global__ void __launch_bounds__(kDv / 4) fp8_combine_kernel(const TcArgs p) {
     if (p.lse && tid == 0) p.lse[(int64_t)t * p.N1 + h] = lse2 * 0.6931471805599453f;
 }
 
-// Tensor map over [rows][D] bf16, boxes of 32 rows x 64 columns (128-byte swizzle) or 32 (64-byte).
-int make_map(CUtensorMap *map, const void *base, int64_t rows, int D, uint32_t columns) {
+// Tensor map over [rows][D] bf16 or fp32, boxes of 32 rows x 128 bytes (128-byte swizzle) or 64 (64-byte).
+int make_map(CUtensorMap *map, const void *base, int64_t rows, int D, bool fp32, uint32_t bytes) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return SAS_ERR_CUDA;
     if (rows >= INT32_MAX) return SAS_ERR_UNSUPPORTED;
+    const uint32_t size = fp32 ? 4 : 2;
     cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)rows};
-    cuuint64_t strides[1] = {(cuuint64_t)D * 2};
-    cuuint32_t box[2] = {columns, 32};
+    cuuint64_t strides[1] = {(cuuint64_t)D * size};
+    cuuint32_t box[2] = {bytes / size, 32};
     cuuint32_t estr[2] = {1, 1};
-    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(base), dims, strides, box, estr,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          columns == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+    const CUresult r = fn(map, fp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                          const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? SAS_OK : SAS_ERR_CUDA;
 }
@@ -1096,7 +1097,7 @@ Plan plan(const SasFp8Args &a) {
     if (P <= 1) return pl;
     pl.M = (int)((est + P - 1) / P);
     pl.P = (int)((est + pl.M - 1) / pl.M);
-    const int64_t bytes = (int64_t)a.num_tokens * pl.P * a.num_heads * kDv * 4;
+    const int64_t bytes = (int64_t)a.num_tokens * pl.P * ((a.num_heads + 31) / 32 * 32) * kDv * 4;
     return pl.P > 1 && bytes <= kMaxPartialBytes ? pl : Plan{1, 0};
 }
 
@@ -1124,9 +1125,12 @@ int launch_fp8_tc(const SasFp8Args &a, const Args &args, const Layout &L, char *
     p.U = a.num_tokens * pl.P;
     p.part_o = reinterpret_cast<float *>(ws + L.part_o);
     p.part_s = reinterpret_cast<float *>(ws + L.part_s);
-    CUtensorMap q_map, out_map;
-    int rc = make_map(&q_map, p.q, (int64_t)p.T * p.N1, p.Dq, 64);
-    if (!rc) rc = make_map(&out_map, p.out, (int64_t)p.T * p.N1, kDv, 32);
+    p.NP = (p.N1 + 31) / 32 * 32;
+    CUtensorMap q_map, out_map, part_map;
+    int rc = make_map(&q_map, p.q, (int64_t)p.T * p.N1, p.Dq, false, 128);
+    if (!rc) rc = make_map(&out_map, p.out, (int64_t)p.T * p.N1, kDv, false, 64);
+    part_map = out_map;
+    if (!rc && p.P > 1) rc = make_map(&part_map, p.part_o, (int64_t)p.T * p.P * p.NP, kDv, true, 64);
     if (rc) return rc;
     int dev = 0;
     if (check_cuda(cudaGetDevice(&dev))) return SAS_ERR_CUDA;
@@ -1156,7 +1160,7 @@ int launch_fp8_tc(const SasFp8Args &a, const Args &args, const Layout &L, char *
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    if (check_cuda(cudaLaunchKernelEx(&cfg, fp8_tc_kernel, p, q_map, out_map))) return SAS_ERR_CUDA;
+    if (check_cuda(cudaLaunchKernelEx(&cfg, fp8_tc_kernel, p, q_map, out_map, part_map))) return SAS_ERR_CUDA;
     if (p.P > 1) {
         cudaLaunchConfig_t cc = {};
         cc.gridDim = dim3(a.num_tokens, a.num_heads, 1);
