@@ -14,8 +14,8 @@ from typing import Optional, Tuple, Union
 import torch
 
 from . import _lib
-from .api import _dense16, _dtype_code, _i32, _out_shapes, _pool16, _ptr, _scenario, _workspace
-from .cache import _eager, _no_grad, _on, _ops
+from .api import _dense16, _dtype_code, _pool16, _ptr, _scenario, _workspace
+from .cache import _eager, _int32, _ops, _raw_stream, _refuse_grad
 
 KERNELS = {"auto": 0, "simt": 1, "tc": 2}
 
@@ -32,48 +32,47 @@ def _call_args(*sizes) -> Tuple["_lib.SasFp8Args", int]:
 def _launch(q, ori_kv, ori_kv_scale, cmp_kv, cmp_kv_scale, cmp_sparse_indices, ori_block_table, cmp_block_table,
             cu_seqlens_q, seqused_kv, sinks, softmax_scale, cmp_ratio, ori_win_left, ori_first, layout_q, v_head_dim,
             kernel, check_status, out, lse):
-    dev = q.device
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
+    device = q.get_device()
+    if device != torch.cuda.current_device():
+        with torch.cuda.device(device):
             return _launch(q, ori_kv, ori_kv_scale, cmp_kv, cmp_kv_scale, cmp_sparse_indices, ori_block_table,
                            cmp_block_table, cu_seqlens_q, seqused_kv, sinks, softmax_scale, cmp_ratio, ori_win_left,
                            ori_first, layout_q, v_head_dim, kernel, check_status, out, lse)
     scenario = _scenario(cmp_kv, cmp_sparse_indices)
-    N1, D = q.shape[-2], q.shape[-1]
-    act_q = None
+    cu = act_q = cmp_bt = idx = None
+    if cu_seqlens_q is not None:
+        cu = _int32(cu_seqlens_q, device)
     if layout_q == "TND":
-        T, S = q.shape[0], 0
-        cu = _i32(cu_seqlens_q, dev)
-        B = cu.numel() - 1
+        T, N1, D = q.shape
+        S, B = 0, cu.numel() - 1
     else:
-        B, S = q.shape[0], q.shape[1]
-        T, cu = B * S, None
-        if cu_seqlens_q is not None:
-            lens = _i32(cu_seqlens_q, dev)
-            act_q = (lens[1:] - lens[:-1]).contiguous()
+        B, S, N1, D = q.shape
+        T = B * S
+        if cu is not None:
+            cu, act_q = None, (cu[1:] - cu[:-1]).contiguous()
     _pool16(ori_kv, "ori_kv")
-    ori_bt, seq = _i32(ori_block_table, dev), _i32(seqused_kv, dev)
-    cmp_bt = idx = None
+    ori_bt, seq = _int32(ori_block_table, device), _int32(seqused_kv, device)
     cb = cs = ct = K = 0
     if scenario >= 2:
         _pool16(cmp_kv, "cmp_kv")
-        cmp_bt = _i32(cmp_block_table, dev)
-        cb, cs, ct = cmp_kv.shape[0], cmp_kv.shape[1], cmp_bt.shape[1]
+        cmp_bt = _int32(cmp_block_table, device)
+        cb, cs, _, _ = cmp_kv.shape
+        ct = cmp_bt.shape[1]
     if scenario == 3:
-        idx = _i32(cmp_sparse_indices, dev)
+        idx = _int32(cmp_sparse_indices, device)
         K = idx.shape[-1]
-    if sinks is not None:
-        sinks = sinks.to(device=dev, dtype=torch.float32).contiguous()
+    if sinks is not None and (sinks.dtype is not torch.float32 or sinks.get_device() != device or not sinks.is_contiguous()):
+        sinks = sinks.to(device=q.device, dtype=torch.float32).contiguous()
     q = _dense16(q)
-    args, nbytes = _call_args(B, T, S, N1, D, v_head_dim, ori_kv.shape[0], ori_kv.shape[1], ori_bt.shape[1], cb, cs, ct,
-                              K, cmp_ratio, scenario, ori_win_left, ori_first, _dtype_code(q.dtype), softmax_scale,
-                              KERNELS[kernel])
-    ws = _workspace(nbytes, dev)
+    ob, obs, _, _ = ori_kv.shape
+    args, nbytes = _call_args(B, T, S, N1, D, v_head_dim, ob, obs, ori_bt.shape[1], cb, cs, ct, K, cmp_ratio, scenario,
+                              ori_win_left, ori_first, _dtype_code(q.dtype), softmax_scale, KERNELS[kernel])
+    ws = _workspace(nbytes, q.device)
     out_user = None
     if out.data_ptr() % 16:  # a caller's out that starts inside a 16-byte vector
         out_user, out = out, torch.empty_like(out)
     lib = _lib.load()
-    stream = torch.cuda.current_stream(dev).cuda_stream
+    stream = _raw_stream(device)
     rc = lib.sas_kvq_forward(args, q.data_ptr(), ori_kv.data_ptr(), ori_kv_scale.data_ptr(), ori_bt.data_ptr(),
                              _ptr(cmp_kv), _ptr(cmp_kv_scale), _ptr(cmp_bt), _ptr(idx), _ptr(cu), _ptr(act_q),
                              seq.data_ptr(), _ptr(sinks), out.data_ptr(), _ptr(lse), ws.data_ptr(), nbytes, stream)
@@ -101,13 +100,16 @@ def _fake(*args):
     return None
 
 
-def _check_pool(name, pool, scale, D):
-    if pool.dtype != torch.float8_e4m3fn:
+def _check_pool(name, pool, scale, D, device):
+    if pool.dtype is not torch.float8_e4m3fn:
         raise ValueError(f"{name} must be float8_e4m3fn (got {pool.dtype}); 16-bit pools go to sparse_attn_sharedkv")
-    if pool.dim() != 4 or pool.shape[2] != 1 or pool.shape[3] != D:
-        raise ValueError(f"{name} must be [blocks, block_size, 1, {D}] (got {tuple(pool.shape)})")
-    if scale is None or scale.dtype != torch.float32 or not scale.is_contiguous() or scale.numel() != pool.shape[0]:
+    shape = pool.shape
+    if len(shape) != 4 or shape[2] != 1 or shape[3] != D:
+        raise ValueError(f"{name} must be [blocks, block_size, 1, {D}] (got {tuple(shape)})")
+    if scale is None or scale.dtype is not torch.float32 or scale.numel() != shape[0] or not scale.is_contiguous():
         raise ValueError(f"{name}_scale must be contiguous float32 with one entry per block of {name}")
+    if pool.device != device or scale.device != device:
+        raise ValueError(f"{name} and {name}_scale must be on {device}")
 
 
 def sparse_attn_sharedkv_fp8(
@@ -154,52 +156,55 @@ def sparse_attn_sharedkv_fp8(
         raise ValueError(f"kernel must be one of {sorted(KERNELS)}")
     if not q.is_cuda:
         raise ValueError("q must be a CUDA tensor (sas_b200 has no CPU path)")
-    lead = 1 if layout_q == "TND" else 2
-    if q.dim() != lead + 2:
-        raise ValueError(f"q must be {'[T, N1, D]' if lead == 1 else '[B, S, N1, D]'} (got {tuple(q.shape)})")
-    _no_grad("sparse_attn_sharedkv_fp8", q, sinks)
-    dev = q.device
-    N1, D = q.shape[-2], q.shape[-1]
-    _on(dev, ori_kv=ori_kv, ori_kv_scale=ori_kv_scale, cmp_kv=cmp_kv, cmp_kv_scale=cmp_kv_scale, out=out,
-        lse_out=lse_out)
-    _check_pool("ori_kv", ori_kv, ori_kv_scale, D)
-    Dv = D if v_head_dim is None else int(v_head_dim)
+    if torch.is_grad_enabled() and (q.requires_grad or (sinks is not None and sinks.requires_grad)):
+        _refuse_grad("sparse_attn_sharedkv_fp8")
+    shape, device, kind = q.shape, q.device, q.dtype
     if layout_q == "TND":
+        lead = 1
         assert cu_seqlens_q is not None, "cu_seqlens_q is required for TND"
-        B, T = cu_seqlens_q.numel() - 1, q.shape[0]
+        B = cu_seqlens_q.numel() - 1
     else:
-        B, T = q.shape[0], q.shape[0] * q.shape[1]
+        lead, B = 2, shape[0]
         if cu_seqlens_q is not None and cu_seqlens_q.numel() != B + 1:
             raise ValueError(f"cu_seqlens_q must have {B + 1} entries (got {cu_seqlens_q.numel()})")
+    if len(shape) != lead + 2:
+        raise ValueError(f"q must be {'[T, N1, D]' if lead == 1 else '[B, S, N1, D]'} (got {tuple(shape)})")
+    N1, D = shape[-2], shape[-1]
+    Dv = D if v_head_dim is None else int(v_head_dim)
+    _check_pool("ori_kv", ori_kv, ori_kv_scale, D, device)
     if ori_block_table.dim() != 2 or ori_block_table.shape[0] < B:
         raise ValueError(f"ori_block_table must be [B>={B}, table_len] (got {tuple(ori_block_table.shape)})")
     if seqused_kv.numel() < B:
         raise ValueError(f"seqused_kv must have {B} entries (got {seqused_kv.numel()})")
     if cmp_kv is not None:
         assert cmp_ratio is not None, "cmp_ratio is required with cmp_kv"
-        _check_pool("cmp_kv", cmp_kv, cmp_kv_scale, D)
+        _check_pool("cmp_kv", cmp_kv, cmp_kv_scale, D, device)
         if cmp_block_table is None or cmp_block_table.dim() != 2 or cmp_block_table.shape[0] < B:
             raise ValueError(f"cmp_block_table must be [B>={B}, table_len]")
         if cmp_sparse_indices is not None:
-            if cmp_sparse_indices.dim() != lead + 2 or cmp_sparse_indices.shape[:lead] != q.shape[:lead] \
-                    or cmp_sparse_indices.shape[lead] != 1:
-                raise ValueError(f"cmp_sparse_indices must hold [1, K] per token (got {tuple(cmp_sparse_indices.shape)})")
+            rows = cmp_sparse_indices.shape
+            if len(rows) != lead + 2 or rows[:lead] != shape[:lead] or rows[lead] != 1:
+                raise ValueError(f"cmp_sparse_indices must hold [1, K] per token (got {tuple(rows)})")
     elif cmp_sparse_indices is not None:
         raise ValueError("cmp_sparse_indices goes with cmp_kv")
     if sinks is not None and sinks.numel() != N1:
         raise ValueError(f"sinks must have {N1} entries (got {sinks.numel()})")
     if ori_win_left < 0 or ori_first < 0:
         raise ValueError("ori_win_left and ori_first must be >= 0")
-    o_shape, l_shape = _out_shapes(q, layout_q, Dv)
+    tokens = shape[:lead]
     if out is None:
-        out = torch.empty(o_shape, dtype=q.dtype, device=dev)
-    elif out.dtype != q.dtype or out.numel() != T * N1 * Dv or not out.is_contiguous():
-        raise ValueError(f"out must be contiguous {q.dtype} of shape {o_shape}")
-    lse = lse_out
-    if lse is None:
-        lse = torch.empty(l_shape, dtype=torch.float32, device=dev) if return_softmax_lse else None
-    elif lse.dtype != torch.float32 or lse.numel() != T * N1 or not lse.is_contiguous():
-        raise ValueError(f"lse_out must be contiguous float32 of shape {l_shape}")
+        result = out = torch.empty((*tokens, N1, Dv), dtype=kind, device=device)
+    else:
+        result = out.view((*tokens, N1, Dv)) if out.is_contiguous() and out.numel() == tokens.numel() * N1 * Dv else None
+        if result is None or out.dtype is not kind or out.device != device:
+            raise ValueError(f"out must be contiguous {kind} of shape {(*tokens, N1, Dv)} on {device}")
+    lse = sums = lse_out
+    if lse is not None:
+        sums = lse.view((*tokens, N1)) if lse.is_contiguous() and lse.numel() == tokens.numel() * N1 else None
+        if sums is None or lse.dtype is not torch.float32 or lse.device != device:
+            raise ValueError(f"lse_out must be contiguous float32 of shape {(*tokens, N1)} on {device}")
+    elif return_softmax_lse:
+        lse = sums = torch.empty((*tokens, N1), dtype=torch.float32, device=device)
     call = (q, ori_kv, ori_kv_scale, cmp_kv, cmp_kv_scale, cmp_sparse_indices, ori_block_table, cmp_block_table,
             cu_seqlens_q, seqused_kv, sinks, float(softmax_scale), 4 if cmp_ratio is None else int(cmp_ratio),
             int(ori_win_left), int(ori_first), layout_q, Dv, kernel, bool(check_status), out, lse)
@@ -207,5 +212,4 @@ def sparse_attn_sharedkv_fp8(
         _launch(*call)
     else:
         torch.ops.sas_b200.sparse_attn_sharedkv_fp8(*call)
-    out, lse = out.view(o_shape), lse.view(l_shape) if lse is not None else None
-    return (out, lse) if return_softmax_lse else out
+    return (result, sums) if return_softmax_lse else result

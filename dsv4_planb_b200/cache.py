@@ -38,15 +38,8 @@ def rope_table(positions: int, rope_dim: int, *, base: float = 10000.0, inv_freq
     return torch.cat([ang.cos(), ang.sin()], dim=1).to(torch.float32)
 
 
-def _on(dev, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} must be on {dev} (got {t.device})")
-
-
-def _no_grad(what, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{what} has no backward pass: call it under torch.no_grad() or detach its inputs")
+def _refuse_grad(what: str) -> None:
+    raise ValueError(f"{what} has no backward pass: call it under torch.no_grad() or detach its inputs")
 
 
 def _eager(t: torch.Tensor) -> bool:
@@ -55,14 +48,28 @@ def _eager(t: torch.Tensor) -> bool:
     return type(t) is torch.Tensor and not torch.compiler.is_compiling()
 
 
+def _int32(t: torch.Tensor, device: int) -> torch.Tensor:
+    """``_i32`` with a short way for what needs no conversion."""
+    if t.dtype is torch.int32 and t.get_device() == device and t.is_contiguous():
+        return t
+    return _i32(t, torch.device("cuda", device))
+
+
+# The current stream's handle: torch.cuda.current_stream builds a Stream object first (3 us a call).
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _rows2d(kv: torch.Tensor, T: int, D: int) -> torch.Tensor:
     """``kv`` as T rows of D consecutive elements, 16-byte aligned; rows may be further apart (a slice
     of a wider projection), anything else is copied."""
-    try:
-        v = kv.view(T, D)
-    except RuntimeError:
-        v = kv.reshape(T, D)
-    if v.stride(1) != 1 or (T > 1 and (v.stride(0) % 8 or v.stride(0) < D)) or v.data_ptr() % 16:
+    v = kv
+    if kv.dim() != 2:
+        try:
+            v = kv.view(T, D)
+        except RuntimeError:
+            v = kv.reshape(T, D)
+    row, one = v.stride()
+    if one != 1 or (T > 1 and (row % 8 or row < D)) or v.data_ptr() % 16:
         v = v.contiguous()
         if v.data_ptr() % 16:
             v = v.clone()
@@ -77,57 +84,52 @@ def _append_args(*sizes) -> "_lib.SasAppendArgs":
 
 def _append(kv, cache, cache_scale, block_table, seqused_kv, cu_seqlens_q, rope_table, rope_interleaved, rope_step, q,
             q_out, layout_q, check_status):
-    dev = cache.device
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            return _append_on(dev, kv, cache, cache_scale, block_table, seqused_kv, cu_seqlens_q, rope_table,
-                              rope_interleaved, rope_step, q, q_out, layout_q, check_status)
-    return _append_on(dev, kv, cache, cache_scale, block_table, seqused_kv, cu_seqlens_q, rope_table, rope_interleaved,
-                      rope_step, q, q_out, layout_q, check_status)
-
-
-def _append_on(dev, kv, cache, cache_scale, block_table, seqused_kv, cu_seqlens_q, rope_table, rope_interleaved,
-               rope_step, q, q_out, layout_q, check_status):
+    device = cache.get_device()
+    if device != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _append(kv, cache, cache_scale, block_table, seqused_kv, cu_seqlens_q, rope_table, rope_interleaved,
+                           rope_step, q, q_out, layout_q, check_status)
     _pool16(cache, "cache")
-    if rope_table is not None and rope_table.data_ptr() % 16:
-        raise ValueError("rope_table must start on a 16-byte boundary")
-    D = cache.shape[3]
+    blocks, bs, _, D = cache.shape
+    R = rope_rows = rope_at = 0
+    if rope_table is not None:
+        rope_at = rope_table.data_ptr()
+        rope_rows, R = rope_table.shape
+        if rope_at % 16:
+            raise ValueError("rope_table must start on a 16-byte boundary")
+    cu = act_q = None
+    if cu_seqlens_q is not None:
+        cu = _int32(cu_seqlens_q, device)
     if layout_q == "TND":
         T, S = kv.shape[0], 0
-        B = cu_seqlens_q.numel() - 1
-        cu, act_q = _i32(cu_seqlens_q, dev), None
+        B = cu.numel() - 1
     else:
         B, S = kv.shape[0], kv.shape[1]
-        T, cu, act_q = B * S, None, None
-        if cu_seqlens_q is not None:
-            lens = _i32(cu_seqlens_q, dev)
-            act_q = (lens[1:] - lens[:-1]).contiguous()
+        T = B * S
+        if cu is not None:
+            cu, act_q = None, (cu[1:] - cu[:-1]).contiguous()
     rows = _rows2d(kv, T, D)
-    table, seq = _i32(block_table, dev), _i32(seqused_kv, dev)
-    R = 0 if rope_table is None else rope_table.shape[1]
-    heads = 0
+    table, seq = _int32(block_table, device), _int32(seqused_kv, device)
+    heads = q_at = out_at = 0
     if q_out is not None:
-        heads = q_out.shape[-2]
-        at = q_out.data_ptr()
-        if at % 16:
+        heads, out_at = q_out.shape[-2], q_out.data_ptr()
+        if out_at % 16:
             raise ValueError("q_out must start on a 16-byte boundary")
         if q is None:
             q = q_out  # turned in place
         else:
-            d = q.data_ptr() - at
+            d = q.data_ptr() - out_at
             n = q_out.numel() * q_out.element_size()
             if -n < d < n and n and not (d == 0 and q.is_contiguous()):
                 raise ValueError("q_out must be q itself or share nothing with it")
             q = _dense16(q)
-    args = _append_args(B, T, heads, D, R, int(rope_interleaved), rope_step, 0 if R == 0 else rope_table.shape[0],
-                        cache.shape[0], cache.shape[1], table.shape[1], S, _dtype_code(kv.dtype),
-                        _CACHE_DTYPES[cache.dtype], max(rows.stride(0), D) if T > 1 else D)
-    lib = _lib.load()
-    word = torch.zeros(1, dtype=torch.int32, device=dev) if check_status else None
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    rc = lib.sas_cache_append(args, rows.data_ptr(), _ptr(q if heads else None), _ptr(q_out), _ptr(rope_table),
-                              table.data_ptr(), _ptr(cu), _ptr(act_q), seq.data_ptr(), cache.data_ptr(),
-                              _ptr(cache_scale), _ptr(word), stream)
+        q_at = q.data_ptr()
+    args = _append_args(B, T, heads, D, R, int(rope_interleaved), rope_step, rope_rows, blocks, bs, table.shape[1], S,
+                        _dtype_code(kv.dtype), _CACHE_DTYPES[cache.dtype], rows.stride(0) if T > 1 else D)
+    word = torch.zeros(1, dtype=torch.int32, device=cache.device) if check_status else None
+    rc = _lib.load().sas_cache_append(args, rows.data_ptr(), q_at, out_at, rope_at, table.data_ptr(), _ptr(cu),
+                                      _ptr(act_q), seq.data_ptr(), cache.data_ptr(), _ptr(cache_scale), _ptr(word),
+                                      _raw_stream(device))
     if rc:
         _lib.check(rc, "sas_cache_append")
     if check_status:
@@ -191,30 +193,33 @@ def sharedkv_cache_append(
     assert layout_q in ("TND", "BSND"), f"unsupported layout_q={layout_q!r}"
     if not cache.is_cuda:
         raise ValueError("cache must be a CUDA tensor (sas_b200 has no CPU path)")
-    _no_grad("sharedkv_cache_append", kv, q, cache, cache_scale, rope_table)
-    dev = cache.device
-    _on(dev, kv=kv, cache_scale=cache_scale, rope_table=rope_table, q=q, q_out=q_out)
-    if kv.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"kv must be bfloat16 or float16 (got {kv.dtype})")
+    if torch.is_grad_enabled() and (kv.requires_grad or (q is not None and q.requires_grad)):
+        _refuse_grad("sharedkv_cache_append")
+    device, kind = cache.device, kv.dtype
+    if kv.device != device or any(t is not None and t.device != device for t in (cache_scale, rope_table, q, q_out)):
+        raise ValueError(f"kv, cache_scale, rope_table, q and q_out must be on {device}")
+    if kind is not torch.bfloat16 and kind is not torch.float16:
+        raise ValueError(f"kv must be bfloat16 or float16 (got {kind})")
     if cache.dim() != 4 or cache.shape[2] != 1:
         raise ValueError(f"cache must be [blocks, block_size, 1, D] (got {tuple(cache.shape)})")
-    D = cache.shape[3]
+    blocks, _, _, D = cache.shape
+    rows = kv.shape
     lead = 1 if layout_q == "TND" else 2
-    if kv.dim() not in (lead + 1, lead + 2) or kv.shape[-1] != D or (kv.dim() == lead + 2 and kv.shape[lead] != 1):
-        raise ValueError(f"kv must hold one row of {D} per token in layout {layout_q} (got {tuple(kv.shape)})")
-    if cache.dtype == torch.float8_e4m3fn:
-        if cache_scale is None or cache_scale.dtype != torch.float32 or not cache_scale.is_contiguous() \
-                or cache_scale.numel() != cache.shape[0]:
+    if len(rows) not in (lead + 1, lead + 2) or rows[-1] != D or (len(rows) == lead + 2 and rows[lead] != 1):
+        raise ValueError(f"kv must hold one row of {D} per token in layout {layout_q} (got {tuple(rows)})")
+    if cache.dtype is torch.float8_e4m3fn:
+        if cache_scale is None or cache_scale.dtype is not torch.float32 or cache_scale.numel() != blocks \
+                or not cache_scale.is_contiguous():
             raise ValueError("a float8_e4m3fn cache needs cache_scale: contiguous float32, one entry per block")
-    elif cache.dtype != kv.dtype:
+    elif cache.dtype is not kind:
         raise ValueError(f"cache must be of the type of kv or float8_e4m3fn (got {cache.dtype})")
     elif cache_scale is not None:
         raise ValueError("cache_scale goes with a float8_e4m3fn cache only")
-    if layout_q == "TND":
+    if lead == 1:
         assert cu_seqlens_q is not None, "cu_seqlens_q is required for TND"
         B = cu_seqlens_q.numel() - 1
     else:
-        B = kv.shape[0]
+        B = rows[0]
         if cu_seqlens_q is not None and cu_seqlens_q.numel() != B + 1:
             raise ValueError(f"cu_seqlens_q must have {B + 1} entries (got {cu_seqlens_q.numel()})")
     if block_table.dim() != 2 or block_table.shape[0] < B or block_table.shape[1] < 1:
@@ -224,16 +229,16 @@ def sharedkv_cache_append(
     if rope_step < 1:
         raise ValueError("rope_step must be >= 1")
     if rope_table is not None:
-        if rope_table.dtype != torch.float32 or rope_table.dim() != 2 or not rope_table.is_contiguous():
+        if rope_table.dtype is not torch.float32 or rope_table.dim() != 2 or not rope_table.is_contiguous():
             raise ValueError("rope_table must be a contiguous float32 [positions, rope_dim]")
         if rope_table.shape[1] % 16 or not 0 < rope_table.shape[1] <= D:
             raise ValueError(f"rope_dim must be a multiple of 16 up to {D} (got {rope_table.shape[1]})")
     if q is not None:
-        if q.dtype != kv.dtype or q.dim() != lead + 2 or q.shape[:lead] != kv.shape[:lead] or q.shape[-1] != D:
+        if q.dtype is not kind or q.dim() != lead + 2 or q.shape[:lead] != rows[:lead] or q.shape[-1] != D:
             raise ValueError(f"q must be of kv's type and hold [N1, {D}] per token (got {q.dtype} {tuple(q.shape)})")
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        elif q_out.shape != q.shape or q_out.dtype != q.dtype or not q_out.is_contiguous():
+            q_out = torch.empty(q.shape, dtype=kind, device=device)
+        elif q_out.shape != q.shape or q_out.dtype is not kind or not q_out.is_contiguous():
             raise ValueError("q_out must be contiguous and of q's shape and type")
     elif q_out is not None:
         raise ValueError("q_out goes with q")
