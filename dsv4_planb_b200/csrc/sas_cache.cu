@@ -14,7 +14,14 @@
 // powers of two moves the exponent and loses nothing above e4m3's subnormals.  Powers of two are
 // taken for that reason: with scales A / 448 every growth would round every old row anew.
 //
-// Bound: bytes (each row read once and written once).  A decode call is one launch latency.
+// Bound: bytes (each row read once and written once); a decode call is one launch latency, 6.4 us on the
+// device.  4 x 8192 rows of 576 to 8 bits take 16.7 us, 57 MB at 3.4 TB/s: the rows are read twice, the
+// second time from L1 or L2, and the two passes and the lookups before them follow one another in a CTA.
+// Clusters of 4 x 128 threads with 4 loads under way per thread take 16.7 us, 2 x 128 18.7, 2 x 256 18.3,
+// 8 x 256 43; one row per CTA (512 requests) takes 8.4 us with 128 threads and 12.4 with 256, which need
+// two waves.  The largest value of the copied dims is found on the bits, two at a time: unpacked to
+// floats, and with 64-bit positions, the kernel was bound by its instructions at 43 us.  Rows kept in
+// registers between the passes cost occupancy, 63 us; two kernels with a warp per two rows, 47 us.
 
 #include <algorithm>
 
@@ -24,8 +31,9 @@
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
+constexpr int kCluster = 4;  // CTAs per block that takes many rows
 constexpr int kQHeads = 16;  // query heads per CTA of the q part
 constexpr int kMaxChunks = 4;  // 16-byte chunks of a row per lane: D <= 1024
 
@@ -94,8 +102,7 @@ __device__ __forceinline__ void load_rotated(const AppendArgs &p, const uint4 *r
 // The new tokens of request b: the position of its first one, its first row among the T flat rows,
 // and how many rows there are (clipped to T and to positions >= 0).
 struct Span {
-    int64_t pos;
-    int row, n;
+    int pos, row, n;
 };
 __device__ __forceinline__ Span span_of(const AppendArgs &p, int b) {
     int64_t row;
@@ -107,21 +114,22 @@ __device__ __forceinline__ Span span_of(const AppendArgs &p, int b) {
         row = (int64_t)b * p.q_rows;
         n = p.act_q ? min(__ldg(p.act_q + b), p.q_rows) : p.q_rows;
     }
-    Span sp;
-    sp.pos = (int64_t)__ldg(p.act_kv + b) - n;
-    if (sp.pos < 0) {  // tokens before the sequence's start have no place
-        row -= sp.pos;
-        n += (int)sp.pos;
-        sp.pos = 0;
+    int64_t pos = (int64_t)__ldg(p.act_kv + b) - n;
+    if (pos < 0) {  // tokens before the sequence's start have no place
+        row -= pos;
+        n += (int)pos;
+        pos = 0;
     }
     if (row < 0 || row >= p.T) n = 0;
+    Span sp;
+    sp.pos = (int)pos;
     sp.row = (int)row;
     sp.n = (int)min((int64_t)n, (int64_t)p.T - row);
     return sp;
 }
 
 // Position of flat row t, or -1 where it belongs to no request (warp-uniform; every lane calls).
-__device__ __forceinline__ int64_t position_of(const AppendArgs &p, int t, int &b) {
+__device__ __forceinline__ int position_of(const AppendArgs &p, int t, int &b) {
     b = p.cu ? sas_fp8::find_request(p.cu, p.B, t) : t / p.q_rows;
     if (b < 0 || b >= p.B) return -1;
     const Span sp = span_of(p, b);
@@ -139,7 +147,7 @@ __device__ __forceinline__ const float *angles(const AppendArgs &p, int64_t pos)
     return p.rope + r * p.R;
 }
 
-__device__ __forceinline__ int64_t block_of(const AppendArgs &p, int b, int64_t blk) {
+__device__ __forceinline__ int64_t block_of(const AppendArgs &p, int b, int blk) {
     int32_t phys = -1;
     if (blk < p.table_len) phys = __ldg(p.table + (int64_t)b * p.table_len + blk);
     if (phys < 0 || phys >= p.block_num) {
@@ -156,7 +164,7 @@ template <typename T> __device__ void rotate_q(const AppendArgs &p, int cta) {
     const int t = cta / groups, h0 = (cta - t * groups) * kQHeads;
     if (t >= p.T) return;
     int b;
-    const int64_t pos = position_of(p, t, b);
+    const int pos = position_of(p, t, b);
     const float *cs = pos >= 0 ? angles(p, pos) : nullptr;
     const bool in_place = p.q == p.q_out;
     if (in_place && cs == nullptr) return;
@@ -199,9 +207,10 @@ template <typename T> __global__ void __launch_bounds__(kThreads) append16_kerne
     const uint4 *row = reinterpret_cast<const uint4 *>(p.kv + (int64_t)t * p.kv_stride * 2);
     const int nc = p.D / 8;
     int b;
-    const int64_t pos = position_of(p, t, b);
+    const int pos = position_of(p, t, b);
     if (pos < 0) return;
-    const int64_t blk = pos / p.bs, phys = block_of(p, b, blk);
+    const int blk = pos / p.bs;
+    const int64_t phys = block_of(p, b, blk);
     const float *cs = angles(p, pos);
     if (phys < 0 || cs == nullptr) return;
     uint4 *dst = reinterpret_cast<uint4 *>(p.cache) + (phys * p.bs + (pos - blk * p.bs)) * nc;
@@ -216,8 +225,47 @@ template <typename T> __global__ void __launch_bounds__(kThreads) append16_kerne
     }
 }
 
-// 8-bit cache: a cluster per (request, block with new rows); its warps share the rows.
+// Bits of the 16-bit types' infinity.
+template <typename T> __device__ constexpr uint32_t infinity_bits();
+template <> __device__ constexpr uint32_t infinity_bits<__nv_bfloat16>() { return 0x7f80u; }
+template <> __device__ constexpr uint32_t infinity_bits<__half>() { return 0x7c00u; }
+
+__device__ __forceinline__ void note_finite(float x, float &amax) {
+    x = fabsf(x);
+    if (x <= 3.402823466e38f) amax = fmaxf(amax, x);  // neither infinity nor NaN
+}
+
+// Steps through the pieces of rows of `width` pieces: `from`, from + by, ...
+struct Walk {
+    int row, at, drow, dat, width;
+    __device__ __forceinline__ Walk(int from, int by, int w)
+        : row(from / w), at(from - from / w * w), drow(by / w), dat(by - by / w * w), width(w) {}
+    __device__ __forceinline__ void next() {
+        row += drow;
+        at += dat;
+        if (at >= width) {
+            at -= width;
+            ++row;
+        }
+    }
+};
+
+// 16 values of a 16-bit type times a power of two, to 16 codes.
+template <typename T> __device__ __forceinline__ uint4 to_codes16(const uint4 (&v)[2], float inv) {
+    float x[16];
+    unpack8<T>(v[0], reinterpret_cast<float (&)[8]>(x[0]));
+    unpack8<T>(v[1], reinterpret_cast<float (&)[8]>(x[8]));
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        w[i] = sas_fp8::to_e4m3x4(x[4 * i] * inv, x[4 * i + 1] * inv, x[4 * i + 2] * inv, x[4 * i + 3] * inv);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// 8-bit cache: a cluster per (request, block with new rows); its threads share the rows, 16 dims of the
+// copied part or 8 of the turned part at a time.
 template <typename T> __global__ void __launch_bounds__(kThreads) append8_kernel(AppendArgs p) {
+    constexpr int kAhead = 4;  // loads of 16 dims under way per thread
     __shared__ int warp_sum[kWarps];
     __shared__ int found[2];
     __shared__ float warp_max[kWarps];
@@ -236,7 +284,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads) append8_kernel
     const int per = (p.B + kThreads - 1) / kThreads;
     int mine = 0;
     auto runs_of = [&](const Span &sp) {
-        return sp.n > 0 ? (int)((sp.pos + sp.n - 1) / p.bs - sp.pos / p.bs) + 1 : 0;
+        return sp.n > 0 ? ((sp.pos + sp.n - 1) / p.bs - sp.pos / p.bs) + 1 : 0;
     };
     for (int b = tid * per; b < min(p.B, (tid + 1) * per); ++b) mine += runs_of(span_of(p, b));
     int incl = mine;
@@ -265,30 +313,67 @@ template <typename T> __global__ void __launch_bounds__(kThreads) append8_kernel
     const int b = found[0];
     if (b < 0) return;  // the whole cluster leaves: it has one unit
     const Span sp = span_of(p, b);
-    const int64_t blk = sp.pos / p.bs + found[1];
-    const int o0 = (int)max(sp.pos - blk * p.bs, (int64_t)0);                    // first new row in the block
-    const int o1 = (int)min(sp.pos + sp.n - blk * p.bs, (int64_t)p.bs);          // one past the last
-    const int64_t t0 = sp.row + (blk * p.bs + o0 - sp.pos);                      // flat row of o0
+    const int blk = sp.pos / p.bs + found[1], first = blk * p.bs;  // the block and its first position
+    const int o0 = max(sp.pos - first, 0);                         // first new row in the block
+    int rows = min(sp.pos + sp.n - first, p.bs) - o0;
+    const char *src = p.kv + ((int64_t)sp.row + (first + o0 - sp.pos)) * p.kv_stride * 2;
     const int64_t phys = block_of(p, b, blk);
     const bool any = phys >= 0;
     float old = any && o0 > 0 ? __ldg(p.scale + phys) : 0.f;
-    const int nc = p.D / 8, w0 = (int)rank * kWarps + warp, nw = (int)ranks * kWarps;
+    const float *cs0 = p.rope + (int64_t)(first + o0) * p.step * p.R;
+    if (p.R > 0) {  // rows past the table's end have no place
+        const int last = (int)min(((int64_t)p.rope_rows + p.step - 1) / p.step - (first + o0), (int64_t)rows);
+        if (last < rows) sas::set_status(p.status, SAS_STATUS_BAD_POSITION);
+        rows = max(last, 0);
+    }
+    if (!any) rows = 0;
+    const int me = (int)rank * kThreads + tid, all = (int)ranks * kThreads;
+    const int plain = (p.D - p.R) / 16, turned = p.R / 8;
+    const int64_t src_bytes = p.kv_stride * 2;
 
     float amax = 0.f;
-    if (any) {
-        for (int o = o0 + w0; o < o1; o += nw) {
-            const float *cs = angles(p, blk * p.bs + o);
-            if (cs == nullptr) continue;
-            const uint4 *row = reinterpret_cast<const uint4 *>(p.kv + (t0 + o - o0) * p.kv_stride * 2);
-            for (int c = lane; c < nc; c += 32) {
-                float x[8];
-                load_rotated<T>(p, row, cs, c, x);
+    if (plain) {
+        uint32_t m = 0;  // magnitudes order as their bits do, two at a time
+        Walk w(me, all, plain);
+        while (w.row < rows) {
+            uint4 v[kAhead][2];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float a = fabsf(x[i]);
-                    if (a <= 3.402823466e38f) amax = fmaxf(amax, a);  // neither infinity nor NaN
+            for (int k = 0; k < kAhead; ++k, w.next()) {
+                const uint4 *x = reinterpret_cast<const uint4 *>(src + w.row * src_bytes) + 2 * w.at;
+                v[k][0] = w.row < rows ? __ldg(x) : make_uint4(0, 0, 0, 0);
+                v[k][1] = w.row < rows ? __ldg(x + 1) : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    m = __vmaxu2(m, v[k][i].x & 0x7fff7fffu);
+                    m = __vmaxu2(m, v[k][i].y & 0x7fff7fffu);
+                    m = __vmaxu2(m, v[k][i].z & 0x7fff7fffu);
+                    m = __vmaxu2(m, v[k][i].w & 0x7fff7fffu);
+                }
+        }
+        m = max(m >> 16, m & 0xffffu);
+        if (m < infinity_bits<T>()) {
+            amax = sas::DT<T>::to_f2(m).x;
+        } else {  // an infinity or a NaN: look again, past those
+            for (Walk r(me, all, plain); r.row < rows; r.next()) {
+                const uint4 *x = reinterpret_cast<const uint4 *>(src + r.row * src_bytes) + 2 * r.at;
+                for (int h = 0; h < 2; ++h) {
+                    float y[8];
+                    unpack8<T>(__ldg(x + h), y);
+                    for (int i = 0; i < 8; ++i) note_finite(y[i], amax);
                 }
             }
+        }
+    }
+    if (turned) {
+        for (Walk w(me, all, turned); w.row < rows; w.next()) {
+            float x[8];
+            load_rotated<T>(p, reinterpret_cast<const uint4 *>(src + w.row * src_bytes), cs0 + (int64_t)w.row * p.step * p.R,
+                            2 * plain + w.at, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) note_finite(x[i], amax);
         }
     }
 #pragma unroll
@@ -339,17 +424,33 @@ template <typename T> __global__ void __launch_bounds__(kThreads) append8_kernel
         }
     }
     const float inv = 1.f / now;
-    for (int o = o0 + w0; o < o1; o += nw) {  // the second read of a row finds it in L1
-        const float *cs = angles(p, blk * p.bs + o);
-        if (cs == nullptr) continue;
-        const uint4 *row = reinterpret_cast<const uint4 *>(p.kv + (t0 + o - o0) * p.kv_stride * 2);
-        uint2 *dst = reinterpret_cast<uint2 *>(block + (int64_t)o * p.D);
-        for (int c = lane; c < nc; c += 32) {
+    uint8_t *dst = block + (int64_t)o0 * p.D;  // the second read of a row finds it in L1 or L2
+    if (plain) {
+        Walk w(me, all, plain);
+        while (w.row < rows) {
+            uint4 v[kAhead][2];
+            Walk r = w;
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k, r.next()) {
+                if (r.row >= rows) continue;
+                const uint4 *x = reinterpret_cast<const uint4 *>(src + r.row * src_bytes) + 2 * r.at;
+                v[k][0] = __ldg(x);
+                v[k][1] = __ldg(x + 1);
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k, w.next())
+                if (w.row < rows) reinterpret_cast<uint4 *>(dst + (int64_t)w.row * p.D)[w.at] = to_codes16<T>(v[k], inv);
+        }
+    }
+    if (turned) {
+        for (Walk w(me, all, turned); w.row < rows; w.next()) {
             float x[8];
-            load_rotated<T>(p, row, cs, c, x);
+            load_rotated<T>(p, reinterpret_cast<const uint4 *>(src + w.row * src_bytes), cs0 + (int64_t)w.row * p.step * p.R,
+                            2 * plain + w.at, x);
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] *= inv;
-            dst[c] = make_uint2(sas_fp8::to_e4m3x4(x[0], x[1], x[2], x[3]), sas_fp8::to_e4m3x4(x[4], x[5], x[6], x[7]));
+            reinterpret_cast<uint2 *>(dst + (int64_t)w.row * p.D)[2 * plain + w.at] =
+                make_uint2(sas_fp8::to_e4m3x4(x[0], x[1], x[2], x[3]), sas_fp8::to_e4m3x4(x[4], x[5], x[6], x[7]));
         }
     }
 }
@@ -427,7 +528,8 @@ extern "C" int sas_cache_append(const SasAppendArgs *args, const void *kv, const
     }
     // at most one unit per token, and n / bs + 2 per request of n tokens
     const int64_t units = std::min<int64_t>(a.num_tokens, a.num_tokens / a.block_size + 2 * (int64_t)a.batch);
-    const int cluster = a.num_tokens >= 16 * units ? 8 : 1;
+    // a cluster where blocks take 16 rows and more: 128 rows per block as above; with one row its other CTAs are idle
+    const int cluster = a.num_tokens >= 16 * units ? kCluster : 1;
     nq = (nq + cluster - 1) / cluster * cluster;
     const int64_t grid = nq + units * cluster;
     if (grid >= INT32_MAX) return SAS_ERR_UNSUPPORTED;
