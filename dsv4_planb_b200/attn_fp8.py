@@ -193,7 +193,7 @@ def sparse_attn_sharedkv_fp8(
         raise ValueError("ori_win_left and ori_first must be >= 0")
     tokens = shape[:lead]
     if out is None:
-        result = out = torch.empty((*tokens, N1, Dv), dtype=kind, device=device)
+        result = out = q.new_empty((*tokens, N1, Dv))
     else:
         result = out.view((*tokens, N1, Dv)) if out.is_contiguous() and out.numel() == tokens.numel() * N1 * Dv else None
         if result is None or out.dtype is not kind or out.device != device:
@@ -204,7 +204,7 @@ def sparse_attn_sharedkv_fp8(
         if sums is None or lse.dtype is not torch.float32 or lse.device != device:
             raise ValueError(f"lse_out must be contiguous float32 of shape {(*tokens, N1)} on {device}")
     elif return_softmax_lse:
-        lse = sums = torch.empty((*tokens, N1), dtype=torch.float32, device=device)
+        lse = sums = q.new_empty((*tokens, N1), dtype=torch.float32)
     call = (q, ori_kv, ori_kv_scale, cmp_kv, cmp_kv_scale, cmp_sparse_indices, ori_block_table, cmp_block_table,
             cu_seqlens_q, seqused_kv, sinks, float(softmax_scale), 4 if cmp_ratio is None else int(cmp_ratio),
             int(ori_win_left), int(ori_first), layout_q, Dv, kernel, bool(check_status), out, lse)

@@ -237,7 +237,7 @@ def sharedkv_cache_append(
         if q.dtype is not kind or q.dim() != lead + 2 or q.shape[:lead] != rows[:lead] or q.shape[-1] != D:
             raise ValueError(f"q must be of kv's type and hold [N1, {D}] per token (got {q.dtype} {tuple(q.shape)})")
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=kind, device=device)
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif q_out.shape != q.shape or q_out.dtype is not kind or not q_out.is_contiguous():
             raise ValueError("q_out must be contiguous and of q's shape and type")
     elif q_out is not None:
