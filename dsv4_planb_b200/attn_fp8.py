@@ -18,6 +18,7 @@ from .api import _dense16, _dtype_code, _pool16, _ptr, _scenario, _workspace
 from .cache import _eager, _int32, _ops, _raw_stream, _refuse_grad
 
 KERNELS = {"auto": 0, "simt": 1, "tc": 2}
+_INT32 = 2**31 - 1  # no position lies beyond it
 
 
 @functools.lru_cache(maxsize=512)
@@ -206,8 +207,8 @@ def sparse_attn_sharedkv_fp8(
     elif return_softmax_lse:
         lse = sums = q.new_empty((*tokens, N1), dtype=torch.float32)
     call = (q, ori_kv, ori_kv_scale, cmp_kv, cmp_kv_scale, cmp_sparse_indices, ori_block_table, cmp_block_table,
-            cu_seqlens_q, seqused_kv, sinks, float(softmax_scale), 4 if cmp_ratio is None else int(cmp_ratio),
-            int(ori_win_left), int(ori_first), layout_q, Dv, kernel, bool(check_status), out, lse)
+            cu_seqlens_q, seqused_kv, sinks, float(softmax_scale), 4 if cmp_ratio is None else min(int(cmp_ratio), _INT32),
+            min(int(ori_win_left), _INT32), min(int(ori_first), _INT32), layout_q, Dv, kernel, bool(check_status), out, lse)
     if _eager(q):
         _launch(*call)
     else:

@@ -187,8 +187,8 @@ def sharedkv_cache_append(
     past the table are skipped (``check_status`` synchronises and raises on the last two and on a block
     without a valid scale).  In an 8-bit cache a block takes the smallest power-of-two scale that its rows
     need when its first row arrives, and raises it when later rows need more; the rows already there are
-    then rounded to the new scale.  A block must receive rows of one request only per call.  No host
-    synchronisation; graph-capturable.  No backward pass.
+    then rounded to the new scale.  A block may take rows of one request, and of one place of its table, per
+    call.  No host synchronisation; graph-capturable.  No backward pass.
     """
     assert layout_q in ("TND", "BSND"), f"unsupported layout_q={layout_q!r}"
     if not cache.is_cuda:
@@ -243,7 +243,7 @@ def sharedkv_cache_append(
     elif q_out is not None:
         raise ValueError("q_out goes with q")
     call = (kv, cache, cache_scale, block_table, seqused_kv, cu_seqlens_q, rope_table, bool(rope_interleaved),
-            int(rope_step), None if q_out is q else q, q_out, layout_q, bool(check_status))
+            min(int(rope_step), 2**31 - 1), None if q_out is q else q, q_out, layout_q, bool(check_status))
     if _eager(cache):
         _append(*call)
     else:

@@ -345,6 +345,72 @@ def test_two_calls_at_once(cuda_device):
             assert torch.equal(o, want[i][0]) and torch.equal(l, want[i][1])
 
 
+def test_two_graphs_at_once(cuda_device):
+    """Captured calls on two streams, replayed together: a split plan and one of whole tokens."""
+    ms = [make([1] * n, [1900 + 7 * i for i in range(n)], N1=64, K=500, seed=s) for n, s in ((5, 22), (80, 23))]
+    held = [kwargs(m) for m in ms]
+    want = [run(m) for m in ms]
+    torch.cuda.synchronize()
+    graphs, got, streams = [], [], [torch.cuda.Stream() for _ in ms]
+    for m, kw in zip(ms, held):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            got.append(sparse_attn_sharedkv_fp8(m["q"], **kw))
+    for _ in range(6):
+        for s, gr in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                gr.replay()
+    torch.cuda.synchronize()
+    for (o, l), (wo, wl) in zip(got, want):
+        assert torch.equal(o, wo) and torch.equal(l, wl)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_widest_arguments(cuda_device, kernel):
+    """A window, first positions or a ratio past every position say "all" or "none", however large."""
+    m = make([2, 1], [300, 900], N1=20, K=60, first=3, seed=24)
+    for small, wide in ((dict(ori_win_left=5000), dict(ori_win_left=2**40)), (dict(ori_first=5000), dict(ori_first=2**35)),
+                        (dict(cmp_ratio=5000), dict(cmp_ratio=2**33 + 4))):
+        a, b = run(m, kernel=kernel, **small), run(m, kernel=kernel, **wide)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def draw(seed):
+    rng = np.random.default_rng(seed)
+    B = int(2 ** rng.uniform(0, 4))
+    new = [int(rng.integers(0, 4)) for _ in range(B - 1)] + [1]
+    kv = [max(int(2 ** rng.uniform(0, 12)), n) for n in new]
+    scenario = int(rng.integers(1, 4))
+    return make(new, kv, N1=int(rng.integers(1, 129)), D=int(rng.choice([512, 576])), K=int(rng.integers(1, 900)), scenario=scenario,
+                ratio=int(rng.choice([2, 4, 7, 128])), win_left=int(rng.integers(0, 700)), first=int(rng.integers(0, 6)),
+                bs=int(rng.choice([1, 16, 48, 64, 128])), skips=scenario == 3 and seed % 2 == 0, seed=seed)
+
+
+@pytest.mark.parametrize("seed", range(100, 112))
+def test_drawn(cuda_device, seed):
+    m = draw(seed)
+    check(m, *run(m, check_status=True), tokens=range(min(len(m["where"]), 10)))
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_rows_past_32_bits(cuda_device, kernel):
+    """Blocks whose rows lie more than 2^32 bytes into the pool, written and read."""
+    D, bs, blocks = 576, 128, 2 ** 32 // (576 * 128) + 40
+    cache = torch.zeros((blocks, bs, 1, D), dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    scale = torch.ones((blocks, 1), device="cuda")
+    m = make([300], [300], N1=24, scenario=1, seed=25)
+    kv = torch.randn((300, D), generator=torch.Generator().manual_seed(25)).to(torch.bfloat16).cuda()
+    table = np.array([[blocks - 1, blocks - 7, blocks - 2]], np.int32)
+    call = dict(cu_seqlens_q=torch.tensor([0, 300], dtype=torch.int32).cuda(), seqused_kv=torch.tensor([300], dtype=torch.int32).cuda())
+    sharedkv_cache_append(kv, cache=cache, cache_scale=scale, block_table=torch.from_numpy(table).cuda(), check_status=True, **call)
+    got = ref.gather(cache[:, :, 0], scale, table[0], list(range(300))).cpu()
+    step = scale[:, 0].double().cpu()[torch.from_numpy(table[0]).long()[torch.arange(300) // bs]]
+    x = kv.double().cpu()
+    assert ((got - x).abs() <= 2.0 ** -4 * x.abs() + 2.0 ** -10 * step[:, None]).all()
+    m["ori"] = (cache, scale, table)
+    check(m, *run(m, kernel=kernel, check_status=True), tokens=[0, 1, 127, 128, 299])
+
+
 @pytest.mark.parametrize("tokens", [2, 90])
 def test_graph(cuda_device, tokens):
     """A captured call replayed on new queries, indices, lengths and tables."""

@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 import torch
 
+from dsv4_planb_b200.api import sparse_attn_sharedkv
 from dsv4_planb_b200.cache import rope_table, sharedkv_cache_append
 from tests import _cache_ref as ref
 
@@ -279,6 +280,43 @@ def test_other_stream_and_graph(cuda_device):
     torch.cuda.synchronize()
     check(m, cache, scale, rope)
     check_q(m["q"], out, rope, m["where"], True, 1)
+
+
+def test_rows_past_32_bits(cuda_device):
+    """16-bit rows more than 2^32 bytes into the pool."""
+    D, bs, blocks = 512, 64, 2 ** 32 // (512 * 64 * 2) + 5
+    cache = torch.zeros((blocks, bs, 1, D), dtype=torch.bfloat16, device="cuda")
+    kv = torch.randn((90, D), generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).cuda()
+    table = torch.tensor([[blocks - 2, blocks - 1]], dtype=torch.int32).cuda()
+    sharedkv_cache_append(kv, cache=cache, block_table=table, cu_seqlens_q=torch.tensor([0, 90], dtype=torch.int32).cuda(),
+                          seqused_kv=torch.tensor([100], dtype=torch.int32).cuda(), check_status=True)
+    assert torch.equal(cache[blocks - 2:].reshape(2 * bs, D)[10:100], kv)
+    assert not cache[:blocks - 2].any()
+
+
+def test_rows_read_by_the_16_bit_attention(cuda_device):
+    """Rows appended in two calls are what the attention reads: the same bits laid out by hand in another
+    order of blocks give the same result."""
+    D, bs, lens = 512, 64, [150, 70]
+    g = torch.Generator().manual_seed(4)
+    rope = rope_table(200, 64)
+    cache = torch.zeros((8, bs, 1, D), dtype=torch.bfloat16, device="cuda")
+    table = torch.tensor([[5, 0, 3], [2, 7, -1]], dtype=torch.int32)
+    for new, done in (([140, 1], [140, 1]), ([10, 69], lens)):
+        cu = torch.tensor([0, new[0], sum(new)], dtype=torch.int32).cuda()
+        seq = torch.tensor(done, dtype=torch.int32).cuda()
+        kv = torch.randn((sum(new), D), generator=g).to(torch.bfloat16).cuda()
+        q = sharedkv_cache_append(kv, cache=cache, block_table=table.cuda(), cu_seqlens_q=cu, seqused_kv=seq, rope_table=rope,
+                                  q=torch.randn((sum(new), 16, D), generator=g).to(torch.bfloat16).cuda())
+    other = torch.tensor([[1, 6, 4], [3, 2, -1]], dtype=torch.int32)
+    moved = torch.zeros_like(cache)
+    for b, n in enumerate(lens):
+        for i in range((n + bs - 1) // bs):
+            moved[other[b, i]] = cache[table[b, i]]
+    outs = [sparse_attn_sharedkv(q, ori_kv=c, ori_block_table=t.cuda(), cu_seqlens_q=cu, seqused_kv=seq, sinks=torch.zeros(16).cuda(),
+                                 softmax_scale=D ** -0.5, v_head_dim=D) for c, t in ((cache, table), (moved, other))]
+    outs = [o[0] if isinstance(o, tuple) else o for o in outs]
+    assert outs[0].abs().sum() > 0 and torch.equal(*outs)
 
 
 def test_compiled(cuda_device):
