@@ -6,7 +6,7 @@
 // scenario 3 it also maps the token's compressed indices to physical rows: the scan of a row of
 // indices stops at the first -1 or after min(K, limit) slots, skips what is out of range, keeps
 // duplicates and slot order.  Latency bound: its loads of the indices start before the request of
-// the row is known.
+// the row is known.  About 3 us of a decode step's 29, most of them beside the launch of the attention.
 
 #include "sas_fp8_attn.cuh"
 

@@ -42,6 +42,17 @@
 //     where its lo is subnormal are 2^-15.75 of it), and O is rescaled 256 columns at a time, each as
 //     soon as the last tile's product of these columns is complete.
 //
+// Whole calls: 64 tokens of 2176 keys, 128 heads of 576 dims: 65 us (38.8 GFLOP, 98.6 MB); 2048 such
+// tokens: 1.07 ms, 930 TFLOP/s, and 1.21 ms once the card is at its power limit (1.7 GHz).  A tile takes
+// 2800 cycles: 1960 of QK issue, the rest mostly waits for an S to come back: the two passes of the softmax
+// are 1370 and 2140 cycles, so that QK and softmax of two tiles, which share an S buffer, take 5700, and a
+// third S has no room.  The gather warps are busy for 2650.  A unit adds 6500 cycles for the split of Q
+// (conversions and byte shuffles at half and quarter rate), and the first tile 8 us of latency.  What did
+// not help: 6 gather warps, or a warp of its own for the row lookups (they take the softmax's issue slots,
+// 3 and 4 % slower); a tile taken in the last tile's frame and redone where that does not hold (some of 128
+// heads mostly rises, 20 %); TMEM loads a step ahead or of 32 columns (0 to 5 %: longer loops; the roles of an
+// SM share its instruction caches); a staging of 8 boxes in the epilogue.
+//
 // Keys of a token: first positions, then the window, then the compressed rows.  Slots without a key
 // carry weight 0 (log2 s = -inf); they and rows of unmapped blocks are filled with zeros.
 //
@@ -65,7 +76,7 @@ using namespace sas_fp8;
 
 constexpr int kBK = 96;              // keys per tile
 constexpr int kSlab = kBK * 128;     // 128 dims of a tile's rows
-constexpr int kStages = 3;
+constexpr int kStages = 3, kVStages = 2;  // of the two CTAs' rings
 constexpr int kDv = 512, kVSlabs = kDv / 128;
 constexpr int kVStage = kVSlabs * kSlab, kKStage = kVStage + kBK * 64;  // K: dims 512 .. 575 as 64-byte rows behind
 constexpr int kQChunk = 128 * 128, kQPerStage = 3;  // raw Q: 64 bf16 dims of 128 heads; chunks per stage of the K ring
@@ -88,6 +99,10 @@ constexpr int kMaxPieces = 64;
 // puts the codes in the weights' place: 96 hi and 32 lo in the first row, the other 64 lo in the second.
 constexpr int kMsgLo = 128 * 128, kMsgStats = kMsgLo + 128 * 64, kMsgBytes = kMsgStats + 1024;
 
+// Messages under way.  A slot is held from its copy's start over the split to the end of its product, about
+// 5000 cycles: with two slots that alone took 2500 a tile (64 tokens 67 us; 65 with four).
+constexpr int kSlots = 4;
+
 struct KeyConst {
     float s[kBK];   // scale; 0: a zero row
     float ls[kBK];  // log2 s; -60 for zero rows (their values do not count), -inf: no key
@@ -96,7 +111,7 @@ struct KeyConst {
 struct Hdr {
     uint64_t full[kStages], empty[kStages], s_full[2], s_free[2], q_raw, q_full, c_full[kConsts];
     uint64_t x_bar[4][2], m_bar[4][2], l_bar[4];  // of the two warps that share 32 heads
-    uint64_t p_full[2], p_ready[2], p_empty[2], p_sent[2], o_full, o_empty, rs_done[2], pv_done[2];
+    uint64_t p_full[kSlots], p_ready[kSlots], p_empty[kSlots], p_sent[2], o_full, o_empty, rs_done[2], pv_done[2][kSlots];
     uint64_t tq_full[kTq], tq_empty[kTq];
     volatile int tq[kTq];
     uint32_t tmem_base;
@@ -110,8 +125,8 @@ constexpr int kScoreMsgs = (kConstOff + kConsts * (int)sizeof(KeyConst) + 1023) 
 constexpr int kScoreRing = kScoreMsgs + 2 * kMsgBytes;
 constexpr int kScoreSmem = kScoreRing + kStages * kKStage;
 constexpr int kOutRing = kHdr;
-constexpr int kOutMsgs = kOutRing + kStages * kVStage;
-constexpr int kOutStage = kOutMsgs + 2 * kMsgBytes;  // epilogue staging: 64 bytes of 32 heads per warp
+constexpr int kOutMsgs = kOutRing + kVStages * kVStage;
+constexpr int kOutStage = kOutMsgs + kSlots * kMsgBytes;  // epilogue staging: 64 bytes of 32 heads per warp
 constexpr int kWarpSlab = 32 * 64;
 constexpr int kOutSmem = kOutStage + kSoftWarps * kWarpSlab;
 constexpr int kSmemBytes = (kScoreSmem > kOutSmem ? kScoreSmem : kOutSmem) + 1024;  // + alignment slack
@@ -284,7 +299,7 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32
 template <bool kScore>
 __device__ void producer(const TcArgs &p, const Sync &sy, const CUtensorMap *q_map, uint8_t *ring, Hdr *hd,
                          KeyConst *consts) {
-    constexpr uint32_t kStageBytes = kScore ? kKStage : kVStage;
+    constexpr uint32_t kStageBytes = kScore ? kKStage : kVStage, kRing = kScore ? kStages : kVStages;
     const int w = (threadIdx.x >> 5) - kProdWarp0, lane = threadIdx.x & 31;
     const bool holds = lane < kRows;
     const int key_at = w * kRows + (holds ? lane : 0);
@@ -297,7 +312,7 @@ __device__ void producer(const TcArgs &p, const Sync &sy, const CUtensorMap *q_m
     uint32_t st = 0, phase = 1, tiles = 0, bits = 0;  // stage, and the parity its empty barrier is waited on
     int pend = -1;
     auto next = [&] {
-        if (++st == kStages) {
+        if (++st == kRing) {
             st = 0;
             phase ^= 1;
         }
@@ -526,20 +541,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         init(&hd->x_bar[0][0], 8, 1);
         init(&hd->m_bar[0][0], 8, 1);
         init(hd->l_bar, 4, 1);
-        init(hd->p_full, 2, 1);
-        init(hd->p_empty, 2, 1);
+        init(hd->p_full, kSlots, 1);
+        init(hd->p_empty, kSlots, 1);
         init(hd->p_sent, 2, 1);
-        init(hd->p_ready, 2, kSoftWarps);
+        init(hd->p_ready, kSlots, kSoftWarps);
         init(&hd->o_full, 1, 1);
         init(&hd->o_empty, 1, kSoftWarps);
         init(hd->rs_done, 2, kSoftWarps);
-        init(hd->pv_done, 2, 1);
+        init(&hd->pv_done[0][0], 2 * kSlots, 1);
         init(hd->tq_full, kTq, 1);
         init(hd->tq_empty, kTq, kReaders);
         hd->abort = 0;
         // the output CTA expects the first message of each P slot (bulk copies complete it)
         if (rank == 1)
-            for (int i = 0; i < 2; ++i) mbar_arrive_expect_tx(smem_u32(&hd->p_full[i]), kMsgBytes);
+            for (int i = 0; i < kSlots; ++i) mbar_arrive_expect_tx(smem_u32(&hd->p_full[i]), kMsgBytes);
         mbar_fence_init();
     }
     if (warp == kMmaWarp) {
@@ -645,8 +660,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint8_t *stage = smem + kScoreMsgs + g * kMsgBytes;
             const uint32_t row1 = smem_u32(stage) + h * 128, row2 = smem_u32(stage) + kMsgLo + h * 64;
             const uint32_t sw1 = (h & 7) << 4, sw2 = ((h >> 1) & 3) << 4;
-            const uint32_t peer_msg = map_to_cta(smem_u32(smem + kOutMsgs), 1) + g * kMsgBytes;
-            const uint32_t peer_full = map_to_cta(smem_u32(&hd->p_full[g]), 1);
+            const uint32_t peer_msgs = map_to_cta(smem_u32(smem + kOutMsgs), 1), peer_full0 = map_to_cta(smem_u32(hd->p_full), 1);
             const float sink = head && p.sinks ? p.sinks[h] : -INFINITY;
             uint32_t sc0 = 0, qc = 0, lc = 0, mine = 0;  // the unit's first tile; units; units of two tiles or more; own tiles
             for (uint32_t k = 0;; ++k) {
@@ -674,6 +688,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int e = (sc0 & 1) == (uint32_t)g ? 0 : 1; e < nt; e += 2, ++mine) {
                     const uint32_t sc = sc0 + e;
                     if (!wait_on(sy, smem_u32(&hd->c_full[sc % kConsts]), (sc / kConsts) & 1)) goto done;
+                    // the maximum so far comes from the other warp's tile and goes on to its next
+                    if (sc > 0 && !wait_on(sy, smem_u32(&hd->m_bar[warp & 3][g ^ 1]), ((sc - 1) >> 1) & 1)) goto done;
+                    const float before = e > 0 ? hd->m[g ^ 1][h] : -INFINITY;
                     if (!wait_on(sy, smem_u32(&hd->s_full[g]), mine & 1)) goto done;
                     tc_fence_after();
                     const KeyConst &c = consts[sc % kConsts];
@@ -694,22 +711,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                     const float mx = fmaxf(mx0, mx1);
-                    // the maximum so far comes from the other warp's tile and goes on to its next
-                    float mn = mx, alpha = 1.f;
-                    if (sc > 0 && !wait_on(sy, smem_u32(&hd->m_bar[warp & 3][g ^ 1]), ((sc - 1) >> 1) & 1)) goto done;
-                    if (e > 0) {
-                        const float before = hd->m[g ^ 1][h];
-                        mn = mx > before + kRise ? mx : before;
-                        if (mn != before) alpha = exp2f(before - mn);
-                    }
+                    const float mn = e == 0 || mx > before + kRise ? mx : before;
                     hd->m[g][h] = mn;
                     __syncwarp();
                     if (lane == 0) mbar_arrive(smem_u32(&hd->m_bar[warp & 3][g]));
-                    if (mn != m) {
-                        l *= exp2f(m - mn);  // 0 before the first tile
-                        m = mn;
-                    }
-                    const float mb = m - (kTop - kRise);
+                    const float mb = mn - (kTop - kRise);
                     const uint64_t mb2 = pack2(-mb, -mb);
                     // the last message has arrived, so its copies have left the staging buffer
                     if (!wait_on(sy, smem_u32(&hd->p_sent[g]), (mine & 1) ^ 1, true)) goto done;
@@ -749,6 +755,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(smem_u32(&hd->s_free[g]));
+                    float alpha = e > 0 && mn != before ? exp2f(before - mn) : 1.f;
+                    if (mn != m) {
+                        l *= exp2f(m - mn);  // 0 before the first tile
+                        m = mn;
+                    }
                     const float2 s0 = unpack2(sum0), s1 = unpack2(sum1);
                     l += (s0.x + s0.y) + (s1.x + s1.y);
                     float fin = 0.f;
@@ -780,8 +791,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     *reinterpret_cast<float2 *>(stage + kMsgStats + h * 8) = make_float2(lane == 0 && some ? -alpha : alpha, fin);
                     fence_proxy_async_smem();
                     // only now must the peer be done with the slot: S has been free since the second pass
-                    if (!wait_on(sy, smem_u32(&hd->p_empty[g]), (mine & 1) ^ 1, true)) goto done;
+                    const uint32_t ps = sc % kSlots;
+                    if (!wait_on(sy, smem_u32(&hd->p_empty[ps]), ((sc / kSlots) & 1) ^ 1, true)) goto done;
                     if (lane == 0) {
+                        const uint32_t peer_msg = peer_msgs + ps * kMsgBytes, peer_full = peer_full0 + ps * 8;
                         const uint32_t w32 = (warp & 3) * 32, src = smem_u32(stage);
                         bulk_to_peer(peer_msg + w32 * 128, src + w32 * 128, 32 * 128, peer_full);
                         bulk_to_peer(peer_msg + kMsgLo + w32 * 64, src + kMsgLo + w32 * 64, 32 * 64, peer_full);
@@ -792,7 +805,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (nt > 1) ++lc;
             }
             // the last message must have been read before this CTA may exit
-            if (mine > 0 && !wait_on(sy, smem_u32(&hd->p_empty[g]), (mine - 1) & 1, true)) goto done;
+            if (sc0 > 0 && !wait_on(sy, smem_u32(&hd->p_empty[(sc0 - 1) % kSlots]), ((sc0 - 1) / kSlots) & 1, true)) goto done;
         }
     } else {
         // ======================= output CTA =======================
@@ -811,8 +824,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!wait_on(sy, smem_u32(&hd->o_empty), (oc & 1) ^ 1)) goto done;
                 ++oc;
                 for (int j = it.j0; j < it.j1; ++j, ++pc) {
-                    const int ps = pc & 1;
-                    if (!wait_on(sy, smem_u32(&hd->p_ready[ps]), (pc >> 1) & 1)) goto done;
+                    const int ps = pc % kSlots;
+                    if (!wait_on(sy, smem_u32(&hd->p_ready[ps]), (pc / kSlots) & 1)) goto done;
                     const uint8_t *msg = msgs + ps * kMsgBytes;
                     const bool last = j == it.j1 - 1, rescale = j > it.j0 && some_alpha(msg);
                     if (!wait_on(sy, smem_u32(&hd->full[st]), phase)) goto done;
@@ -831,7 +844,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 mma8_ss(d, a1 + 2 * i, b + 256 * i, idesc, (j > it.j0 || i > 0) ? 1u : 0u);
                                 mma8_ss(d, i == 0 ? a1 + 6 : a2 + 2 * (i - 1), b + 256 * i, idesc, 1u);
                             }
-                            tc_commit(smem_u32(&hd->pv_done[c]));
+                            tc_commit(smem_u32(&hd->pv_done[c][ps]));
                         }
                         __syncwarp();
                     }
@@ -842,7 +855,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (last) tc_commit(smem_u32(&hd->o_full));
                     }
                     __syncwarp();
-                    if (++st == kStages) {
+                    if (++st == kVStages) {
                         st = 0;
                         phase ^= 1;
                     }
@@ -869,16 +882,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 float fin = 1.f;
                 for (int j = it.j0; j < it.j1; ++j, ++pc) {
-                    const int ps = pc & 1;
+                    const int ps = pc % kSlots;
                     uint8_t *msg = msgs + ps * kMsgBytes;
-                    if (!wait_on(sy, smem_u32(&hd->p_full[ps]), (pc >> 1) & 1, true)) goto done;
+                    if (!wait_on(sy, smem_u32(&hd->p_full[ps]), (pc / kSlots) & 1, true)) goto done;
                     const float2 stat = reinterpret_cast<const float2 *>(msg + kMsgStats)[h];
                     const bool rescale = j > it.j0 && some_alpha(msg);
                     fin = stat.y;
-                    if (g == ps) {  // this warp's tile: its 32 heads' weights into hi and lo codes, in place
+                    if (g == (int)(pc & 1)) {  // this warp's tile: its 32 heads' weights into hi and lo codes, in place
                         if (threadIdx.x == g * 128) {
                             mbar_arrive_expect_tx(smem_u32(&hd->p_full[ps]), kMsgBytes);  // the next message
-                            mbar_arrive_remote(map_to_cta(smem_u32(&hd->p_sent[ps]), 0));
+                            mbar_arrive_remote(map_to_cta(smem_u32(&hd->p_sent[g]), 0));
                         }
                         uint8_t *row1 = msg + h * 128, *row2 = msg + kMsgLo + h * 64;
                         uint4 x[12], y[12];
@@ -907,8 +920,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const bool any = __any_sync(0xffffffffu, a != 1.f);
 #pragma unroll 1
                     for (int c = 0; c < 2; ++c) {
-                        // the product of the tile before, of these columns
-                        if (!wait_on(sy, smem_u32(&hd->pv_done[c]), (pc - 1) & 1)) goto done;
+                        // the product of the tile before, of these columns (a barrier per slot: the products of the
+                        // three tiles before may be outstanding, which one barrier's two phases cannot tell apart)
+                        if (!wait_on(sy, smem_u32(&hd->pv_done[c][(pc - 1) % kSlots]), ((pc - 1) / kSlots) & 1)) goto done;
                         if (any) {
                             tc_fence_after();
 #pragma unroll 1
@@ -1013,7 +1027,8 @@ done:
 // Pieces of split tokens, and the sink: out = sum_i 2^(own_i - lse2) o_i with o_i normalised within its
 // piece and own_i the log2 of the piece's weight sum; lse2 = log2 (sum_i 2^own_i + 2^sink2).
 // Block (t, h), thread = 4 columns.  Latency bound: the record, the sums and the first pieces' columns
-// are loaded together, before the number of pieces is known (the slots of all P exist).
+// are loaded together, before the number of pieces is known (the slots of all P exist).  About 4 us for
+// 23 pieces; two groups of threads with 12 pieces each ahead took 0.5 us off.
 __global__ void __launch_bounds__(kDv / 4) fp8_combine_kernel(const TcArgs p) {
     constexpr int kAhead = 8;
     asm volatile("griddepcontrol.wait;" ::: "memory");
