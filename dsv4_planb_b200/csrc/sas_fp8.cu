@@ -20,7 +20,9 @@ constexpr int kPer = 8;
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // Record of flat row t (warp-uniform; every lane calls).  `limit`: compressed rows below it are visible.
-__device__ __forceinline__ void make_record(const Args &p, int t, int32_t (&r)[TR_INTS], int &limit) {
+// `found(b)` runs as soon as the row's request is known (-1: none).
+template <class F>
+__device__ __forceinline__ void make_record(const Args &p, int t, int32_t (&r)[TR_INTS], int &limit, F found) {
     int b, s = 0, n = 0;
     if (p.cu) {
         b = find_request(p.cu, p.B, t);
@@ -35,6 +37,7 @@ __device__ __forceinline__ void make_record(const Args &p, int t, int32_t (&r)[T
         if (b >= p.B) b = -1;
         else n = p.act_q ? min(__ldg(p.act_q + b), p.q_rows) : p.q_rows;
     }
+    found(b);
     const bool valid = b >= 0 && s < n;
     const int64_t pos = valid ? (int64_t)__ldg(p.act_kv + b) - n + s : -1;
     const int g = (int)max(pos, (int64_t)-1);
@@ -65,7 +68,7 @@ __global__ void __launch_bounds__(kThreads) resolve_kernel(Args p) {
     if (t >= p.T) return;
     int32_t r[TR_INTS];
     int limit;
-    make_record(p, t, r, limit);
+    make_record(p, t, r, limit, [](int) {});
     if ((threadIdx.x & 31) == 0) store_record(p, t, r);
 }
 
@@ -92,7 +95,16 @@ __global__ void __launch_bounds__(kThreads) resolve_rows_kernel(Args p) {
     load(0);
     int32_t r[TR_INTS];
     int limit;
-    make_record(p, t, r, limit);
+    // the table's entries need the request only: their loads run beside that of its length
+    int32_t phys[kPer];
+    auto look_up = [&](int b) {
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            const int blk = max(v[k], 0) / p.cmp_bs;
+            phys[k] = b >= 0 && blk < p.cmp_table_len ? __ldg(p.cmp_bt + (int64_t)b * p.cmp_table_len + blk) : -2;
+        }
+    };
+    make_record(p, t, r, limit, look_up);
     if (tid == 0) {
         stop_s = min(p.K, limit);
         bits_s = 0;
@@ -101,7 +113,10 @@ __global__ void __launch_bounds__(kThreads) resolve_rows_kernel(Args p) {
     int kept = 0;
     uint32_t bits = 0;
     for (int base = 0; base < p.K; base += kThreads * kPer) {
-        if (base > 0) load(base);
+        if (base > 0) {
+            load(base);
+            look_up(r[TR_B]);
+        }
         __syncthreads();
         if (base >= stop_s) break;
         const int i0 = base + tid * kPer;
@@ -120,7 +135,9 @@ __global__ void __launch_bounds__(kThreads) resolve_rows_kernel(Args p) {
             if (i0 + k < stop) {
                 if (v[k] < -1) bits |= SAS_STATUS_BAD_INDEX;
                 if (v[k] >= 0 && v[k] < limit) {
-                    row[k] = paged_row(p.cmp_bt, r[TR_B], p.cmp_table_len, p.cmp_bs, p.cmp_block_num, v[k], bits);
+                    const bool bad = phys[k] < -1 || phys[k] >= p.cmp_block_num;
+                    if (bad) bits |= SAS_STATUS_BAD_BLOCK;
+                    row[k] = bad || phys[k] < 0 ? -1 : phys[k] * p.cmp_bs + v[k] % p.cmp_bs;
                     ++cnt;
                 }
             }
