@@ -318,15 +318,14 @@ template <typename T> __global__ void __launch_bounds__(kThreads) append8_kernel
     int rows = min(sp.pos + sp.n - first, p.bs) - o0;
     const char *src = p.kv + ((int64_t)sp.row + (first + o0 - sp.pos)) * p.kv_stride * 2;
     const int64_t phys = block_of(p, b, blk);
-    const bool any = phys >= 0;
-    float old = any && o0 > 0 ? __ldg(p.scale + phys) : 0.f;
     const float *cs0 = p.rope + (int64_t)(first + o0) * p.step * p.R;
     if (p.R > 0) {  // rows past the table's end have no place
         const int last = (int)min(((int64_t)p.rope_rows + p.step - 1) / p.step - (first + o0), (int64_t)rows);
         if (last < rows) sas::set_status(p.status, SAS_STATUS_BAD_POSITION);
         rows = max(last, 0);
     }
-    if (!any) rows = 0;
+    if (phys < 0 || rows == 0) return;  // no row has a place: the block and its scale stay (in the whole cluster)
+    float old = o0 > 0 ? __ldg(p.scale + phys) : 0.f;
     const int me = (int)rank * kThreads + tid, all = (int)ranks * kThreads;
     const int plain = (p.D - p.R) / 16, turned = p.R / 8;
     const int64_t src_bytes = p.kv_stride * 2;
@@ -398,7 +397,6 @@ template <typename T> __global__ void __launch_bounds__(kThreads) append8_kernel
     } else {
         __syncthreads();  // every warp has read the old scale
     }
-    if (!any) return;
     const float need = sas_fp8::scale_for(amax);
     float now = need;
     if (o0 > 0) {

@@ -235,6 +235,18 @@ def test_skipped_rows(cuda_device, pool):
     check(m, *run(m, rope)[:2], rope)
 
 
+@pytest.mark.parametrize("q_lens,kv_lens", [([3], [130]), ([1], [200]), ([600], [700])])
+def test_blocks_past_the_angles_stay(cuda_device, q_lens, kv_lens):
+    """A block none of whose rows has angles keeps its contents and its scale."""
+    m = make(q_lens, kv_lens, seed=10)
+    rope = rope_table(128, 64)
+    cache, scale, _ = run(m, rope)
+    check(m, cache, scale, rope)
+    phys = int(m["table"][0, 1])
+    assert torch.equal(cache[phys].cpu().view(torch.uint8), m["cache"][phys].view(torch.uint8))
+    assert torch.equal(scale.cpu().reshape(-1)[phys], m["scale"].reshape(-1)[phys])
+
+
 @pytest.mark.parametrize("old", [0.0, -1.0, math.nan, math.inf])
 def test_block_without_scale(cuda_device, old):
     m = make([1], [3], seed=4)
