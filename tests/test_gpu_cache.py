@@ -257,6 +257,26 @@ def test_block_without_scale(cuda_device, old):
         run(m, None, check_status=True)
 
 
+@pytest.mark.parametrize("q_lens", [[1] * 1500, [0, 3] * 400 + [700], [40] * 33, [0] * 40 + [1] + [0] * 70], ids=["1500x1", "gaps", "33x40", "one"])
+def test_many_requests(cuda_device, q_lens):
+    """Every request's runs are found among many, with requests that bring nothing between them."""
+    rng = np.random.default_rng(31)
+    m = make(q_lens, [n + int(rng.integers(0, 150)) for n in q_lens], D=64, bs=16, seed=31)
+    rope = rope_table(900, 64)
+    check(m, *run(m, rope, check_status=True)[:2], rope)
+
+
+@pytest.mark.parametrize("pool", ["fp8", "bf16"])
+def test_rows_before_the_first_request(cuda_device, pool):
+    """Flat rows in front of the first request and behind the last belong to none."""
+    m = make([60, 2], [100, 300], bs=16, pool=pool, seed=32)
+    rope, front = rope_table(300, 64), 35
+    kv = torch.full((front + 62 + 9, m["kv"].shape[1]), 7.0, dtype=m["kv"].dtype)
+    kv[front:front + 62] = m["kv"]
+    m["cu"] += front
+    check(m, *run(m, rope, kv=kv.cuda(), check_status=True)[:2], rope)
+
+
 def test_no_rows(cuda_device):
     m = make([0, 0], [4, 0], seed=4)
     check(m, *run(m, rope_table(8, 64), check_status=True)[:2], None)
