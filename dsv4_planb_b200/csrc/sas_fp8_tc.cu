@@ -80,6 +80,7 @@ constexpr int kStages = 3, kVStages = 2;  // of the two CTAs' rings
 constexpr int kDv = 512, kVSlabs = kDv / 128;
 constexpr int kVStage = kVSlabs * kSlab, kKStage = kVStage + kBK * 64;  // K: dims 512 .. 575 as 64-byte rows behind
 constexpr int kQChunk = 128 * 128, kQPerStage = 3;  // raw Q: 64 bf16 dims of 128 heads; chunks per stage of the K ring
+constexpr int kQStages = (576 / 64 + kQPerStage - 1) / kQPerStage;
 constexpr int kSoftWarps = 8, kMmaWarp = 8, kProdWarp0 = 9, kProdWarps = 4;
 constexpr int kRows = kBK / kProdWarps;
 static_assert(kRows % 8 == 0 && kProdWarps == 4, "whole swizzle periods, 32 heads of Q a warp");
@@ -109,7 +110,7 @@ struct KeyConst {
 };
 
 struct Hdr {
-    uint64_t full[kStages], empty[kStages], s_full[2], s_free[2], q_raw, q_full, c_full[kConsts];
+    uint64_t full[kStages], empty[kStages], s_full[2], s_free[2], q_raw[kQStages], q_full, c_full[kConsts];
     uint64_t x_bar[4][2], m_bar[4][2], l_bar[4];  // of the two warps that share 32 heads
     uint64_t p_full[kSlots], p_ready[kSlots], p_empty[kSlots], p_sent[2], o_full, o_empty, rs_done[2], pv_done[2][kSlots];
     uint64_t tq_full[kTq], tq_empty[kTq];
@@ -339,7 +340,7 @@ __device__ void producer(const TcArgs &p, const Sync &sy, const CUtensorMap *q_m
         int u = -1;
         if (!(writer ? tq_publish(p, sy, k, pend, u) : tq_read(p, sy, kScore ? 0 : 1, k, u))) return;
         if (u < 0) break;
-        // q is older than the resolve kernel: the first unit's is loaded beside it, whatever the unit holds
+        // q is older than the resolve kernel: the first unit's is loaded and split beside it, whatever the unit holds
         if (kScore && k == 0 && !load_q(u % p.T)) return;
         if (k == 0) wait_resolved();
         const Item it = load_unit(p, u);
@@ -448,8 +449,11 @@ __device__ float split_q(const Sync &sy, Hdr *hd, uint32_t trow, int chunks, uin
     const int warp = threadIdx.x >> 5, g = warp >> 2, h = threadIdx.x & 127;
     __nv_bfloat162 top = __floats2bfloat162_rn(0.f, 0.f);
 #pragma unroll 1
-    for (int c = g; c < chunks; c += 2) {
+    for (int c = g; c < chunks; c += 2) {  // as the chunks come
         uint32_t r[32];
+        ok = wait_on(sy, smem_u32(&hd->q_raw[c / kQPerStage]), parity);
+        if (!ok) return 0.f;
+        tc_fence_after();
         tmem_ld32(trow + c * 32, r);
         tc_wait_ld();
 #pragma unroll
@@ -535,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         init(hd->empty, kStages, 1);
         init(hd->s_full, 2, 1);
         init(hd->s_free, 2, 4);
-        init(&hd->q_raw, 1, 1);
+        init(hd->q_raw, kQStages, 1);
         init(&hd->q_full, 1, kSoftWarps);
         init(hd->c_full, kConsts, kProdWarps);
         init(&hd->x_bar[0][0], 8, 1);
@@ -565,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     cluster_sync();  // both CTAs' barriers are initialised before any remote arrive
     tc_fence_after();
-    if (warp < kProdWarp0) wait_resolved();  // the gather warps wait later
+    if (rank == 1 && warp < kProdWarp0) wait_resolved();  // the others wait when they need a record
     if (p.P > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem = hd->tmem_base;
     Sync sy{&hd->abort, p.status, map_to_cta(smem_u32((const void *)&hd->abort), rank ^ 1u), hd->tq_full, hd->tq_empty,
@@ -591,16 +595,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 int u;
                 if (!tq_read(p, sy, rank, k, u)) goto done;
                 if (u < 0) break;
-                const Item it = load_unit(p, u);
-                if (it.skip || it.j1 <= it.j0) {
-                    // the first unit's Q has been loaded all the same
-                    for (int c = 0; k == 0 && c < chunks; c += kQPerStage, next()) {
-                        if (!wait_on(sy, smem_u32(&hd->full[st]), phase)) goto done;
-                        if (elect_one()) mbar_arrive(smem_u32(&hd->empty[st]));
-                        __syncwarp();
-                    }
-                    continue;
-                }
+                Item it;
+                auto open = [&] {
+                    it = load_unit(p, u);
+                    return !it.skip && it.j1 > it.j0;
+                };
+                if (k > 0 && !open()) continue;
                 // raw Q -> TMEM, once the previous unit's last product has read the old one
                 if (sc > 0 && !wait_on(sy, smem_u32(&hd->s_full[(sc - 1) & 1]), ((sc - 1) >> 1) & 1)) goto done;
                 for (int c = 0; c < chunks; c += kQPerStage, next()) {
@@ -612,12 +612,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                             for (int kq = 0; kq < 4; ++kq) tmem_cp_128x256b(tmem + ((c + e) * 4 + kq) * 8, d + 2 * kq);
                         }
                         tc_commit(smem_u32(&hd->empty[st]));
-                        if (c + kQPerStage >= chunks) tc_commit(smem_u32(&hd->q_raw));
+                        tc_commit(smem_u32(&hd->q_raw[c / kQPerStage]));
                     }
                     __syncwarp();
                 }
                 if (!wait_on(sy, smem_u32(&hd->q_full), qc & 1)) goto done;
                 ++qc;
+                if (k == 0) {
+                    wait_resolved();
+                    if (!open()) continue;
+                }
                 for (int j = it.j0; j < it.j1; ++j, ++sc, next()) {
                     const int sb = sc & 1;
                     const uint32_t d = tmem + kTmemS + sb * kBK;
@@ -667,15 +671,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 int u;
                 if (!tq_read(p, sy, rank, k, u)) goto done;
                 if (u < 0) break;
-                const Item it = load_unit(p, u);
-                if (it.skip) continue;
-                if (it.ntiles == 0) {
-                    if (p.lse && head && g == 0) p.lse[(int64_t)it.t * p.N1 + h] = it.rec[TR_VALID] ? sink : 0.f;
-                    continue;
-                }
-                const int nt = it.j1 - it.j0;
-                if (!wait_on(sy, smem_u32(&hd->q_raw), qc & 1)) goto done;
-                tc_fence_after();
+                Item it;
+                auto open = [&] {
+                    it = load_unit(p, u);
+                    if (!it.skip && it.ntiles == 0 && p.lse && head && g == 0)
+                        p.lse[(int64_t)it.t * p.N1 + h] = it.rec[TR_VALID] ? sink : 0.f;
+                    return !it.skip && it.ntiles > 0;
+                };
+                if (k > 0 && !open()) continue;
                 bool ok;
                 const float rq = p.scale_log2 / split_q(sy, hd, trow, p.Dq / 64, qc & 1, ok);
                 if (!ok) goto done;
@@ -683,6 +686,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&hd->q_full));
+                if (k == 0) {
+                    wait_resolved();
+                    if (!open()) continue;
+                }
+                const int nt = it.j1 - it.j0;
                 const uint64_t rq2 = pack2(rq, rq);
                 float m = -INFINITY, l = 0.f;  // of this thread's tiles, l in the frame of m
                 for (int e = (sc0 & 1) == (uint32_t)g ? 0 : 1; e < nt; e += 2, ++mine) {
