@@ -51,7 +51,8 @@
 // not help: 6 gather warps, or a warp of its own for the row lookups (they take the softmax's issue slots,
 // 3 and 4 % slower); a tile taken in the last tile's frame and redone where that does not hold (some of 128
 // heads mostly rises, 20 %); TMEM loads a step ahead or of 32 columns (0 to 5 %: longer loops; the roles of an
-// SM share its instruction caches); a staging of 8 boxes in the epilogue.
+// SM share its instruction caches); a
+// staging of 8 boxes, or rows of 128 bytes, in the epilogue.
 //
 // Keys of a token: first positions, then the window, then the compressed rows.  Slots without a key
 // carry weight 0 (log2 s = -inf); they and rows of unmapped blocks are filled with zeros.
@@ -101,8 +102,8 @@ constexpr int kMaxPieces = 64;
 constexpr int kMsgLo = 128 * 128, kMsgStats = kMsgLo + 128 * 64, kMsgBytes = kMsgStats + 1024;
 
 // Messages under way.  A slot is held from its copy's start over the split to the end of its product, about
-// 5000 cycles: with two slots that alone took 2500 a tile (64 tokens 67 us; 65 with four).
-constexpr int kSlots = 4;
+// 5000 cycles: with two slots that alone took 2500 a tile (64 tokens 67 us; 65 with three or four).
+constexpr int kSlots = 3;
 
 struct KeyConst {
     float s[kBK];   // scale; 0: a zero row
@@ -127,9 +128,9 @@ constexpr int kScoreRing = kScoreMsgs + 2 * kMsgBytes;
 constexpr int kScoreSmem = kScoreRing + kStages * kKStage;
 constexpr int kOutRing = kHdr;
 constexpr int kOutMsgs = kOutRing + kVStages * kVStage;
-constexpr int kOutStage = kOutMsgs + kSlots * kMsgBytes;  // epilogue staging: 64 bytes of 32 heads per warp
+constexpr int kOutStage = kOutMsgs + kSlots * kMsgBytes;  // epilogue staging: twice 64 bytes of 32 heads per warp
 constexpr int kWarpSlab = 32 * 64;
-constexpr int kOutSmem = kOutStage + kSoftWarps * kWarpSlab;
+constexpr int kOutSmem = kOutStage + 2 * kSoftWarps * kWarpSlab;
 constexpr int kSmemBytes = (kScoreSmem > kOutSmem ? kScoreSmem : kOutSmem) + 1024;  // + alignment slack
 static_assert(kScoreMsgs % 1024 == 0 && kScoreRing % 1024 == 0 && kKStage % 1024 == 0 && kOutRing % 1024 == 0 &&
               kOutMsgs % 1024 == 0 && kMsgBytes % 1024 == 0 && kOutStage % 1024 == 0, "swizzled tiles are 1 KiB aligned");
@@ -928,8 +929,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const bool any = __any_sync(0xffffffffu, a != 1.f);
 #pragma unroll 1
                     for (int c = 0; c < 2; ++c) {
-                        // the product of the tile before, of these columns (a barrier per slot: the products of the
-                        // three tiles before may be outstanding, which one barrier's two phases cannot tell apart)
+                        // the product of the tile before, of these columns (a barrier per slot: several products
+                        // may be outstanding, which one barrier's two phases cannot tell apart)
                         if (!wait_on(sy, smem_u32(&hd->pv_done[c][(pc - 1) % kSlots]), ((pc - 1) / kSlots) & 1)) goto done;
                         if (any) {
                             tc_fence_after();
@@ -962,17 +963,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // Each warp stages 64 bytes of its 32 head rows (64-byte swizzle) and writes them out: one TMA
                 // store, or 64-byte pieces of rows where a box would reach into the next token's heads.  Whole
                 // tokens in bf16, pieces in fp32, normalised within the piece.  (Direct stores, 16 bytes a lane
-                // to 32 rows, took 9.5 us for a piece.)
+                // to 32 rows, took 9.5 us for a piece; one buffer per warp 0.5 us more than two.)
                 if ((warp & 3) * 32 < p.N1) {
-                    const uint32_t buf = smem_u32(smem + kOutStage) + warp * kWarpSlab;
+                    uint8_t *const bufs = smem + kOutStage + warp * 2 * kWarpSlab;
                     const bool piece = it.np > 1;
                     const int row = piece ? ((it.t * p.P + it.piece) * p.NP + (warp & 3) * 32) : it.t * p.N1 + (warp & 3) * 32;
                     const int step = piece ? 16 : 32;
 #pragma unroll 1
                     for (int c = 0; c < kDv / 2; c += step) {
+                        uint8_t *const at = bufs + (c & step ? kWarpSlab : 0);
+                        const uint32_t buf = smem_u32(at);
                         uint32_t r[32], w[16];
                         tmem_ld32(tcol + (c & ~31), r);
-                        if (lane == 0) bulk_wait_read<0>();  // the last store has read buf
+                        if (lane == 0) bulk_wait_read<1>();  // the store before the last has read buf
                         __syncwarp();
                         tc_wait_ld();
                         if (piece) {
@@ -1000,8 +1003,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                             for (int i = 0; i < 32; i += 8) {
                                 const int e = i + (lane >> 2), q = lane & 3;
-                                const uint4 v = *reinterpret_cast<const uint4 *>(smem + kOutStage + warp * kWarpSlab + e * 64 +
-                                                                                 ((q ^ ((e >> 1) & 3)) << 4));
+                                const uint4 v = *reinterpret_cast<const uint4 *>(at + e * 64 + ((q ^ ((e >> 1) & 3)) << 4));
                                 if ((warp & 3) * 32 + e < p.N1)
                                     *reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(p.out) + (int64_t)(row + e) * kDv +
                                                                g * (kDv / 2) + c + q * 8) = v;
