@@ -15,13 +15,15 @@
 // taken for that reason: with scales A / 448 every growth would round every old row anew.
 //
 // Bound: bytes (each row read once and written once); a decode call is one launch latency, 6.4 us on the
-// device.  4 x 8192 rows of 576 to 8 bits take 16.7 us, 57 MB at 3.4 TB/s: the rows are read twice, the
+// device.  4 x 8192 rows of 576 to 8 bits take 16.5 us, 57 MB at 3.4 TB/s: the rows are read twice, the
 // second time from L1 or L2, and the two passes and the lookups before them follow one another in a CTA.
 // Clusters of 4 x 128 threads with 4 loads under way per thread take 16.7 us, 2 x 128 18.7, 2 x 256 18.3,
 // 8 x 256 43; one row per CTA (512 requests) takes 8.4 us with 128 threads and 12.4 with 256, which need
 // two waves.  The largest value of the copied dims is found on the bits, two at a time: unpacked to
 // floats, and with 64-bit positions, the kernel was bound by its instructions at 43 us.  Rows kept in
-// registers between the passes cost occupancy, 63 us; two kernels with a warp per two rows, 47 us.
+// registers between the passes cost occupancy, 63 us; two kernels with a warp per two rows, 47 us.  Calls one
+// after the other, with the last one's codes still to be written back, take 20.6 us each; turning the tail in
+// both passes, without the copy in shared memory, 22.5.
 
 #include <algorithm>
 
@@ -286,8 +288,10 @@ __device__ __forceinline__ int request_of_unit(const AppendArgs &p, int unit) { 
 // copied part or 8 of the turned part at a time.
 template <typename T> __global__ void __launch_bounds__(kThreads) append8_kernel(AppendArgs p) {
     constexpr int kAhead = 4;  // loads of 16 dims under way per thread
+    constexpr int kHeld = 2;   // turned pieces of 8 dims kept per thread: 32 rows of 64 dims in all
     __shared__ float warp_max[kWarps];
     __shared__ float block_max;
+    __shared__ float4 held[kHeld][2][kThreads];  // turned values, from the first pass to the second
     if ((int)blockIdx.x < p.nq) {
         rotate_q<T>(p, blockIdx.x);
         return;
@@ -321,6 +325,29 @@ template <typename T> __global__ void __launch_bounds__(kThreads) append8_kernel
     const int64_t src_bytes = p.kv_stride * 2;
 
     float amax = 0.f;
+    auto turn = [&](const Walk &w, float (&x)[8]) {
+        load_rotated<T>(p, reinterpret_cast<const uint4 *>(src + w.row * src_bytes), cs0 + (int64_t)w.row * p.step * p.R,
+                        2 * plain + w.at, x);
+    };
+    if (turned) {
+        Walk w(me, all, turned);
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k, w.next()) {
+            if (w.row >= rows) continue;
+            float x[8];
+            turn(w, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) note_finite(x[i], amax);
+            held[k][0][tid] = make_float4(x[0], x[1], x[2], x[3]);
+            held[k][1][tid] = make_float4(x[4], x[5], x[6], x[7]);
+        }
+        for (; w.row < rows; w.next()) {
+            float x[8];
+            turn(w, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) note_finite(x[i], amax);
+        }
+    }
     if (plain) {
         uint32_t m = 0;  // magnitudes order as their bits do, two at a time
         Walk w(me, all, plain);
@@ -344,7 +371,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads) append8_kernel
         }
         m = max(m >> 16, m & 0xffffu);
         if (m < infinity_bits<T>()) {
-            amax = sas::DT<T>::to_f2(m).x;
+            amax = fmaxf(amax, sas::DT<T>::to_f2(m).x);
         } else {  // an infinity or a NaN: look again, past those
             for (Walk r(me, all, plain); r.row < rows; r.next()) {
                 const uint4 *x = reinterpret_cast<const uint4 *>(src + r.row * src_bytes) + 2 * r.at;
@@ -354,15 +381,6 @@ template <typename T> __global__ void __launch_bounds__(kThreads) append8_kernel
                     for (int i = 0; i < 8; ++i) note_finite(y[i], amax);
                 }
             }
-        }
-    }
-    if (turned) {
-        for (Walk w(me, all, turned); w.row < rows; w.next()) {
-            float x[8];
-            load_rotated<T>(p, reinterpret_cast<const uint4 *>(src + w.row * src_bytes), cs0 + (int64_t)w.row * p.step * p.R,
-                            2 * plain + w.at, x);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) note_finite(x[i], amax);
         }
     }
 #pragma unroll
@@ -431,14 +449,19 @@ template <typename T> __global__ void __launch_bounds__(kThreads) append8_kernel
         }
     }
     if (turned) {
-        for (Walk w(me, all, turned); w.row < rows; w.next()) {
-            float x[8];
-            load_rotated<T>(p, reinterpret_cast<const uint4 *>(src + w.row * src_bytes), cs0 + (int64_t)w.row * p.step * p.R,
-                            2 * plain + w.at, x);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] *= inv;
+        auto put = [&](const Walk &w, const float4 &a, const float4 &b) {
             reinterpret_cast<uint2 *>(dst + (int64_t)w.row * p.D)[2 * plain + w.at] =
-                make_uint2(sas_fp8::to_e4m3x4(x[0], x[1], x[2], x[3]), sas_fp8::to_e4m3x4(x[4], x[5], x[6], x[7]));
+                make_uint2(sas_fp8::to_e4m3x4(a.x * inv, a.y * inv, a.z * inv, a.w * inv),
+                           sas_fp8::to_e4m3x4(b.x * inv, b.y * inv, b.z * inv, b.w * inv));
+        };
+        Walk w(me, all, turned);
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k, w.next())
+            if (w.row < rows) put(w, held[k][0][tid], held[k][1][tid]);
+        for (; w.row < rows; w.next()) {
+            float x[8];
+            turn(w, x);
+            put(w, make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]));
         }
     }
 }

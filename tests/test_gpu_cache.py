@@ -93,6 +93,7 @@ LENGTHS = [
     ([128, 256, 127], [128, 300, 255]),      # whole blocks
     ([2] * 70, [2 + 3 * i for i in range(70)]),
     ([2000], [2600]),
+    ([1] * 20 + [128], [5] * 20 + [256]),   # a whole block among single rows
 ]
 
 
