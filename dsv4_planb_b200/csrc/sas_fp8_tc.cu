@@ -82,6 +82,7 @@ constexpr int kDv = 512, kVSlabs = kDv / 128;
 constexpr int kVStage = kVSlabs * kSlab, kKStage = kVStage + kBK * 64;  // K: dims 512 .. 575 as 64-byte rows behind
 constexpr int kQChunk = 128 * 128, kQPerStage = 3;  // raw Q: 64 bf16 dims of 128 heads; chunks per stage of the K ring
 constexpr int kQStages = (576 / 64 + kQPerStage - 1) / kQPerStage;
+static_assert((512 / 64 + kQPerStage - 1) / kQPerStage == kQStages, "the last stage is the same one");
 constexpr int kSoftWarps = 8, kMmaWarp = 8, kProdWarp0 = 9, kProdWarps = 4;
 constexpr int kRows = kBK / kProdWarps;
 static_assert(kRows % 8 == 0 && kProdWarps == 4, "whole swizzle periods, 32 heads of Q a warp");
@@ -531,6 +532,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     Hdr *hd = reinterpret_cast<Hdr *>(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
+    const int quads = (p.N1 + 31) / 32;  // of 32 heads, a softmax warp's share
+    const uint32_t msg_bytes = quads * (kMsgBytes / 4);
 
     if (threadIdx.x == 0) {
         auto init = [](uint64_t *b, int n, uint32_t count) {
@@ -559,9 +562,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         hd->abort = 0;
         // the output CTA expects the first message of each P slot (bulk copies complete it)
         if (rank == 1)
-            for (int i = 0; i < kSlots; ++i) mbar_arrive_expect_tx(smem_u32(&hd->p_full[i]), kMsgBytes);
+            for (int i = 0; i < kSlots; ++i) mbar_arrive_expect_tx(smem_u32(&hd->p_full[i]), msg_bytes);
         mbar_fence_init();
     }
+    if (rank == 1)  // factors of heads that no message brings
+        for (int i = threadIdx.x; i < kSlots * 128; i += kThreads)
+            if ((i & 127) >= quads * 32)
+                reinterpret_cast<float2 *>(smem + kOutMsgs + (i >> 7) * kMsgBytes + kMsgStats)[i & 127] = make_float2(1.f, 0.f);
     if (warp == kMmaWarp) {
         tmem_alloc(smem_u32(&hd->tmem_base), kTmemCols);
         tmem_relinquish();
@@ -667,6 +674,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t sw1 = (h & 7) << 4, sw2 = ((h >> 1) & 3) << 4;
             const uint32_t peer_msgs = map_to_cta(smem_u32(smem + kOutMsgs), 1), peer_full0 = map_to_cta(smem_u32(hd->p_full), 1);
             const float sink = head && p.sinks ? p.sinks[h] : -INFINITY;
+            // a warp without heads: its rows of Q, S and P hold whatever lies there, and reach no other row (16 heads,
+            // 11 tiles: 33 us instead of 35 with all warps at work)
+            const bool idle = (warp & 3) >= quads;
             uint32_t sc0 = 0, qc = 0, lc = 0, mine = 0;  // the unit's first tile; units; units of two tiles or more; own tiles
             for (uint32_t k = 0;; ++k) {
                 int u;
@@ -681,7 +691,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 };
                 if (k > 0 && !open()) continue;
                 bool ok;
-                const float rq = p.scale_log2 / split_q(sy, hd, trow, p.Dq / 64, qc & 1, ok);
+                float rq = 0.f;
+                // (without the wait an idle warp could give the next unit's arrival in place of another warp's)
+                if (idle) ok = wait_on(sy, smem_u32(&hd->q_raw[kQStages - 1]), qc & 1);
+                else rq = p.scale_log2 / split_q(sy, hd, trow, p.Dq / 64, qc & 1, ok);
                 if (!ok) goto done;
                 ++qc;
                 tc_fence_before();
@@ -696,6 +709,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 float m = -INFINITY, l = 0.f;  // of this thread's tiles, l in the frame of m
                 for (int e = (sc0 & 1) == (uint32_t)g ? 0 : 1; e < nt; e += 2, ++mine) {
                     const uint32_t sc = sc0 + e;
+                    if (idle) {
+                        if (!wait_on(sy, smem_u32(&hd->s_full[g]), mine & 1)) goto done;
+                        if (lane == 0) mbar_arrive(smem_u32(&hd->s_free[g]));
+                        continue;
+                    }
                     if (!wait_on(sy, smem_u32(&hd->c_full[sc % kConsts]), (sc / kConsts) & 1)) goto done;
                     // the maximum so far comes from the other warp's tile and goes on to its next
                     if (sc > 0 && !wait_on(sy, smem_u32(&hd->m_bar[warp & 3][g ^ 1]), ((sc - 1) >> 1) & 1)) goto done;
@@ -899,27 +917,29 @@ __global__ void __launch_bounds__(kThreads, 1)
                     fin = stat.y;
                     if (g == (int)(pc & 1)) {  // this warp's tile: its 32 heads' weights into hi and lo codes, in place
                         if (threadIdx.x == g * 128) {
-                            mbar_arrive_expect_tx(smem_u32(&hd->p_full[ps]), kMsgBytes);  // the next message
+                            mbar_arrive_expect_tx(smem_u32(&hd->p_full[ps]), msg_bytes);  // the next message
                             mbar_arrive_remote(map_to_cta(smem_u32(&hd->p_sent[g]), 0));
                         }
-                        uint8_t *row1 = msg + h * 128, *row2 = msg + kMsgLo + h * 64;
-                        uint4 x[12], y[12];
+                        if ((warp & 3) < quads) {
+                            uint8_t *row1 = msg + h * 128, *row2 = msg + kMsgLo + h * 64;
+                            uint4 x[12], y[12];
 #pragma unroll
-                        for (int v = 0; v < 8; ++v) x[v] = *reinterpret_cast<const uint4 *>(row1 + ((v << 4) ^ sw1));
+                            for (int v = 0; v < 8; ++v) x[v] = *reinterpret_cast<const uint4 *>(row1 + ((v << 4) ^ sw1));
 #pragma unroll
-                        for (int v = 0; v < 4; ++v) x[8 + v] = *reinterpret_cast<const uint4 *>(row2 + ((v << 4) ^ sw2));
+                            for (int v = 0; v < 4; ++v) x[8 + v] = *reinterpret_cast<const uint4 *>(row2 + ((v << 4) ^ sw2));
 #pragma unroll
-                        for (int v = 0; v < 6; ++v) {
-                            split4h(x[2 * v].x, x[2 * v].y, y[v].x, y[6 + v].x);
-                            split4h(x[2 * v].z, x[2 * v].w, y[v].y, y[6 + v].y);
-                            split4h(x[2 * v + 1].x, x[2 * v + 1].y, y[v].z, y[6 + v].z);
-                            split4h(x[2 * v + 1].z, x[2 * v + 1].w, y[v].w, y[6 + v].w);
+                            for (int v = 0; v < 6; ++v) {
+                                split4h(x[2 * v].x, x[2 * v].y, y[v].x, y[6 + v].x);
+                                split4h(x[2 * v].z, x[2 * v].w, y[v].y, y[6 + v].y);
+                                split4h(x[2 * v + 1].x, x[2 * v + 1].y, y[v].z, y[6 + v].z);
+                                split4h(x[2 * v + 1].z, x[2 * v + 1].w, y[v].w, y[6 + v].w);
+                            }
+#pragma unroll
+                            for (int v = 0; v < 8; ++v) *reinterpret_cast<uint4 *>(row1 + ((v << 4) ^ sw1)) = y[v];
+#pragma unroll
+                            for (int v = 0; v < 4; ++v) *reinterpret_cast<uint4 *>(row2 + ((v << 4) ^ sw2)) = y[8 + v];
+                            fence_proxy_async_smem();
                         }
-#pragma unroll
-                        for (int v = 0; v < 8; ++v) *reinterpret_cast<uint4 *>(row1 + ((v << 4) ^ sw1)) = y[v];
-#pragma unroll
-                        for (int v = 0; v < 4; ++v) *reinterpret_cast<uint4 *>(row2 + ((v << 4) ^ sw2)) = y[8 + v];
-                        fence_proxy_async_smem();
                     }
                     // every warp, so that none reads the factors of a message that has been overwritten
                     __syncwarp();

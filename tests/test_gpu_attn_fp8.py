@@ -392,6 +392,19 @@ def test_drawn(cuda_device, seed):
     check(m, *run(m, check_status=True), tokens=range(min(len(m["where"]), 10)))
 
 
+@pytest.mark.parametrize("N1", [1, 31, 33, 64, 65, 96, 97])
+def test_short_units_of_few_heads(cuda_device, N1):
+    """Many tokens of one or two tiles each: warps without heads must keep the others' pace."""
+    m = make([1] * 400, [1 + 7 * (i % 23) for i in range(400)], N1=N1, scenario=1, win_left=150, seed=N1)
+    out, lse = run(m, kernel="tc", check_status=True)
+    check(m, out, lse, tokens=list(range(0, 400, 37)))
+    # every row against the other kernel: values below 4 are rounded twice (2^-6 each), and the weights differ
+    # by 2^-8 at most; a score of magnitudes up to 100 is off by 36 * 2^-22 of them on either side
+    simt = run(m, kernel="simt")
+    assert torch.isfinite(out).all() and (out.float() - simt[0].float()).abs().max() < 0.05
+    assert (lse - simt[1]).abs().max() < 1e-3
+
+
 @pytest.mark.parametrize("kernel", KERNELS)
 def test_rows_past_32_bits(cuda_device, kernel):
     """Blocks whose rows lie more than 2^32 bytes into the pool, written and read."""
