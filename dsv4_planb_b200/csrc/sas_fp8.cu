@@ -106,19 +106,21 @@ __global__ void __launch_bounds__(kThreads) resolve_rows_kernel(Args p) {
     };
     make_record(p, t, r, limit, look_up);
     if (tid == 0) {
-        stop_s = min(p.K, limit);
+        stop_s = 0x7fffffff;
         bits_s = 0;
     }
+    __syncthreads();
     int32_t *rows = p.rows + (int64_t)t * p.K;
     int kept = 0;
     uint32_t bits = 0;
-    for (int base = 0; base < p.K; base += kThreads * kPer) {
+    // Every thread leaves by its own copy of `end`, which is the same in all of them: stop_s changes only between
+    // a chunk's start and its first barrier, and is read only between the first and the second.
+    int end = min(p.K, limit);
+    for (int base = 0; base < end; base += kThreads * kPer) {
         if (base > 0) {
             load(base);
             look_up(r[TR_B]);
         }
-        __syncthreads();
-        if (base >= stop_s) break;
         const int i0 = base + tid * kPer;
         int stop = 0x7fffffff;
 #pragma unroll
@@ -126,13 +128,13 @@ __global__ void __launch_bounds__(kThreads) resolve_rows_kernel(Args p) {
             if (v[k] == -1) stop = i0 + k;
         if (stop != 0x7fffffff) atomicMin(&stop_s, stop);
         __syncthreads();
-        stop = stop_s;
+        end = min(end, stop_s);
         int32_t row[kPer];
         int cnt = 0;
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
             row[k] = -2;
-            if (i0 + k < stop) {
+            if (i0 + k < end) {
                 if (v[k] < -1) bits |= SAS_STATUS_BAD_INDEX;
                 if (v[k] >= 0 && v[k] < limit) {
                     const bool bad = phys[k] < -1 || phys[k] >= p.cmp_block_num;
