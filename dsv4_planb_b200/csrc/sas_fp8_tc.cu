@@ -207,9 +207,10 @@ __device__ __forceinline__ bool wait_on(const Sync &s, uint32_t bar, uint32_t pa
     return __all_sync(0xffffffffu, done) || wait_long(s, bar, parity, cluster_scope);
 }
 
-// Whether some row of O is to be rescaled before the message's product.
+// Whether some row of O is to be rescaled before the message's product: the sign bits of the four warps' first
+// factors (bits, because a factor may be -0: a maximum that rose by 2^150 leaves nothing of what came before).
 __device__ __forceinline__ bool some_alpha(const uint8_t *msg) {
-    return __any_sync(0xffffffffu, reinterpret_cast<const float2 *>(msg + kMsgStats)[(threadIdx.x & 3) * 32].x < 0.f);
+    return __any_sync(0xffffffffu, reinterpret_cast<const int2 *>(msg + kMsgStats)[(threadIdx.x & 3) * 32].x < 0);
 }
 
 // One lane of the warp, the same one each time.  The compiler takes what it runs as warp-uniform: with
@@ -812,10 +813,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                             p.part_s[((int64_t)it.t * p.P + it.piece) * p.N1 + h] = own;
                         }
                     }
-                    // the sign of the warp's first alpha: some row of the warp has one
+                    // the sign bit of the warp's first alpha: some row of the warp has one
                     if (!head) alpha = 1.f;
                     const bool some = __any_sync(0xffffffffu, alpha != 1.f);
-                    *reinterpret_cast<float2 *>(stage + kMsgStats + h * 8) = make_float2(lane == 0 && some ? -alpha : alpha, fin);
+                    *reinterpret_cast<float2 *>(stage + kMsgStats + h * 8) =
+                        make_float2(__uint_as_float(__float_as_uint(alpha) | (lane == 0 && some ? 0x80000000u : 0u)), fin);
                     fence_proxy_async_smem();
                     // only now must the peer be done with the slot: S has been free since the second pass
                     const uint32_t ps = sc % kSlots;

@@ -38,3 +38,27 @@ def test_long_index_rows(cuda_device, K, kernel):
     for _ in range(5):
         again = run(m, kernel=kernel)
         assert torch.equal(again[0], out) and torch.equal(again[1], lse)
+
+
+def far_rise(tokens, N1, rise, seed):
+    """Every head's scores lie near 0 except for one late key, which all heads meet at about ``rise`` nats."""
+    m = make([1] * tokens, [900] * tokens, N1=N1, scenario=1, win_left=799, seed=seed)
+    g = torch.Generator().manual_seed(seed)
+    pattern = torch.randint(0, 2, (576,), generator=g).float() * 2 - 1
+    m["q"] = (pattern + 0.05 * torch.randn((tokens, N1, 576), generator=g)).to(torch.bfloat16).cuda()
+    codes, scale, table = m["ori"]
+    scale.fill_(2.0 ** -4)
+    codes.copy_((torch.randn(codes.shape, generator=g) * 8).to(codes.dtype).cuda())  # values of size 0.5
+    for b in range(tokens):  # position 700: several tiles behind the window's start at 100, not in its last one
+        row = pattern * (rise / 24 / 2.0 ** -4)  # q . k / sqrt(576) = rise
+        codes[int(table[b, 700 // 128]), 700 % 128, 0] = row.to(codes.dtype).cuda()
+    return m
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("N1", [1, 16, 32, 33, 128])
+@pytest.mark.parametrize("rise", [60, 110, 250, 600])
+def test_one_late_key_far_above(cuda_device, rise, N1, kernel):
+    """A maximum that rises by more than 104 nats: the factor of what came before it is 0 in 32 bits."""
+    m = far_rise(40, N1, rise, seed=41)
+    check(m, *run(m, kernel=kernel, check_status=True), tokens=[0, 7, 39])
