@@ -1,17 +1,23 @@
 // sm_100a tensor-core attention over the 8-bit cache: bf16 queries, D_qk 512 or 576, D_v 512, up to
 // 128 heads.
 //
-// The keys stay e4m3 from HBM to the MMA (kind::f8f6f4).  What multiplies them is split exactly into
-// two e4m3 terms: a bf16 value has 8 significant bits, and x = hi + lo with hi = e4m3(x) leaves a lo
-// of 4 bits.  Queries are scaled per row by a power of two that brings the largest element to
-// [128, 256): elements down to 2^-10 of it split without error, smaller ones are off by at most 2^-10
-// (2^-17 of the largest).  Softmax weights, at most 431 by their scale, lose 2^-9 relative (bf16 would
-// lose 2^-8) and 2^-10 where lo is subnormal.  So one product costs two e4m3 MMAs, which is the time
-// of one bf16 MMA, at half the bytes gathered.
+// The keys stay e4m3 from HBM to the MMA (kind::f8f6f4).  What multiplies them is split into 8-bit
+// terms.  Queries: two e4m3 terms, since a bf16 value has 8 significant bits and x = hi + lo with
+// hi = e4m3(x) leaves a lo of 4 bits.  They are scaled per row by a power of two that brings the largest
+// element to [128, 256): elements down to 2^-10 of it split without error, smaller ones are off by at most
+// 2^-10 (2^-17 of the largest).  Softmax weights, at most 431 by their scale and rounded to fp16 (2^-11):
+// hi in e4m3, then two e5m2 terms, which reach 2^-16 where hi has no bits left.  hi leaves at most 2^-4 of
+// a weight's power of two (2^-10 where it is subnormal), and each e5m2 term cuts three bits off what is left:
+// 2^-10 of a weight, or 2^-16 of a scale in which the row's largest weight is 2^6 or more.  Two e4m3 terms, whose
+// smallest step is 2^-9, took 10 % less time (1.06 ms instead of 1.19 for 2048 tokens, 69.5 us instead of 76
+// for 64; the products of V in the output CTA are 18 MMAs a tile instead of 12), but lost every weight below
+// 2^-16 of the largest: 3 to 50 % of the output where one key with a small value holds 80 to 99 % of a row.
+// One e5m2 term behind hi takes no more time than that, but loses 2^-8 of a weight where two e4m3 terms lose 2^-9.
+// A QK product costs two 8-bit MMAs, the time of one bf16 MMA, at half the bytes gathered.
 //
 // A key's scale s_j multiplies its score and its value.  With t_ij = scale q_i k_j in log2 units, the
 // weight of value row j (its codes) is 2^(t_ij) s_j, so the running maximum m_i is taken over
-// t_ij + log2 s_j.  e_ij = 2^(t_ij - m_i + 5.75) adds to the softmax's denominator and
+// t_ij + log2 s_j.  e_ij = 2^(t_ij - m_i + 6) adds to the softmax's denominator and
 // P_ij = e_ij s_j goes to the MMA.  The sink joins at the end.
 //
 // A unit of work (a token, or a piece of one) goes to a cluster of two CTAs on two SMs that split it
@@ -22,9 +28,9 @@
 //         S (2 x 96 columns)
 //   4 warps gather 96 key rows per tile          4 warps gather the first 512 bytes of the rows
 //           (cp.async into the MMA's swizzle)
-//   1 warp  S = Q K^T: 2 MMAs (hi, lo) of M 128, 1 warp  O += P V: 2 (hi, lo) per 32 keys and 256
-//           N 96, K 32 per 32 dims                       value dims; V is the N-major B operand, the
-//                                                        same bytes in the same swizzle as K
+//   1 warp  S = Q K^T: 2 MMAs (hi, lo) of M 128, 1 warp  O += P V: 3 per 32 keys and 256 value dims; V is the
+//           N 96, K 32 per 32 dims                       N-major B operand, the same bytes in the same
+//                                                        swizzle as K
 //   8 warps split Q; softmax (thread = head;     8 warps split P (thread = head; warps 0-3 the even
 //           warps 0-3 take the even tiles,               tiles, 4-7 the odd ones); rescale O where a
 //           4-7 the odd ones); P in fp16 and             maximum rose; epilogue
@@ -37,10 +43,10 @@
 //     16-byte cp.async reaches 56 bytes per cycle from L2 (110 GB/s), and the HBM's rate over all SMs.
 //   - st.async to the other SM moves 12 bytes per cycle and holds the issuing warps meanwhile; a tile's
 //     P is 24 KiB.  Bulk copies from a staging buffer run beside the next tile's softmax.
-//   - With 128 heads some maximum rises in most tiles.  It is followed only past 2^3 (P <= 2^8.75, the
-//     e4m3 range; the largest weight is then at least 2^5.75, and the 2^-10 that a weight can be off by
-//     where its lo is subnormal are 2^-15.75 of it), and O is rescaled 256 columns at a time, each as
-//     soon as the last tile's product of these columns is complete.
+//   - With 128 heads some maximum rises in most tiles.  It is followed only past 2^2.75 (P <= 2^8.75, the
+//     e4m3 range; the largest weight is then at least 2^6, and what a small weight is off by 2^-22 of it; 2^0.75
+//     would take 2 % more time), and O is rescaled 256 columns at a time, each as soon as the last tile's
+//     product of these columns is complete.
 //
 // Whole calls: 64 tokens of 2176 keys, 128 heads of 576 dims: 65 us (38.8 GFLOP, 98.6 MB); 2048 such
 // tokens: 1.07 ms, 930 TFLOP/s, and 1.21 ms once the card is at its power limit (1.7 GHz).  A tile takes
@@ -94,16 +100,17 @@ constexpr int kTmemCols = 512, kTmemS = 320;
 // done with tile n - 8.
 constexpr int kConsts = 8;
 constexpr float kTop = 8.75f;        // log2 of the largest P: 431, within e4m3's 448
-constexpr float kRise = 3.f;         // log2 of the rise of a maximum that is left to P
+constexpr float kRise = 2.75f;       // log2 of the rise of a maximum that is left to P
 constexpr int kMaxPieces = 64;
 
 // P message: per head 96 weights in fp16, 64 in a 128-byte row (SW128) and 32 in a 64-byte row (SW64), then
 // {alpha, the unit's final factor}.  The 32 heads of a warp are contiguous in each part.  The output CTA
-// puts the codes in the weights' place: 96 hi and 32 lo in the first row, the other 64 lo in the second.
+// puts codes in the weights' place: 96 hi and 32 mid in the first row, the other 64 mid in the second; lo goes
+// to a buffer of its own.
 constexpr int kMsgLo = 128 * 128, kMsgStats = kMsgLo + 128 * 64, kMsgBytes = kMsgStats + 1024;
 
-// Messages under way.  A slot is held from its copy's start over the split to the end of its product, about
-// 5000 cycles: with two slots that alone took 2500 a tile (64 tokens 67 us; 65 with three or four).
+// Messages under way.  A slot is held from its copy's start over the split to the end of its product: 64 tokens take
+// 79 us with two slots, 76 with three or four.
 constexpr int kSlots = 3;
 
 struct KeyConst {
@@ -129,12 +136,16 @@ constexpr int kScoreRing = kScoreMsgs + 2 * kMsgBytes;
 constexpr int kScoreSmem = kScoreRing + kStages * kKStage;
 constexpr int kOutRing = kHdr;
 constexpr int kOutMsgs = kOutRing + kVStages * kVStage;
-constexpr int kOutStage = kOutMsgs + kSlots * kMsgBytes;  // epilogue staging: twice 64 bytes of 32 heads per warp
+// Third terms of the weights, for even and for odd tiles: per 8 heads three blocks of 32 keys, each 8 rows of 32 bytes
+// (SW32), so that a warp's 32 heads are contiguous.
+constexpr int kThirdBytes = 128 / 8 * 3 * 256;
+constexpr int kOutThirds = kOutMsgs + kSlots * kMsgBytes;
+constexpr int kOutStage = kOutThirds + 2 * kThirdBytes;  // epilogue staging: 64 bytes of 32 heads per warp
 constexpr int kWarpSlab = 32 * 64;
-constexpr int kOutSmem = kOutStage + 2 * kSoftWarps * kWarpSlab;
+constexpr int kOutSmem = kOutStage + kSoftWarps * kWarpSlab;
 constexpr int kSmemBytes = (kScoreSmem > kOutSmem ? kScoreSmem : kOutSmem) + 1024;  // + alignment slack
 static_assert(kScoreMsgs % 1024 == 0 && kScoreRing % 1024 == 0 && kKStage % 1024 == 0 && kOutRing % 1024 == 0 &&
-              kOutMsgs % 1024 == 0 && kMsgBytes % 1024 == 0 && kOutStage % 1024 == 0, "swizzled tiles are 1 KiB aligned");
+              kOutMsgs % 1024 == 0 && kMsgBytes % 1024 == 0 && kOutStage % 1024 == 0 && kThirdBytes / 4 % 512 == 0 && kThirdBytes / 4 >= kWarpSlab, "swizzled tiles are 1 KiB aligned");
 static_assert(kQPerStage * kQChunk <= kKStage && kSmemBytes <= 232448, "shared memory");
 
 // n / d for 0 <= n < 2^31 as a multiplication: 2^(32 + s) <= m d < 2^(32 + s) + 2^(s + 1) with 2^s < d <= 2^(s + 1)
@@ -175,10 +186,10 @@ __device__ __forceinline__ void mma8_ss(uint32_t d, uint64_t a, uint64_t b, uint
         "l"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
-// Instruction descriptor of kind::f8f6f4, both operands e4m3 (format 0), fp32 accumulation; b_mn: B is
+// Instruction descriptor of kind::f8f6f4, A e4m3 (format 0) or e5m2 (1), B e4m3, fp32 accumulation; b_mn: B is
 // N-major.
-__host__ __device__ constexpr uint32_t idesc_e4m3(uint32_t m, uint32_t n, uint32_t b_mn) {
-    return (1u << 4) | (b_mn << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
+__host__ __device__ constexpr uint32_t idesc_f8(uint32_t m, uint32_t n, uint32_t b_mn, uint32_t a_e5m2) {
+    return (1u << 4) | (a_e5m2 << 7) | (b_mn << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
@@ -418,23 +429,31 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     return *reinterpret_cast<const uint32_t *>(&v);
 }
 
-// Two fp16 values (at most 448) as two pairs of e4m3 codes, hi + lo.  The difference is exact in fp16.
-__device__ __forceinline__ void split2(uint32_t x, uint32_t &hi, uint32_t &lo) {
-    uint16_t h, l;
-    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(h) : "r"(x));
-    const uint32_t back = e4m3x2_to_half2(h);
-    const __half2 d = __hsub2(*reinterpret_cast<const __half2 *>(&x), *reinterpret_cast<const __half2 *>(&back));
-    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(l) : "r"(*reinterpret_cast<const uint32_t *>(&d)));
-    hi = h;
-    lo = l;
+// Two fp16 values (at most 448) as pairs of e4m3 codes, hi + lo, in 16 bits each.  Differences of a value and its
+// code are exact in fp16.
+__device__ __forceinline__ uint32_t to_e4m3(uint32_t x) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(x));
+    return r;
 }
-// Four fp16 values into four hi and four lo codes.
+__device__ __forceinline__ uint32_t less(uint32_t x, uint32_t y) {  // halves of x minus halves of y
+    const __half2 d = __hsub2(*reinterpret_cast<const __half2 *>(&x), *reinterpret_cast<const __half2 *>(&y));
+    return *reinterpret_cast<const uint32_t *>(&d);
+}
+// Four fp16 values into four hi and four lo codes, both e4m3.
 __device__ __forceinline__ void split4h(uint32_t a, uint32_t b, uint32_t &hi, uint32_t &lo) {
-    uint32_t h0, l0, h1, l1;
-    split2(a, h0, l0);
-    split2(b, h1, l1);
+    const uint32_t h0 = to_e4m3(a), h1 = to_e4m3(b);
+    lo = to_e4m3(less(a, e4m3x2_to_half2(h0))) | (to_e4m3(less(b, e4m3x2_to_half2(h1))) << 16);
     hi = h0 | (h1 << 16);
-    lo = l0 | (l1 << 16);
+}
+// Four fp16 values as hi (e4m3) + mid + lo (e5m2).  An fp16 value's upper byte is its e5m2 code, cut towards zero, so
+// that mid and lo take no conversions.
+__device__ __forceinline__ void split4w(uint32_t a, uint32_t b, uint32_t &hi, uint32_t &mid, uint32_t &lo) {
+    const uint32_t h0 = to_e4m3(a), h1 = to_e4m3(b);
+    const uint32_t r0 = less(a, e4m3x2_to_half2(h0)), r1 = less(b, e4m3x2_to_half2(h1));
+    hi = __byte_perm(h0, h1, 0x5410);
+    mid = __byte_perm(r0, r1, 0x7531);
+    lo = __byte_perm(less(r0, r0 & 0xff00ff00u), less(r1, r1 & 0xff00ff00u), 0x7531);
 }
 
 // Four bf16 values times f into four hi and four lo codes.
@@ -520,9 +539,13 @@ __device__ __forceinline__ void bulk_to_peer(uint32_t dst, uint32_t src, uint32_
                  : "memory");
 }
 
-// Shared-memory matrix descriptor, K-major rows of 64 bytes, 64-byte swizzle.
-__device__ __forceinline__ uint64_t sdesc_sw64(uint32_t saddr) {
-    return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)1 << 16 | (uint64_t)(512 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)4 << 61;
+// Shared-memory matrix descriptors, K-major rows of 64 or 32 bytes, 64- or 32-byte swizzle; sbo: bytes between groups
+// of 8 rows.
+__device__ __forceinline__ uint64_t sdesc_sw64(uint32_t saddr, uint32_t sbo) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)1 << 16 | (uint64_t)(sbo >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)4 << 61;
+}
+__device__ __forceinline__ uint64_t sdesc_sw32(uint32_t saddr, uint32_t sbo) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)1 << 16 | (uint64_t)(sbo >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)6 << 61;
 }
 
 __global__ void __launch_bounds__(kThreads, 1)
@@ -591,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (warp >= kProdWarp0) {
             producer<true>(p, sy, &q_map, ring, hd, consts);
         } else if (warp == kMmaWarp) {
-            constexpr uint32_t idesc = idesc_e4m3(128, kBK, 0);
+            constexpr uint32_t idesc = idesc_f8(128, kBK, 0, 0);
             const int chunks = p.Dq / 64;
             uint32_t st = 0, phase = 0, sc = 0, qc = 0;
             auto next = [&] {
@@ -652,7 +675,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             }
                         }
                         if (chunks > 8) {
-                            const uint64_t b = sdesc_sw64(base + kVStage);
+                            const uint64_t b = sdesc_sw64(base + kVStage, 512);
 #pragma unroll
                             for (int i = 0; i < 2; ++i) {
                                 mma8_ts(d, tmem + 256 + i * 8, b + 2 * i, idesc, 1u);
@@ -842,7 +865,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (warp >= kProdWarp0) {
             producer<false>(p, sy, nullptr, ring, hd, nullptr);
         } else if (warp == kMmaWarp) {
-            constexpr uint32_t idesc = idesc_e4m3(128, 256, 1);
+            constexpr uint32_t idesc = idesc_f8(128, 256, 1, 0), idesc5 = idesc_f8(128, 256, 1, 1);
             uint32_t st = 0, phase = 0, pc = 0, oc = 0, rsc = 0;
             for (uint32_t k = 0;; ++k) {
                 int u;
@@ -859,7 +882,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const bool last = j == it.j1 - 1, rescale = j > it.j0 && some_alpha(msg);
                     if (!wait_on(sy, smem_u32(&hd->full[st]), phase)) goto done;
                     fence_proxy_async_smem();  // the rows were written by cp.async
-                    const uint64_t a1 = sdesc_sw128(smem_u32(msg), 16, 1024), a2 = sdesc_sw64(smem_u32(msg) + kMsgLo);
+                    const uint64_t a1 = sdesc_sw128(smem_u32(msg), 16, 1024), a2 = sdesc_sw64(smem_u32(msg) + kMsgLo, 512);
+                    const uint64_t a3 = sdesc_sw32(smem_u32(smem + kOutThirds) + (pc & 1) * kThirdBytes, 768);
                     const uint32_t base = smem_u32(ring) + st * kVStage;
 #pragma unroll 1
                     for (int c = 0; c < 2; ++c) {  // 256 value dims each
@@ -871,7 +895,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                             for (int i = 0; i < kBK / 32; ++i) {
                                 mma8_ss(d, a1 + 2 * i, b + 256 * i, idesc, (j > it.j0 || i > 0) ? 1u : 0u);
-                                mma8_ss(d, i == 0 ? a1 + 6 : a2 + 2 * (i - 1), b + 256 * i, idesc, 1u);
+                                mma8_ss(d, i == 0 ? a1 + 6 : a2 + 2 * (i - 1), b + 256 * i, idesc5, 1u);
+                                mma8_ss(d, a3 + 16 * i, b + 256 * i, idesc5, 1u);
                             }
                             tc_commit(smem_u32(&hd->pv_done[c][ps]));
                         }
@@ -894,7 +919,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int g = warp >> 2, h = threadIdx.x & 127;  // which half of the columns, head row
             const bool head = h < p.N1;
             const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-            const uint32_t sw1 = (h & 7) << 4, sw2 = ((h >> 1) & 3) << 4;
+            const uint32_t sw1 = (h & 7) << 4, sw2 = ((h >> 1) & 3) << 4, sw3 = ((h >> 2) & 1) << 4;
+            uint8_t *const thirds = smem + kOutThirds + g * kThirdBytes + (h >> 3) * 768 + (h & 7) * 32;
             uint32_t ofc = 0, pc = 0;
             for (uint32_t k = 0;; ++k) {
                 int u;
@@ -917,12 +943,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const float2 stat = reinterpret_cast<const float2 *>(msg + kMsgStats)[h];
                     const bool rescale = j > it.j0 && some_alpha(msg);
                     fin = stat.y;
-                    if (g == (int)(pc & 1)) {  // this warp's tile: its 32 heads' weights into hi and lo codes, in place
+                    if (g == (int)(pc & 1)) {  // this warp's tile: its 32 heads' weights into codes
                         if (threadIdx.x == g * 128) {
                             mbar_arrive_expect_tx(smem_u32(&hd->p_full[ps]), msg_bytes);  // the next message
                             mbar_arrive_remote(map_to_cta(smem_u32(&hd->p_sent[g]), 0));
                         }
                         if ((warp & 3) < quads) {
+                            // the thirds' buffer is free: the product of two tiles before, and the last unit's stores
+                            if (pc >= 2 && !wait_on(sy, smem_u32(&hd->pv_done[1][(pc - 2) % kSlots]), ((pc - 2) / kSlots) & 1)) goto done;
+                            if (lane == 0) bulk_wait_read<0>();
+                            __syncwarp();
                             uint8_t *row1 = msg + h * 128, *row2 = msg + kMsgLo + h * 64;
                             uint4 x[12], y[12];
 #pragma unroll
@@ -931,10 +961,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                             for (int v = 0; v < 4; ++v) x[8 + v] = *reinterpret_cast<const uint4 *>(row2 + ((v << 4) ^ sw2));
 #pragma unroll
                             for (int v = 0; v < 6; ++v) {
-                                split4h(x[2 * v].x, x[2 * v].y, y[v].x, y[6 + v].x);
-                                split4h(x[2 * v].z, x[2 * v].w, y[v].y, y[6 + v].y);
-                                split4h(x[2 * v + 1].x, x[2 * v + 1].y, y[v].z, y[6 + v].z);
-                                split4h(x[2 * v + 1].z, x[2 * v + 1].w, y[v].w, y[6 + v].w);
+                                uint4 z;
+                                split4w(x[2 * v].x, x[2 * v].y, y[v].x, y[6 + v].x, z.x);
+                                split4w(x[2 * v].z, x[2 * v].w, y[v].y, y[6 + v].y, z.y);
+                                split4w(x[2 * v + 1].x, x[2 * v + 1].y, y[v].z, y[6 + v].z, z.z);
+                                split4w(x[2 * v + 1].z, x[2 * v + 1].w, y[v].w, y[6 + v].w, z.w);
+                                *reinterpret_cast<uint4 *>(thirds + (v >> 1) * 256 + ((v & 1) ? 16 ^ sw3 : sw3)) = z;
                             }
 #pragma unroll
                             for (int v = 0; v < 8; ++v) *reinterpret_cast<uint4 *>(row1 + ((v << 4) ^ sw1)) = y[v];
@@ -987,13 +1019,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // tokens in bf16, pieces in fp32, normalised within the piece.  (Direct stores, 16 bytes a lane
                 // to 32 rows, took 9.5 us for a piece; one buffer per warp 0.5 us more than two.)
                 if ((warp & 3) * 32 < p.N1) {
-                    uint8_t *const bufs = smem + kOutStage + warp * 2 * kWarpSlab;
+                    // two buffers: one of its own, and this warp's part of the thirds, which no product reads any more
+                    uint8_t *const buf0 = smem + kOutStage + warp * kWarpSlab;
+                    uint8_t *const buf1 = smem + kOutThirds + g * kThirdBytes + (warp & 3) * (kThirdBytes / 4);
                     const bool piece = it.np > 1;
                     const int row = piece ? ((it.t * p.P + it.piece) * p.NP + (warp & 3) * 32) : it.t * p.N1 + (warp & 3) * 32;
                     const int step = piece ? 16 : 32;
 #pragma unroll 1
                     for (int c = 0; c < kDv / 2; c += step) {
-                        uint8_t *const at = bufs + (c & step ? kWarpSlab : 0);
+                        uint8_t *const at = c & step ? buf1 : buf0;
                         const uint32_t buf = smem_u32(at);
                         uint32_t r[32], w[16];
                         tmem_ld32(tcol + (c & ~31), r);

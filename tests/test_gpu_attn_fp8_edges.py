@@ -1,9 +1,12 @@
 """sparse_attn_sharedkv_fp8 where index rows end at a chunk's border, maxima rise far, and one key dominates."""
 
+import math
+
 import pytest
 import torch
 
-from tests.test_gpu_attn_fp8 import KERNELS, check, make, run
+from tests import _cache_ref as ref
+from tests.test_gpu_attn_fp8 import HALF_STEP, KERNELS, SHAPES, check, ident, make, run
 
 pytestmark = pytest.mark.gpu
 
@@ -62,3 +65,75 @@ def test_one_late_key_far_above(cuda_device, rise, N1, kernel):
     """A maximum that rises by more than 104 nats: the factor of what came before it is 0 in 32 bits."""
     m = far_rise(40, N1, rise, seed=41)
     check(m, *run(m, kernel=kernel, check_status=True), tokens=[0, 7, 39])
+
+
+# Error of a tensor-core weight: rounded to fp16 (2^-11 of it), then split into an e4m3 term (nearest) and two e5m2
+# terms (cut). Where the first is normal it leaves at most 2^-4 of the weight's power of two, the second less than
+# 2^-7, the third less than 2^-10. Where the first is subnormal (weights below 2^-6) they leave 2^-10, 2^-13 and 2^-16,
+# the smallest step of e5m2. A row's largest weight ends at 2^6 or more (the frame follows rises above 2^2.75, the top
+# is 2^8.75), so 2^-16 is 2^-22 of it.
+WEIGHT, WEIGHT_OF_TOP = 2.0 ** -10 + 2.0 ** -11 + 2.0 ** -20, 2.0 ** -22
+
+
+def check_weights(m, out, lse, tokens=None):
+    """As ``check``, with the bounds above for the weights."""
+    for t in range(len(m["where"])) if tokens is None else tokens:
+        b, p = m["where"][t]
+        o, l, spread, top, reach = ref.attend(
+            m["case"], m["q"][t], p, b, (m["ori"][0][:, :, 0], m["ori"][1], m["ori"][2][b]),
+            None if m["cmp"] is None else (m["cmp"][0][:, :, 0], m["cmp"][1], m["cmp"][2][b]),
+            None if m["idx"] is None else m["idx"][t, 0].numpy(), m["sinks"], m["scale"], m["Dv"])
+        d = (36 * 2.0 ** -22 + 3 * 2.0 ** -24) * reach
+        assert ((lse[t].double() - l).abs() <= d + 2.0 ** -20 + 2.0 ** -22 * l.abs()).all()
+        tol = (HALF_STEP[m["src"]] * o.abs() + 2.0 ** -24 + spread * (2 * d + 2.0 ** -20 + WEIGHT + 70 * 2.0 ** -22)[:, None]
+               + WEIGHT_OF_TOP * top)
+        err = (out[t].double() - o).abs()
+        assert (err <= tol).all(), (t, float((err - tol).max()), float((err.norm(dim=1) / o.norm(dim=1)).max()))
+
+
+def one_key_dominates(tokens, N1, mass, spread, mean, seed):
+    """The first position, which stays visible, takes ``mass`` of the softmax and has a small value; 2176 other keys
+    share the rest, with scores that differ by about ``spread`` nats and values with a common mean."""
+    K = 2048
+    m = make([1] * tokens, [9000] * tokens, N1=N1, K=K, first=1, seed=seed)
+    m["sinks"] = None
+    g = torch.Generator().manual_seed(seed)
+    pattern = torch.randint(0, 2, (64,), generator=g).float() * 2 - 1
+    q = torch.randn((tokens, N1, 576), generator=g) * spread
+    q[:, :, 512:] = pattern
+    m["q"] = q.to(torch.bfloat16).cuda()
+    base = torch.randn(512, generator=g) * mean
+    for codes, scale, _ in (m["ori"], m["cmp"]):
+        scale.fill_(2.0 ** -5)
+        x = base + torch.randn(codes.shape[:-1] + (512,), generator=g)
+        codes.copy_(torch.cat([x, torch.zeros(codes.shape[:-1] + (64,))], dim=-1).mul_(32).clamp_(-448, 448).to(codes.dtype).cuda())
+    codes, _, table = m["ori"]
+    top = math.log(mass / (1 - mass) * 2176) * 24 / 64
+    for b in range(tokens):
+        row = torch.cat([torch.randn(512, generator=g) * 0.02, pattern * top]) * 32
+        codes[int(table[b, 0]), 0, 0] = row.to(codes.dtype).cuda()
+    return m
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("tokens", [2, 40])  # in pieces, and whole
+@pytest.mark.parametrize("mass,spread,mean", [(0.8, 1.0, 1.0), (0.9, 0.02, 1.0), (0.95, 1.0, 1.0), (0.95, 0.02, 0.0), (0.99, 0.5, 1.0)])
+def test_tail_behind_one_key(cuda_device, mass, spread, mean, tokens, kernel):
+    """What many small weights add up to is not lost beside one large weight."""
+    m = one_key_dominates(tokens, 32, mass, spread, mean, seed=42)
+    check_weights(m, *run(m, kernel=kernel, check_status=True), tokens=[0, tokens - 1])
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=ident)
+def test_weights_of_16_bits(cuda_device, shape):
+    m = make(**shape, seed=len(shape["q_lens"]))
+    if all(n <= k for n, k in zip(m["q_lens"], m["kv_lens"])):
+        check_weights(m, *run(m, kernel="tc", check_status=True))
+
+
+def test_sharp_scores_and_their_tails(cuda_device):
+    """Queries of very different sizes: flat softmaxes, sharp ones and all between."""
+    m = make([1] * 40, [3000] * 40, N1=128, seed=43)
+    size = torch.exp2(torch.arange(128, device="cuda").float() / 8 - 6)
+    m["q"] = (m["q"].float() * size[None, :, None]).to(torch.bfloat16)
+    check_weights(m, *run(m, kernel="tc", check_status=True), tokens=[0, 13, 39])
