@@ -15,7 +15,7 @@ import torch
 
 from . import _lib
 from .api import _dense16, _dtype_code, _pool16, _ptr, _scenario, _workspace
-from .cache import _eager, _int32, _ops, _raw_stream, _refuse_grad
+from .cache import _eager, _int32, _ops, _raw_stream, _refuse_derivatives, _written
 
 KERNELS = {"auto": 0, "simt": 1, "tc": 2}
 _INT32 = 2**31 - 1  # no position lies beyond it
@@ -81,6 +81,7 @@ def _launch(q, ori_kv, ori_kv_scale, cmp_kv, cmp_kv_scale, cmp_sparse_indices, o
         _lib.check(rc, "sas_kvq_forward")
     if out_user is not None:
         out_user.copy_(out)
+    _written(out, lse)
     if check_status:
         st = _lib.ctypes.c_uint32(0)
         _lib.check(lib.sas_kvq_read_status(args, ws.data_ptr(), st, stream), "sas_kvq_read_status")
@@ -157,8 +158,7 @@ def sparse_attn_sharedkv_fp8(
         raise ValueError(f"kernel must be one of {sorted(KERNELS)}")
     if not q.is_cuda:
         raise ValueError("q must be a CUDA tensor (sas_b200 has no CPU path)")
-    if torch.is_grad_enabled() and (q.requires_grad or (sinks is not None and sinks.requires_grad)):
-        _refuse_grad("sparse_attn_sharedkv_fp8")
+    _refuse_derivatives("sparse_attn_sharedkv_fp8", q, ori_kv, ori_kv_scale, cmp_kv, cmp_kv_scale, sinks, out, lse_out)
     shape, device, kind = q.shape, q.device, q.dtype
     if layout_q == "TND":
         lead = 1
@@ -209,7 +209,8 @@ def sparse_attn_sharedkv_fp8(
     call = (q, ori_kv, ori_kv_scale, cmp_kv, cmp_kv_scale, cmp_sparse_indices, ori_block_table, cmp_block_table,
             cu_seqlens_q, seqused_kv, sinks, float(softmax_scale), 4 if cmp_ratio is None else min(int(cmp_ratio), _INT32),
             min(int(ori_win_left), _INT32), min(int(ori_first), _INT32), layout_q, Dv, kernel, bool(check_status), out, lse)
-    if _eager(q):
+    if _eager(q, ori_kv, ori_kv_scale, cmp_kv, cmp_kv_scale, cmp_sparse_indices, ori_block_table, cmp_block_table, cu_seqlens_q,
+              seqused_kv, sinks, out, lse):
         _launch(*call)
     else:
         torch.ops.sas_b200.sparse_attn_sharedkv_fp8(*call)

@@ -14,6 +14,7 @@ import functools
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .api import _dense16, _dtype_code, _i32, _pool16, _ptr
@@ -38,14 +39,32 @@ def rope_table(positions: int, rope_dim: int, *, base: float = 10000.0, inv_freq
     return torch.cat([ang.cos(), ang.sin()], dim=1).to(torch.float32)
 
 
-def _refuse_grad(what: str) -> None:
-    raise ValueError(f"{what} has no backward pass: call it under torch.no_grad() or detach its inputs")
+def _refuse_derivatives(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Raises where one of the call's floating-point tensors would silently get no gradient or lose its tangent."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{what} has no backward pass: call it under torch.no_grad() or detach its inputs")
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{what} has no derivative: pass tensors without tangents")
 
 
-def _eager(t: torch.Tensor) -> bool:
-    """A plain tensor outside tracing: the launch needs no dispatcher (whose Python kernels cost
-    about 10 us a call); fake tensors and torch.compile take the registered op."""
-    return type(t) is torch.Tensor and not torch.compiler.is_compiling()
+_PLAIN = frozenset((torch.Tensor, type(None)))
+
+
+def _eager(*tensors: Optional[torch.Tensor]) -> bool:
+    """Plain tensors outside tracing, modes and transforms: the launch needs no dispatcher (whose Python kernels
+    cost about 10 us a call).  Everything else takes the registered op."""
+    C = torch._C
+    return not (torch.compiler.is_compiling() or C._is_tracing() or C._len_torch_dispatch_stack() or C._len_torch_function_stack()
+                or C._are_functorch_transforms_active()) and _PLAIN.issuperset(map(type, tensors))
+
+
+def _written(*tensors: Optional[torch.Tensor]) -> None:
+    """Tells autograd that a launch has changed these tensors."""
+    torch.autograd.graph.increment_version([t for t in tensors if t is not None])
 
 
 def _int32(t: torch.Tensor, device: int) -> torch.Tensor:
@@ -132,6 +151,7 @@ def _append(kv, cache, cache_scale, block_table, seqused_kv, cu_seqlens_q, rope_
                                       _raw_stream(device))
     if rc:
         _lib.check(rc, "sas_cache_append")
+    _written(cache, cache_scale, q_out)
     if check_status:
         bits = int(word.item())
         if bits:
@@ -193,8 +213,7 @@ def sharedkv_cache_append(
     assert layout_q in ("TND", "BSND"), f"unsupported layout_q={layout_q!r}"
     if not cache.is_cuda:
         raise ValueError("cache must be a CUDA tensor (sas_b200 has no CPU path)")
-    if torch.is_grad_enabled() and (kv.requires_grad or (q is not None and q.requires_grad)):
-        _refuse_grad("sharedkv_cache_append")
+    _refuse_derivatives("sharedkv_cache_append", kv, cache, cache_scale, rope_table, q, q_out)
     device, kind = cache.device, kv.dtype
     if kv.device != device or any(t is not None and t.device != device for t in (cache_scale, rope_table, q, q_out)):
         raise ValueError(f"kv, cache_scale, rope_table, q and q_out must be on {device}")
@@ -244,7 +263,7 @@ def sharedkv_cache_append(
         raise ValueError("q_out goes with q")
     call = (kv, cache, cache_scale, block_table, seqused_kv, cu_seqlens_q, rope_table, bool(rope_interleaved),
             min(int(rope_step), 2**31 - 1), None if q_out is q else q, q_out, layout_q, bool(check_status))
-    if _eager(cache):
+    if _eager(kv, cache, cache_scale, block_table, seqused_kv, cu_seqlens_q, rope_table, q, q_out):
         _append(*call)
     else:
         torch.ops.sas_b200.sharedkv_cache_append(*call)

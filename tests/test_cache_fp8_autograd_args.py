@@ -1,0 +1,52 @@
+"""Arguments that require a gradient and get none are refused before anything is launched (fake CUDA tensors: no GPU)."""
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+from dsv4_planb_b200.attn_fp8 import sparse_attn_sharedkv_fp8
+from dsv4_planb_b200.cache import sharedkv_cache_append
+
+F8 = torch.float8_e4m3fn
+
+
+def empty(*shape, dtype=torch.float32):
+    return torch.empty(shape, dtype=dtype, device="cuda")
+
+
+def append_call(pool):
+    a = dict(cache=empty(4, 128, 1, 576, dtype=pool), block_table=empty(1, 4, dtype=torch.int32), cu_seqlens_q=empty(2, dtype=torch.int32),
+             seqused_kv=empty(1, dtype=torch.int32), rope_table=empty(300, 64), q=empty(3, 8, 576, dtype=torch.bfloat16))
+    if pool is F8:
+        a["cache_scale"] = empty(4)
+    return a
+
+
+@pytest.mark.parametrize("pool,name", [(F8, "kv"), (F8, "cache_scale"), (F8, "rope_table"), (F8, "q"), (F8, "q_out"), (torch.bfloat16, "cache")])
+def test_append(pool, name):
+    with FakeTensorMode():
+        kv, a = empty(3, 576, dtype=torch.bfloat16), append_call(pool)
+        sharedkv_cache_append(kv, **a)
+        a["q_out"] = empty(3, 8, 576, dtype=torch.bfloat16)
+        (kv if name == "kv" else a[name]).requires_grad_()
+        with pytest.raises(ValueError, match="no backward"):
+            sharedkv_cache_append(kv, **a)
+        with torch.no_grad():
+            sharedkv_cache_append(kv, **a)
+
+
+@pytest.mark.parametrize("name", ["q", "ori_kv", "ori_kv_scale", "cmp_kv", "cmp_kv_scale", "sinks", "out", "lse_out"])
+def test_attention(name):
+    with FakeTensorMode():
+        i32 = torch.int32
+        a = dict(ori_kv=empty(4, 128, 1, 576, dtype=F8), ori_kv_scale=empty(4), cmp_kv=empty(4, 128, 1, 576, dtype=F8), cmp_kv_scale=empty(4),
+                 ori_block_table=empty(1, 4, dtype=i32), cmp_block_table=empty(1, 4, dtype=i32), cu_seqlens_q=empty(2, dtype=i32),
+                 seqused_kv=empty(1, dtype=i32), sinks=empty(8), softmax_scale=1.0, cmp_ratio=4, v_head_dim=512,
+                 out=empty(3, 8, 512, dtype=torch.bfloat16), lse_out=empty(3, 8))
+        q = empty(3, 8, 576, dtype=torch.bfloat16)
+        sparse_attn_sharedkv_fp8(q, **a)
+        (q if name == "q" else a[name]).requires_grad_()
+        with pytest.raises(ValueError, match="no backward"):
+            sparse_attn_sharedkv_fp8(q, **a)
+        with torch.no_grad():
+            sparse_attn_sharedkv_fp8(q, **a)
