@@ -492,9 +492,10 @@ extern "C" int sas_cache_append(const SasAppendArgs *args, const void *kv, const
     if (!cu_seqlens_q && (a.max_q_len <= 0 || (int64_t)a.batch * a.max_q_len != a.num_tokens)) {
         if (a.num_tokens != 0) return SAS_ERR_INVALID_ARG;
     }
-    if (a.num_tokens == 0 || a.batch == 0) return SAS_OK;
-    if (!kv || !cache || !block_table || !act_kv_len || (a.rope_dim > 0 && !rope_table) || (e4m3 && !cache_scale) ||
-        (a.num_heads > 0 && (!q || !q_out)))
+    const bool turn_q = a.num_heads > 0;
+    if (a.num_tokens == 0 || (a.batch == 0 && (!turn_q || (q && q == q_out)))) return SAS_OK;
+    if (!kv || !cache || (a.batch > 0 && (!block_table || !act_kv_len)) || (a.rope_dim > 0 && !rope_table) || (e4m3 && !cache_scale) ||
+        (turn_q && (!q || !q_out)))
         return SAS_ERR_INVALID_ARG;
     if (!aligned(kv, 16) || !aligned(q, 16) || !aligned(q_out, 16) || !aligned(cache, 16) || !aligned(rope_table, 16) ||
         !aligned(block_table, 4) || !aligned(cu_seqlens_q, 4) || !aligned(act_q_len, 4) || !aligned(act_kv_len, 4) ||
@@ -527,10 +528,10 @@ extern "C" int sas_cache_append(const SasAppendArgs *args, const void *kv, const
     p.table_len = a.table_len;
     p.q_rows = std::max(a.max_q_len, 1);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    int64_t nq = a.num_heads > 0 ? (int64_t)a.num_tokens * ((a.num_heads + kQHeads - 1) / kQHeads) : 0;
+    int64_t nq = turn_q ? (int64_t)a.num_tokens * ((a.num_heads + kQHeads - 1) / kQHeads) : 0;
     const bool bf16 = a.dtype == SAS_DTYPE_BF16;
-    if (!e4m3) {
-        const int64_t grid = nq + (a.num_tokens + kWarps - 1) / kWarps;
+    if (!e4m3 || a.batch == 0) {  // rows of no request: their query heads are copied, and that is all
+        const int64_t grid = nq + (a.batch > 0 ? (a.num_tokens + kWarps - 1) / kWarps : 0);
         if (grid >= INT32_MAX) return SAS_ERR_UNSUPPORTED;
         p.nq = (int)nq;
         if (bf16) append16_kernel<__nv_bfloat16><<<(unsigned)grid, kThreads, 0, s>>>(p);

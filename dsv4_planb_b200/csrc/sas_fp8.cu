@@ -245,9 +245,10 @@ int sas_kvq_forward(const SasFp8Args *args, const void *q, const void *ori_kv, c
         return SAS_ERR_INVALID_ARG;
     const Layout L = layout_of(a);
     if (!workspace || workspace_bytes < L.total) return SAS_ERR_WORKSPACE;
-    if (a.num_tokens > 0 && (!q || !out || !ori_kv || !ori_scale || !ori_block_table || !act_kv_len))
-        return SAS_ERR_INVALID_ARG;
-    if (a.num_tokens > 0 && a.scenario >= 2 && (!cmp_kv || !cmp_scale || !cmp_block_table)) return SAS_ERR_INVALID_ARG;
+    const bool rows = a.num_tokens > 0, owned = rows && a.batch > 0;  // with no request the tables may be empty
+    if (rows && (!q || !out || !ori_kv || !ori_scale)) return SAS_ERR_INVALID_ARG;
+    if (owned && (!ori_block_table || !act_kv_len)) return SAS_ERR_INVALID_ARG;
+    if (rows && a.scenario >= 2 && (!cmp_kv || !cmp_scale || (owned && !cmp_block_table))) return SAS_ERR_INVALID_ARG;
     if (a.num_tokens > 0 && a.scenario == 3 && a.topk > 0 && !cmp_indices) return SAS_ERR_INVALID_ARG;
     for (const void *x : {q, ori_kv, cmp_kv, (const void *)out, (const void *)workspace})
         if (!aligned(x, 16)) return SAS_ERR_INVALID_ARG;

@@ -49,6 +49,7 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t codes, float f) {
 // calls with the same t; each round the 32 lanes cut the range of candidates 32-fold.
 __device__ __forceinline__ int find_request(const int32_t *__restrict__ cu, int B, int t) {
     const int lane = threadIdx.x & 31;
+    if (B <= 0) return -1;
     int lo = 0, n = B;  // b is in [lo, lo + n)
     while (n > 1) {
         const int step = (n + 31) / 32;
