@@ -492,10 +492,11 @@ extern "C" int sas_cache_append(const SasAppendArgs *args, const void *kv, const
     if (!cu_seqlens_q && (a.max_q_len <= 0 || (int64_t)a.batch * a.max_q_len != a.num_tokens)) {
         if (a.num_tokens != 0) return SAS_ERR_INVALID_ARG;
     }
-    const bool turn_q = a.num_heads > 0;
+    // in place and without a rotation nothing of q moves
+    const bool turn_q = a.num_heads > 0 && !(q && q == q_out && a.rope_dim == 0);
     if (a.num_tokens == 0 || (a.batch == 0 && (!turn_q || (q && q == q_out)))) return SAS_OK;
     if (!kv || !cache || (a.batch > 0 && (!block_table || !act_kv_len)) || (a.rope_dim > 0 && !rope_table) || (e4m3 && !cache_scale) ||
-        (turn_q && (!q || !q_out)))
+        (a.num_heads > 0 && (!q || !q_out)))
         return SAS_ERR_INVALID_ARG;
     if (!aligned(kv, 16) || !aligned(q, 16) || !aligned(q_out, 16) || !aligned(cache, 16) || !aligned(rope_table, 16) ||
         !aligned(block_table, 4) || !aligned(cu_seqlens_q, 4) || !aligned(act_q_len, 4) || !aligned(act_kv_len, 4) ||
