@@ -203,9 +203,9 @@ def sharedkv_cache_append(
     or ``[B, S, N1, D]``) is turned by the same angles into ``q_out`` (new when None; ``q`` itself turns in
     place), which is returned.
 
-    Writes rows of the call's tokens only: padding rows, unmapped blocks, negative positions and positions
-    past the table are skipped (``check_status`` synchronises and raises on the last two and on a block
-    without a valid scale).  In an 8-bit cache a block takes the smallest power-of-two scale that its rows
+    Writes rows of the call's tokens only: padding rows are skipped, and so are rows that their request has no
+    place for (negative positions, positions past the angles or the block table, unmapped blocks).
+    ``check_status`` synchronises and raises on the latter and on a block without a valid scale.  In an 8-bit cache a block takes the smallest power-of-two scale that its rows
     need when its first row arrives, and raises it when later rows need more; the rows already there are
     then rounded to the new scale.  A block may take rows of one request, and of one place of its table, per
     call.  No host synchronisation; graph-capturable.  No backward pass.

@@ -118,6 +118,7 @@ __device__ __forceinline__ Span span_of(const AppendArgs &p, int b) {
     }
     int64_t pos = (int64_t)__ldg(p.act_kv + b) - n;
     if (pos < 0) {  // tokens before the sequence's start have no place
+        if (n > 0) sas::set_status(p.status, SAS_STATUS_BAD_POSITION);
         row -= pos;
         n += (int)pos;
         pos = 0;

@@ -43,7 +43,7 @@ enum {
 
 /* bits set by the calls on the 8-bit cache and by sas_cache_append only */
 #define SAS_STATUS_BAD_SCALE 0x20u    /* a block's scale outside [2^-60, 2^60] (zero, negative, infinite, NaN) */
-#define SAS_STATUS_BAD_POSITION 0x40u /* sas_cache_append: a position past the rope table; the row was skipped */
+#define SAS_STATUS_BAD_POSITION 0x40u /* sas_cache_append: a position below 0 or past the rope table; the row was skipped */
 
 /* SAS_DTYPE_E4M3 is a cache type only (sas_cache_append, sas_kvq_forward). */
 typedef enum { SAS_DTYPE_BF16 = 0, SAS_DTYPE_FP16 = 1, SAS_DTYPE_E4M3 = 2 } SasDtype;
@@ -318,8 +318,9 @@ int sas_noalloc_read_status(uint32_t *status, void *stream);
  *   cache        [block_num][block_size][1][head_dim] cache_dtype (dtype, or e4m3)
  *   cache_scale  [block_num] fp32, e4m3 only: a code stands for code * scale
  *   status       a device word the call ORs SAS_STATUS_* bits into, or NULL
- * Rows of no request, rows before position 0, rows of unmapped blocks and rows past
- * the rope table are not written.  An e4m3 block whose first row is among the new
+ * Rows of no request are not written, and neither are rows that a request has no place
+ * for: positions below 0 or past the rope table (SAS_STATUS_BAD_POSITION), unmapped
+ * blocks and positions past the block table (SAS_STATUS_BAD_BLOCK).  An e4m3 block whose first row is among the new
  * rows takes the smallest power of two s with max |x| <= 448 s (s in [2^-60, 2^60]);
  * any other block keeps its scale or raises it to that value, and the rows already
  * in it are then rounded to the new scale.  Infinities saturate, NaN stays NaN, and

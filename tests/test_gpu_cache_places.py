@@ -19,3 +19,31 @@ def test_queries_without_rotation(cuda_device, interleaved, pool):
         cache, scale, out = run(m, None, q=q, q_out=q if place else None, rope_interleaved=interleaved, check_status=True)
         check(m, cache, scale, None)
         assert torch.equal(out.cpu(), m["q"]) and (out is q) == place
+
+
+@pytest.mark.parametrize("pool", ["fp8", "bf16"])
+@pytest.mark.parametrize("q_lens,kv_lens", [([5], [3]), ([1, 2, 1], [4, 0, 9]), ([300], [40])])
+def test_rows_before_the_start_are_reported(cuda_device, q_lens, kv_lens, pool):
+    """Lengths that do not count the new rows in: rows before position 0 are skipped, and reported."""
+    m = make(q_lens, [max(a, b) for a, b in zip(q_lens, kv_lens)], pool=pool, seed=60)
+    m["seq"] = torch.tensor(kv_lens, dtype=torch.int32)
+    m["where"] = [(b, kv_lens[b] - n + s) for b, n in enumerate(q_lens) for s in range(n)]
+    rope = rope_table(400, 64)
+    check(m, *run(m, rope)[:2], rope)
+    with pytest.raises(RuntimeError, match="bad_position"):
+        run(m, rope, check_status=True)
+
+
+@pytest.mark.parametrize("pool", ["fp8", "bf16"])
+def test_what_is_reported(cuda_device, pool):
+    """Padding is not reported; an unmapped block and the end of the block table are."""
+    m = make([3, 0, 66], [70, 0, 140], pool=pool, seed=62)
+    rope = rope_table(200, 64)
+    kv = torch.cat([m["kv"], m["kv"][:9]]).cuda()
+    check(m, *run(m, rope, kv=kv, check_status=True)[:2], rope)
+    for change in (lambda t: t[2].fill_(-1), lambda t: t.resize_(3, 1)):
+        m = make([3, 0, 66], [70, 0, 140], pool=pool, seed=62)
+        change(m["table"])
+        check(m, *run(m, rope)[:2], rope)
+        with pytest.raises(RuntimeError, match="bad_block"):
+            run(m, rope, check_status=True)
