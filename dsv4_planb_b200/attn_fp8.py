@@ -149,9 +149,12 @@ def sparse_attn_sharedkv_fp8(
     exp(sink) to the softmax's denominator.  Returns ``out`` in the type and layout of ``q`` (last dim
     ``v_head_dim``) and with ``return_softmax_lse`` the natural-log LSE in fp32.
 
+    ``D`` is a multiple of 16 up to 1024 and ``v_head_dim`` (``D`` when None) one of 32 up to 512, so that
+    rows of 576 need it said.  ``kernel``: "tc" (tensor cores: D 512 or 576, ``v_head_dim`` 512, up to 128
+    heads, bf16 q), "simt" (CUDA cores: every shape), "auto".
+
     No host synchronisation (``check_status`` reads the status bits and raises); graph-capturable; no
-    backward pass.  ``kernel``: "tc" (tensor cores: D 512 or 576, ``v_head_dim`` 512, up to 128 heads, bf16
-    q), "simt" (every shape), "auto".
+    backward pass.
     """
     assert layout_q in ("TND", "BSND"), f"unsupported layout_q={layout_q!r}"
     if kernel not in KERNELS:
@@ -172,6 +175,11 @@ def sparse_attn_sharedkv_fp8(
         raise ValueError(f"q must be {'[T, N1, D]' if lead == 1 else '[B, S, N1, D]'} (got {tuple(shape)})")
     N1, D = shape[-2], shape[-1]
     Dv = D if v_head_dim is None else int(v_head_dim)
+    if D % 16 or D > 1024:
+        raise ValueError(f"the head dim must be a multiple of 16 up to 1024 (got {D})")
+    if Dv <= 0 or Dv % 32 or Dv > min(D, 512):
+        given = "" if v_head_dim is not None else ", the head dim: pass v_head_dim"
+        raise ValueError(f"v_head_dim must be a multiple of 32 up to {min(D, 512)} (got {Dv}{given})")
     _check_pool("ori_kv", ori_kv, ori_kv_scale, D, device)
     if ori_block_table.dim() != 2 or ori_block_table.shape[0] < B:
         raise ValueError(f"ori_block_table must be [B>={B}, table_len] (got {tuple(ori_block_table.shape)})")

@@ -1,4 +1,5 @@
-"""Arguments that require a gradient and get none are refused before anything is launched (fake CUDA tensors: no GPU)."""
+"""Arguments that no kernel takes, and arguments that require a gradient and get none, are refused before anything is
+launched (fake CUDA tensors: no GPU)."""
 
 import pytest
 import torch
@@ -50,3 +51,16 @@ def test_attention(name):
             sparse_attn_sharedkv_fp8(q, **a)
         with torch.no_grad():
             sparse_attn_sharedkv_fp8(q, **a)
+
+
+@pytest.mark.parametrize("D,Dv,text", [(576, None, r"up to 512 \(got 576, the head dim: pass v_head_dim"), (576, 528, "multiple of 32 up to 512"),
+                                       (576, 500, "multiple of 32"), (256, 288, "up to 256"), (576, 0, "multiple of 32"), (48, None, "up to 48"),
+                                       (584, 512, "multiple of 16 up to 1024"), (1040, 512, "multiple of 16 up to 1024")])
+def test_value_dims(D, Dv, text):
+    """Sizes that no kernel takes are refused by name, the default of v_head_dim among them."""
+    with FakeTensorMode():
+        i32 = torch.int32
+        with pytest.raises(ValueError, match=text):
+            sparse_attn_sharedkv_fp8(empty(3, 8, D, dtype=torch.bfloat16), ori_kv=empty(4, 128, 1, D, dtype=F8), ori_kv_scale=empty(4),
+                                     ori_block_table=empty(1, 4, dtype=i32), cu_seqlens_q=empty(2, dtype=i32), seqused_kv=empty(1, dtype=i32),
+                                     softmax_scale=1.0, v_head_dim=Dv)
