@@ -16,9 +16,11 @@
 // A QK product costs two 8-bit MMAs, the time of one bf16 MMA, at half the bytes gathered.
 //
 // A key's scale s_j multiplies its score and its value.  With t_ij = scale q_i k_j in log2 units, the
-// weight of value row j (its codes) is 2^(t_ij) s_j, so the running maximum m_i is taken over
-// t_ij + log2 s_j.  e_ij = 2^(t_ij - m_i + 6) adds to the softmax's denominator and
-// P_ij = e_ij s_j goes to the MMA.  The sink joins at the end.
+// weight of value row j (its codes) is 2^(t_ij) s_j = 2^(x_ij) with x_ij = t_ij + log2 s_j.  The running
+// maximum m_i is taken over x_ij, P_ij = 2^(x_ij - m_i + 6) goes to the MMA and e_ij = P_ij / s_j adds to the
+// softmax's denominator.  (P as e s with e = 2^(t - m + 6) saves a constant per key, 0.7 % of a prefill's time, but
+// scores of 2^24 and more, which scales of 2^20 bring with them, have no digits left for log2 s, and P
+// overflows.)  The sink joins at the end.
 //
 // A unit of work (a token, or a piece of one) goes to a cluster of two CTAs on two SMs that split it
 // by role, because O alone (128 heads x 512 fp32) fills one SM's tensor memory:
@@ -95,10 +97,9 @@ static_assert(kRows % 8 == 0 && kProdWarps == 4, "whole swizzle periods, 32 head
 constexpr int kThreads = 32 * (kProdWarp0 + kProdWarps);
 constexpr uint32_t kReaders = 2 * (kSoftWarps + 1 + kProdWarps) - 1;  // of the unit queue: every warp but its writer
 constexpr int kTmemCols = 512, kTmemS = 320;
-// Ring of per-tile key constants.  Those of tile n are written once the stage of tile n - 1 is free: the
-// scores of tile n - 4 are complete, so those of n - 6 have been taken to registers, by warps that are
-// done with tile n - 8.
-constexpr int kConsts = 8;
+// Ring of per-tile key constants.  Those of tile n are written once its stage is free: the scores of tile n - 3 are
+// complete, so that their buffer had been given back by tile n - 5, and the other one by tile n - 6 before.
+constexpr int kConsts = 6;
 constexpr float kTop = 8.75f;        // log2 of the largest P: 431, within e4m3's 448
 constexpr float kRise = 2.75f;       // log2 of the rise of a maximum that is left to P
 constexpr int kMaxPieces = 64;
@@ -114,8 +115,9 @@ constexpr int kMsgLo = 128 * 128, kMsgStats = kMsgLo + 128 * 64, kMsgBytes = kMs
 constexpr int kSlots = 3;
 
 struct KeyConst {
-    float s[kBK];   // scale; 0: a zero row
-    float ls[kBK];  // log2 s; -60 for zero rows (their values do not count), -inf: no key
+    float s[kBK];    // scale; 0: a zero row
+    float ls[kBK];   // log2 s; -60 for zero rows (their values do not count), -inf: no key
+    float inv[kBK];  // 2^-ls; 0: no key
 };
 
 struct Hdr {
@@ -394,9 +396,10 @@ __device__ void producer(const TcArgs &p, const Sync &sy, const CUtensorMap *q_m
             if constexpr (kScore) {
                 KeyConst &c = consts[tiles % kConsts];
                 const bool row = key.row != nullptr;
-                if (holds) {  // ls decides on the frame only, so that an approximation does
+                if (holds) {
                     c.s[key_at] = row ? key.s : key.live ? 0.f : 1.f;
-                    c.ls[key_at] = row ? __log2f(key.s) : key.live ? -60.f : -INFINITY;
+                    c.ls[key_at] = row ? log2f(key.s) : key.live ? -60.f : -INFINITY;
+                    c.inv[key_at] = row ? __frcp_rn(key.s) : key.live ? 0x1p60f : 0.f;
                 }
                 __syncwarp();
                 if (lane == 0) {
@@ -420,9 +423,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
+// To fp16, a in the low half: nearest even, saturating; NaN stays NaN.
 __device__ __forceinline__ uint32_t pack_half(float a, float b) {
-    const __half2 v = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&v);
+    uint32_t r;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
 }
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
@@ -730,7 +735,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 const int nt = it.j1 - it.j0;
                 const uint64_t rq2 = pack2(rq, rq);
-                float m = -INFINITY, l = 0.f;  // of this thread's tiles, l in the frame of m
+                float frame = -INFINITY, l = 0.f;  // of this thread's tiles: the sum of e 2^-frame
                 for (int e = (sc0 & 1) == (uint32_t)g ? 0 : 1; e < nt; e += 2, ++mine) {
                     const uint32_t sc = sc0 + e;
                     if (idle) {
@@ -766,33 +771,26 @@ __global__ void __launch_bounds__(kThreads, 1)
                     hd->m[g][h] = mn;
                     __syncwarp();
                     if (lane == 0) mbar_arrive(smem_u32(&hd->m_bar[warp & 3][g]));
-                    const float mb = mn - (kTop - kRise);
+                    const float mb = mn - (kTop - kRise);  // the tile's frame (rounded: scores may be as large as 2^60)
                     const uint64_t mb2 = pack2(-mb, -mb);
                     // the last message has arrived, so its copies have left the staging buffer
                     if (!wait_on(sy, smem_u32(&hd->p_sent[g]), (mine & 1) ^ 1, true)) goto done;
                     uint64_t sum0 = 0, sum1 = 0;
-                    const int live = it.rec[TR_NORI] + it.rec[TR_NCMP] - (it.j0 + e) * kBK;
 #pragma unroll 1
                     for (int i0 = 0; i0 < kBK; i0 += 16) {
                         uint32_t sr[16], hp[8];
                         tmem_ld16(s_at + i0, sr);
                         tc_wait_ld();
-                        uint64_t f2 = rq2;
-                        if (live - i0 < 16) {  // slots without a key, in the token's last tile: weight 0
-                            f2 = pack2(1.f, 1.f);
-#pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                sr[i] = __float_as_uint(i < live - i0 ? __uint_as_float(sr[i]) * rq : -INFINITY);
-                        }
 #pragma unroll
                         for (int i = 0; i < 16; i += 4) {
                             const ulonglong2 s4 = *reinterpret_cast<const ulonglong2 *>(&c.s[i0 + i]);
-                            const float2 a = unpack2(fma2(mul2(pack2(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1])), f2), s4.x, mb2));
-                            const float2 b = unpack2(fma2(mul2(pack2(__uint_as_float(sr[i + 2]), __uint_as_float(sr[i + 3])), f2), s4.y, mb2));
-                            const uint64_t e0 = pack2(ex2_approx(a.x), ex2_approx(a.y)), e1 = pack2(ex2_approx(b.x), ex2_approx(b.y));
-                            sum0 = add2(sum0, e0);
-                            sum1 = add2(sum1, e1);
-                            const float2 p0 = unpack2(mul2(e0, s4.x)), p1 = unpack2(mul2(e1, s4.y));
+                            const ulonglong2 l4 = *reinterpret_cast<const ulonglong2 *>(&c.ls[i0 + i]);
+                            const ulonglong2 v4 = *reinterpret_cast<const ulonglong2 *>(&c.inv[i0 + i]);
+                            const float2 a = unpack2(add2(fma2(mul2(pack2(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1])), rq2), s4.x, l4.x), mb2));
+                            const float2 b = unpack2(add2(fma2(mul2(pack2(__uint_as_float(sr[i + 2]), __uint_as_float(sr[i + 3])), rq2), s4.y, l4.y), mb2));
+                            const float2 p0 = make_float2(ex2_approx(a.x), ex2_approx(a.y)), p1 = make_float2(ex2_approx(b.x), ex2_approx(b.y));
+                            sum0 = fma2(pack2(p0.x, p0.y), v4.x, sum0);
+                            sum1 = fma2(pack2(p1.x, p1.y), v4.y, sum1);
                             hp[i >> 1] = pack_half(p0.x, p0.y);
                             hp[(i >> 1) + 1] = pack_half(p1.x, p1.y);
                         }
@@ -806,25 +804,25 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(smem_u32(&hd->s_free[g]));
-                    float alpha = e > 0 && mn != before ? exp2f(before - mn) : 1.f;
-                    if (mn != m) {
-                        l *= exp2f(m - mn);  // 0 before the first tile
-                        m = mn;
+                    float alpha = e > 0 && mn != before ? exp2f(before - (kTop - kRise) - mb) : 1.f;
+                    if (mb != frame) {
+                        l *= exp2f(frame - mb);  // 0 before the first tile
+                        frame = mb;
                     }
                     const float2 s0 = unpack2(sum0), s1 = unpack2(sum1);
                     l += (s0.x + s0.y) + (s1.x + s1.y);
                     float fin = 0.f;
                     if (e == nt - 2) {  // the other warp ends the unit: it needs this one's sum, in the frame it ends with
                         hd->l[lc & 1][0][h] = l;
-                        hd->l[lc & 1][1][h] = m;
+                        hd->l[lc & 1][1][h] = frame;
                         __syncwarp();
                         if (lane == 0) mbar_arrive(smem_u32(&hd->l_bar[warp & 3]));
                     } else if (e == nt - 1) {
                         float total = l;
                         if (nt > 1) {
                             if (!wait_on(sy, smem_u32(&hd->l_bar[warp & 3]), lc & 1)) goto done;
-                            const float other = hd->l[lc & 1][0][h], frame = hd->l[lc & 1][1][h];
-                            total += frame == m ? other : other * exp2f(frame - m);
+                            const float other = hd->l[lc & 1][0][h], theirs = hd->l[lc & 1][1][h];
+                            total += theirs == mb ? other : other * exp2f(theirs - mb);
                         }
                         const float own = mb + log2f(total);
                         fin = 1.f / total;

@@ -137,3 +137,33 @@ def test_sharp_scores_and_their_tails(cuda_device):
     size = torch.exp2(torch.arange(128, device="cuda").float() / 8 - 6)
     m["q"] = (m["q"].float() * size[None, :, None]).to(torch.bfloat16)
     check_weights(m, *run(m, kernel="tc", check_status=True), tokens=[0, 13, 39])
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("q_size,scale", [(24, -9), (30, -9), (100, -9), (0, 20), (0, 40), (0, 60), (-40, 40), (60, 20)])
+def test_scores_past_all_digits(cuda_device, q_size, scale, kernel):
+    """Scores whose 32-bit steps are whole nats, by large queries or by large scales: each head takes its best key."""
+    m = make([1] * 40, [1500] * 40, N1=33, K=300, seed=44)
+    m["sinks"] = None
+    m["q"] = (m["q"].float() * 2.0 ** q_size).to(torch.bfloat16)
+    for _, s, _ in (m["ori"], m["cmp"]):
+        s.mul_(2.0 ** (scale + 9))
+        s.clamp_(2.0 ** -60, 2.0 ** 60)
+    out, lse = run(m, kernel=kernel, check_status=True)
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+    if q_size + scale <= 0:  # scores of a hundred nats: no key is clear of the others by 200
+        check(m, out, lse, tokens=[0, 20, 39])
+        return
+    for t in (0, 20, 39):
+        b, p = m["where"][t]
+        ori, cmp_ = ref.visible(m["case"], b, p, m["idx"][t, 0].numpy())
+        k = torch.cat([ref.gather(m["ori"][0][:, :, 0], m["ori"][1], m["ori"][2][b], ori),
+                       ref.gather(m["cmp"][0][:, :, 0], m["cmp"][1], m["cmp"][2][b], cmp_)])
+        s = m["q"][t].double() @ k.T * m["scale"]
+        best = s.topk(2, dim=1)
+        reach = (m["q"][t].double().abs() @ k.abs().T * m["scale"]).amax(dim=1)
+        clear = best.values[:, 0] - best.values[:, 1] > 2 * 40 * 2.0 ** -22 * reach + 200  # more than scores are off by
+        assert clear.sum() > 25
+        v = k[best.indices[:, 0], :512]
+        assert ((out[t].double() - v).abs() <= 2.0 ** -7 * v.abs())[clear].all()
+        assert ((lse[t].double() - best.values[:, 0]).abs() <= 40 * 2.0 ** -22 * reach + 2.0 ** -22 * best.values[:, 0].abs())[clear].all()
