@@ -95,6 +95,15 @@ def _rows2d(kv: torch.Tensor, T: int, D: int) -> torch.Tensor:
     return v
 
 
+def _rows_meet(rows: torch.Tensor, T: int, D: int, at: int, elements: int) -> bool:
+    """Whether some of the T rows of D 16-bit elements lie within ``elements`` such elements from address ``at`` on."""
+    row, step, size = rows.data_ptr(), 2 * rows.stride(0), 2 * D
+    if not elements or row >= at + 2 * elements or row + (T - 1) * step + size <= at:
+        return False
+    first = max((at - row - size) // step + 1, 0)  # the first row that ends behind the address
+    return first < T and row + first * step < at + 2 * elements
+
+
 @functools.lru_cache(maxsize=512)
 def _append_args(*sizes) -> "_lib.SasAppendArgs":
     """The call's sizes as the C struct (nothing of the tensors themselves)."""
@@ -134,6 +143,8 @@ def _append(kv, cache, cache_scale, block_table, seqused_kv, cu_seqlens_q, rope_
         heads, out_at = q_out.shape[-2], q_out.data_ptr()
         if out_at % 16:
             raise ValueError("q_out must start on a 16-byte boundary")
+        if _rows_meet(rows, T, D, out_at, q_out.numel()):
+            raise ValueError("q_out must share nothing with kv")
         if q is None:
             q = q_out  # turned in place
         else:
@@ -201,7 +212,7 @@ def sharedkv_cache_append(
     ``rope_table`` (``rope_table()``; fp32 ``[positions, R]``) turns the last R dims: row p x ``rope_step``
     for position p; ``rope_interleaved`` pairs dims (2 i, 2 i + 1), else (i, i + R / 2).  ``q`` (``[T, N1, D]``
     or ``[B, S, N1, D]``) is turned by the same angles into ``q_out`` (new when None; ``q`` itself turns in
-    place), which is returned.
+    place; it shares nothing with ``kv``), which is returned.
 
     Writes rows of the call's tokens only: padding rows are skipped, and so are rows that their request has no
     place for (negative positions, positions past the angles or the block table, unmapped blocks).

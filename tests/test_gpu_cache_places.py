@@ -47,3 +47,29 @@ def test_what_is_reported(cuda_device, pool):
         check(m, *run(m, rope)[:2], rope)
         with pytest.raises(RuntimeError, match="bad_block"):
             run(m, rope, check_status=True)
+
+
+def test_queries_beside_rows_in_one_buffer(cuda_device):
+    """Queries turn in place in a buffer that holds kv too; a buffer whose heads are kv rows is refused."""
+    rope = rope_table(300, 64)
+    m = make([1], [77], heads=4, seed=63)
+    want = run(m, rope, q=m["q"].cuda())
+    buf = torch.cat([m["q"].reshape(1, -1), m["kv"]], dim=1).cuda()  # [1, (4 + 1) * 576]
+    q = buf[:, :4 * 576].reshape(1, 4, 576)
+    got = run(m, rope, kv=buf[:, 4 * 576:], q=q, q_out=q)
+    assert torch.equal(got[0].view(torch.uint8), want[0].view(torch.uint8)) and torch.equal(q, want[2])
+    m = make([3, 2], [77, 9], heads=4, seed=64)
+    rows = torch.cat([m["q"].reshape(-1, 576), m["kv"]]).cuda()  # queries, then rows
+    q = rows[:20].view(5, 4, 576)
+    check(m, *run(m, rope, kv=rows[20:], q=q, q_out=q)[:2], rope)
+    buf = torch.zeros((5, 4, 576), dtype=torch.bfloat16, device="cuda")
+    for kv in (buf[:, 3], buf[:, 0], buf.view(20, 576)[-5:]):
+        with pytest.raises(ValueError, match="nothing with kv"):
+            run(m, rope, kv=kv, q=buf, q_out=buf)
+        with pytest.raises(ValueError, match="nothing with kv"):
+            run(m, rope, kv=kv, q=m["q"].cuda(), q_out=buf)
+    gaps = torch.zeros((5, 40 * 576), dtype=torch.bfloat16, device="cuda")  # q_out between two rows
+    gaps[:, :576] = m["kv"].cuda()
+    out = gaps[1, 576:21 * 576].view(5, 4, 576)
+    got = run(m, rope, kv=gaps[:, :576], q=m["q"].cuda(), q_out=out, check_status=True)
+    check(m, *got[:2], rope)
