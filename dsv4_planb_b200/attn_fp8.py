@@ -14,8 +14,8 @@ from typing import Optional, Tuple, Union
 import torch
 
 from . import _lib
-from .api import _dense16, _dtype_code, _pool16, _ptr, _scenario, _workspace
-from .cache import _eager, _int32, _ops, _raw_stream, _refuse_derivatives, _written
+from .api import _dense16, _dtype_code, _pool16, _scenario
+from .cache import _current_device, _eager, _int32, _ops, _raw_stream, _refuse_derivatives, _written
 
 KERNELS = {"auto": 0, "simt": 1, "tc": 2}
 _INT32 = 2**31 - 1  # no position lies beyond it
@@ -34,7 +34,7 @@ def _launch(q, ori_kv, ori_kv_scale, cmp_kv, cmp_kv_scale, cmp_sparse_indices, o
             cu_seqlens_q, seqused_kv, sinks, softmax_scale, cmp_ratio, ori_win_left, ori_first, layout_q, v_head_dim,
             kernel, check_status, out, lse):
     device = q.get_device()
-    if device != torch.cuda.current_device():
+    if device != _current_device():
         with torch.cuda.device(device):
             return _launch(q, ori_kv, ori_kv_scale, cmp_kv, cmp_kv_scale, cmp_sparse_indices, ori_block_table,
                            cmp_block_table, cu_seqlens_q, seqused_kv, sinks, softmax_scale, cmp_ratio, ori_win_left,
@@ -68,15 +68,20 @@ def _launch(q, ori_kv, ori_kv_scale, cmp_kv, cmp_kv_scale, cmp_sparse_indices, o
     ob, obs, _, _ = ori_kv.shape
     args, nbytes = _call_args(B, T, S, N1, D, v_head_dim, ob, obs, ori_bt.shape[1], cb, cs, ct, K, cmp_ratio, scenario,
                               ori_win_left, ori_first, _dtype_code(q.dtype), softmax_scale, KERNELS[kernel])
-    ws = _workspace(nbytes, q.device)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)  # from the caching allocator, in stream order
     out_user = None
     if out.data_ptr() % 16:  # a caller's out that starts inside a 16-byte vector
         out_user, out = out, torch.empty_like(out)
     lib = _lib.load()
     stream = _raw_stream(device)
+    # (conditions in place: eight calls of _ptr cost 1 us)
     rc = lib.sas_kvq_forward(args, q.data_ptr(), ori_kv.data_ptr(), ori_kv_scale.data_ptr(), ori_bt.data_ptr(),
-                             _ptr(cmp_kv), _ptr(cmp_kv_scale), _ptr(cmp_bt), _ptr(idx), _ptr(cu), _ptr(act_q),
-                             seq.data_ptr(), _ptr(sinks), out.data_ptr(), _ptr(lse), ws.data_ptr(), nbytes, stream)
+                             None if cmp_kv is None else cmp_kv.data_ptr(),
+                             None if cmp_kv is None else cmp_kv_scale.data_ptr(),
+                             None if cmp_bt is None else cmp_bt.data_ptr(), None if idx is None else idx.data_ptr(),
+                             None if cu is None else cu.data_ptr(), None if act_q is None else act_q.data_ptr(),
+                             seq.data_ptr(), None if sinks is None else sinks.data_ptr(), out.data_ptr(),
+                             None if lse is None else lse.data_ptr(), ws.data_ptr(), nbytes, stream)
     if rc:
         _lib.check(rc, "sas_kvq_forward")
     if out_user is not None:
@@ -102,7 +107,7 @@ def _fake(*args):
     return None
 
 
-def _check_pool(name, pool, scale, D, device):
+def _check_pool(name, pool, scale, D, q):
     if pool.dtype is not torch.float8_e4m3fn:
         raise ValueError(f"{name} must be float8_e4m3fn (got {pool.dtype}); 16-bit pools go to sparse_attn_sharedkv")
     shape = pool.shape
@@ -110,8 +115,8 @@ def _check_pool(name, pool, scale, D, device):
         raise ValueError(f"{name} must be [blocks, block_size, 1, {D}] (got {tuple(shape)})")
     if scale is None or scale.dtype is not torch.float32 or scale.numel() != shape[0] or not scale.is_contiguous():
         raise ValueError(f"{name}_scale must be contiguous float32 with one entry per block of {name}")
-    if pool.device != device or scale.device != device:
-        raise ValueError(f"{name} and {name}_scale must be on {device}")
+    if not pool.get_device() == scale.get_device() == q.get_device():
+        raise ValueError(f"{name} and {name}_scale must be on {q.device}")
 
 
 def sparse_attn_sharedkv_fp8(
@@ -162,7 +167,7 @@ def sparse_attn_sharedkv_fp8(
     if not q.is_cuda:
         raise ValueError("q must be a CUDA tensor (sas_b200 has no CPU path)")
     _refuse_derivatives("sparse_attn_sharedkv_fp8", q, ori_kv, ori_kv_scale, cmp_kv, cmp_kv_scale, sinks, out, lse_out)
-    shape, device, kind = q.shape, q.device, q.dtype
+    shape, kind = q.shape, q.dtype
     if layout_q == "TND":
         lead = 1
         assert cu_seqlens_q is not None, "cu_seqlens_q is required for TND"
@@ -180,14 +185,14 @@ def sparse_attn_sharedkv_fp8(
     if Dv <= 0 or Dv % 32 or Dv > min(D, 512):
         given = "" if v_head_dim is not None else ", the head dim: pass v_head_dim"
         raise ValueError(f"v_head_dim must be a multiple of 32 up to {min(D, 512)} (got {Dv}{given})")
-    _check_pool("ori_kv", ori_kv, ori_kv_scale, D, device)
+    _check_pool("ori_kv", ori_kv, ori_kv_scale, D, q)
     if ori_block_table.dim() != 2 or ori_block_table.shape[0] < B:
         raise ValueError(f"ori_block_table must be [B>={B}, table_len] (got {tuple(ori_block_table.shape)})")
     if seqused_kv.numel() < B:
         raise ValueError(f"seqused_kv must have {B} entries (got {seqused_kv.numel()})")
     if cmp_kv is not None:
         assert cmp_ratio is not None, "cmp_ratio is required with cmp_kv"
-        _check_pool("cmp_kv", cmp_kv, cmp_kv_scale, D, device)
+        _check_pool("cmp_kv", cmp_kv, cmp_kv_scale, D, q)
         if cmp_block_table is None or cmp_block_table.dim() != 2 or cmp_block_table.shape[0] < B:
             raise ValueError(f"cmp_block_table must be [B>={B}, table_len]")
         if cmp_sparse_indices is not None:
@@ -205,20 +210,19 @@ def sparse_attn_sharedkv_fp8(
         result = out = q.new_empty((*tokens, N1, Dv))
     else:
         result = out.view((*tokens, N1, Dv)) if out.is_contiguous() and out.numel() == tokens.numel() * N1 * Dv else None
-        if result is None or out.dtype is not kind or out.device != device:
-            raise ValueError(f"out must be contiguous {kind} of shape {(*tokens, N1, Dv)} on {device}")
+        if result is None or out.dtype is not kind or out.get_device() != q.get_device():
+            raise ValueError(f"out must be contiguous {kind} of shape {(*tokens, N1, Dv)} on {q.device}")
     lse = sums = lse_out
     if lse is not None:
         sums = lse.view((*tokens, N1)) if lse.is_contiguous() and lse.numel() == tokens.numel() * N1 else None
-        if sums is None or lse.dtype is not torch.float32 or lse.device != device:
-            raise ValueError(f"lse_out must be contiguous float32 of shape {(*tokens, N1)} on {device}")
+        if sums is None or lse.dtype is not torch.float32 or lse.get_device() != q.get_device():
+            raise ValueError(f"lse_out must be contiguous float32 of shape {(*tokens, N1)} on {q.device}")
     elif return_softmax_lse:
         lse = sums = q.new_empty((*tokens, N1), dtype=torch.float32)
     call = (q, ori_kv, ori_kv_scale, cmp_kv, cmp_kv_scale, cmp_sparse_indices, ori_block_table, cmp_block_table,
             cu_seqlens_q, seqused_kv, sinks, float(softmax_scale), 4 if cmp_ratio is None else min(int(cmp_ratio), _INT32),
             min(int(ori_win_left), _INT32), min(int(ori_first), _INT32), layout_q, Dv, kernel, bool(check_status), out, lse)
-    if _eager(q, ori_kv, ori_kv_scale, cmp_kv, cmp_kv_scale, cmp_sparse_indices, ori_block_table, cmp_block_table, cu_seqlens_q,
-              seqused_kv, sinks, out, lse):
+    if _eager(q, ori_kv, cmp_kv, out, lse):
         _launch(*call)
     else:
         torch.ops.sas_b200.sparse_attn_sharedkv_fp8(*call)

@@ -52,19 +52,21 @@ def _refuse_derivatives(what: str, *tensors: Optional[torch.Tensor]) -> None:
 
 
 _PLAIN = frozenset((torch.Tensor, type(None)))
+_is_tracing, _transforms = torch._C._is_tracing, torch._C._are_functorch_transforms_active
+_dispatch_modes, _function_modes = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack
+_increment_version = torch._C._increment_version  # torch.autograd.graph.increment_version takes half a us more
 
 
 def _eager(*tensors: Optional[torch.Tensor]) -> bool:
     """Plain tensors outside tracing, modes and transforms: the launch needs no dispatcher (whose Python kernels
     cost about 10 us a call).  Everything else takes the registered op."""
-    C = torch._C
-    return not (torch.compiler.is_compiling() or C._is_tracing() or C._len_torch_dispatch_stack() or C._len_torch_function_stack()
-                or C._are_functorch_transforms_active()) and _PLAIN.issuperset(map(type, tensors))
+    return not (torch.compiler.is_compiling() or _is_tracing() or _dispatch_modes() or _function_modes()
+                or _transforms()) and _PLAIN.issuperset(map(type, tensors))
 
 
 def _written(*tensors: Optional[torch.Tensor]) -> None:
     """Tells autograd that a launch has changed these tensors."""
-    torch.autograd.graph.increment_version([t for t in tensors if t is not None])
+    _increment_version([t for t in tensors if t is not None])
 
 
 def _int32(t: torch.Tensor, device: int) -> torch.Tensor:
@@ -76,6 +78,7 @@ def _int32(t: torch.Tensor, device: int) -> torch.Tensor:
 
 # The current stream's handle: torch.cuda.current_stream builds a Stream object first (3 us a call).
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)  # of an initialised CUDA: 1 us less
 
 
 def _rows2d(kv: torch.Tensor, T: int, D: int) -> torch.Tensor:
@@ -95,13 +98,13 @@ def _rows2d(kv: torch.Tensor, T: int, D: int) -> torch.Tensor:
     return v
 
 
-def _rows_meet(rows: torch.Tensor, T: int, D: int, at: int, elements: int) -> bool:
-    """Whether some of the T rows of D 16-bit elements lie within ``elements`` such elements from address ``at`` on."""
-    row, step, size = rows.data_ptr(), 2 * rows.stride(0), 2 * D
-    if not elements or row >= at + 2 * elements or row + (T - 1) * step + size <= at:
+def _rows_meet(rows: torch.Tensor, T: int, D: int, at: int, size: int) -> bool:
+    """Whether some of the T rows of D 16-bit elements lie within ``size`` bytes from address ``at`` on."""
+    row, step = rows.data_ptr(), 2 * rows.stride(0)
+    if not size or row >= at + size or row + (T - 1) * step + 2 * D <= at:
         return False
-    first = max((at - row - size) // step + 1, 0)  # the first row that ends behind the address
-    return first < T and row + first * step < at + 2 * elements
+    first = max((at - row - 2 * D) // step + 1, 0)  # the first row that ends behind the address
+    return first < T and row + first * step < at + size
 
 
 @functools.lru_cache(maxsize=512)
@@ -113,7 +116,7 @@ def _append_args(*sizes) -> "_lib.SasAppendArgs":
 def _append(kv, cache, cache_scale, block_table, seqused_kv, cu_seqlens_q, rope_table, rope_interleaved, rope_step, q,
             q_out, layout_q, check_status):
     device = cache.get_device()
-    if device != torch.cuda.current_device():
+    if device != _current_device():
         with torch.cuda.device(device):
             return _append(kv, cache, cache_scale, block_table, seqused_kv, cu_seqlens_q, rope_table, rope_interleaved,
                            rope_step, q, q_out, layout_q, check_status)
@@ -137,19 +140,20 @@ def _append(kv, cache, cache_scale, block_table, seqused_kv, cu_seqlens_q, rope_
         if cu is not None:
             cu, act_q = None, (cu[1:] - cu[:-1]).contiguous()
     rows = _rows2d(kv, T, D)
+    rows_at = rows.data_ptr()
     table, seq = _int32(block_table, device), _int32(seqused_kv, device)
     heads = q_at = out_at = 0
     if q_out is not None:
         heads, out_at = q_out.shape[-2], q_out.data_ptr()
         if out_at % 16:
             raise ValueError("q_out must start on a 16-byte boundary")
-        if _rows_meet(rows, T, D, out_at, q_out.numel()):
+        n = 2 * q_out.numel()
+        if rows_at < out_at + n and _rows_meet(rows, T, D, out_at, n):
             raise ValueError("q_out must share nothing with kv")
         if q is None:
             q = q_out  # turned in place
         else:
             d = q.data_ptr() - out_at
-            n = q_out.numel() * q_out.element_size()
             if -n < d < n and n and not (d == 0 and q.is_contiguous()):
                 raise ValueError("q_out must be q itself or share nothing with it")
             q = _dense16(q)
@@ -157,7 +161,7 @@ def _append(kv, cache, cache_scale, block_table, seqused_kv, cu_seqlens_q, rope_
     args = _append_args(B, T, heads, D, R, int(rope_interleaved), rope_step, rope_rows, blocks, bs, table.shape[1], S,
                         _dtype_code(kv.dtype), _CACHE_DTYPES[cache.dtype], rows.stride(0) if T > 1 else D)
     word = torch.zeros(1, dtype=torch.int32, device=cache.device) if check_status else None
-    rc = _lib.load().sas_cache_append(args, rows.data_ptr(), q_at, out_at, rope_at, table.data_ptr(), _ptr(cu),
+    rc = _lib.load().sas_cache_append(args, rows_at, q_at, out_at, rope_at, table.data_ptr(), _ptr(cu),
                                       _ptr(act_q), seq.data_ptr(), cache.data_ptr(), _ptr(cache_scale), _ptr(word),
                                       _raw_stream(device))
     if rc:
@@ -225,9 +229,10 @@ def sharedkv_cache_append(
     if not cache.is_cuda:
         raise ValueError("cache must be a CUDA tensor (sas_b200 has no CPU path)")
     _refuse_derivatives("sharedkv_cache_append", kv, cache, cache_scale, rope_table, q, q_out)
-    device, kind = cache.device, kv.dtype
-    if kv.device != device or any(t is not None and t.device != device for t in (cache_scale, rope_table, q, q_out)):
-        raise ValueError(f"kv, cache_scale, rope_table, q and q_out must be on {device}")
+    device, kind = cache.get_device(), kv.dtype
+    for t in (kv, cache_scale, rope_table, q, q_out):
+        if t is not None and t.get_device() != device:
+            raise ValueError(f"kv, cache_scale, rope_table, q and q_out must be on {cache.device}")
     if kind is not torch.bfloat16 and kind is not torch.float16:
         raise ValueError(f"kv must be bfloat16 or float16 (got {kind})")
     if cache.dim() != 4 or cache.shape[2] != 1:
@@ -274,7 +279,7 @@ def sharedkv_cache_append(
         raise ValueError("q_out goes with q")
     call = (kv, cache, cache_scale, block_table, seqused_kv, cu_seqlens_q, rope_table, bool(rope_interleaved),
             min(int(rope_step), 2**31 - 1), None if q_out is q else q, q_out, layout_q, bool(check_status))
-    if _eager(kv, cache, cache_scale, block_table, seqused_kv, cu_seqlens_q, rope_table, q, q_out):
+    if _eager(kv, cache, cache_scale, q, q_out):
         _append(*call)
     else:
         torch.ops.sas_b200.sharedkv_cache_append(*call)
