@@ -9,7 +9,7 @@
 // hi in e4m3, then two e5m2 terms, which reach 2^-16 where hi has no bits left.  hi leaves at most 2^-4 of
 // a weight's power of two (2^-10 where it is subnormal), and each e5m2 term cuts three bits off what is left:
 // 2^-10 of a weight, or 2^-16 of a scale in which the row's largest weight is 2^6 or more.  Two e4m3 terms, whose
-// smallest step is 2^-9, took 10 % less time (1.06 ms instead of 1.19 for 2048 tokens, 69.5 us instead of 76
+// smallest step is 2^-9, took 5 to 9 % less time (1.06 ms instead of 1.16 for 2048 tokens, 69.5 us instead of 73
 // for 64; the products of V in the output CTA are 18 MMAs a tile instead of 12), but lost every weight below
 // 2^-16 of the largest: 3 to 50 % of the output where one key with a small value holds 80 to 99 % of a row.
 // One e5m2 term behind hi takes no more time than that, but loses 2^-8 of a weight where two e4m3 terms lose 2^-9.
@@ -106,12 +106,11 @@ constexpr int kMaxPieces = 64;
 
 // P message: per head 96 weights in fp16, 64 in a 128-byte row (SW128) and 32 in a 64-byte row (SW64), then
 // {alpha, the unit's final factor}.  The 32 heads of a warp are contiguous in each part.  The output CTA
-// puts codes in the weights' place: 96 hi and 32 mid in the first row, the other 64 mid in the second; lo goes
-// to a buffer of its own.
+// puts codes in the weights' place, per 32 keys 32 hi and 32 mid; lo goes to a buffer of its own.
 constexpr int kMsgLo = 128 * 128, kMsgStats = kMsgLo + 128 * 64, kMsgBytes = kMsgStats + 1024;
 
-// Messages under way.  A slot is held from its copy's start over the split to the end of its product: 64 tokens take
-// 79 us with two slots, 76 with three or four.
+// Messages under way.  A slot is held from its copy's start over the split to the end of its product: with two of them
+// 64 tokens take 4 % more time, with four as much as with three.
 constexpr int kSlots = 3;
 
 struct KeyConst {
@@ -136,18 +135,19 @@ constexpr int kConstOff = kHdr;
 constexpr int kScoreMsgs = (kConstOff + kConsts * (int)sizeof(KeyConst) + 1023) / 1024 * 1024;
 constexpr int kScoreRing = kScoreMsgs + 2 * kMsgBytes;
 constexpr int kScoreSmem = kScoreRing + kStages * kKStage;
-constexpr int kOutRing = kHdr;
+constexpr int kOutRing = 1024;  // behind the barriers: the rest of the header is the score CTA's
+static_assert(offsetof(Hdr, amax) <= kOutRing, "barriers of the output CTA");
 constexpr int kOutMsgs = kOutRing + kVStages * kVStage;
-// Third terms of the weights, for even and for odd tiles: per 8 heads three blocks of 32 keys, each 8 rows of 32 bytes
-// (SW32), so that a warp's 32 heads are contiguous.
+// Third terms of a slot's weights: per 8 heads three blocks of 32 keys, each 8 rows of 32 bytes (SW32).  (Two buffers for
+// even and odd tiles, which a split waits for, leave room for a second staging buffer per warp: 2 % slower.)
 constexpr int kThirdBytes = 128 / 8 * 3 * 256;
 constexpr int kOutThirds = kOutMsgs + kSlots * kMsgBytes;
-constexpr int kOutStage = kOutThirds + 2 * kThirdBytes;  // epilogue staging: 64 bytes of 32 heads per warp
+constexpr int kOutStage = kOutThirds + kSlots * kThirdBytes;  // epilogue staging: 64 bytes of 32 heads per warp
 constexpr int kWarpSlab = 32 * 64;
 constexpr int kOutSmem = kOutStage + kSoftWarps * kWarpSlab;
 constexpr int kSmemBytes = (kScoreSmem > kOutSmem ? kScoreSmem : kOutSmem) + 1024;  // + alignment slack
 static_assert(kScoreMsgs % 1024 == 0 && kScoreRing % 1024 == 0 && kKStage % 1024 == 0 && kOutRing % 1024 == 0 &&
-              kOutMsgs % 1024 == 0 && kMsgBytes % 1024 == 0 && kOutStage % 1024 == 0 && kThirdBytes / 4 % 512 == 0 && kThirdBytes / 4 >= kWarpSlab, "swizzled tiles are 1 KiB aligned");
+              kOutMsgs % 1024 == 0 && kMsgBytes % 1024 == 0 && kOutStage % 1024 == 0 && kThirdBytes % 1024 == 0, "swizzled tiles are 1 KiB aligned");
 static_assert(kQPerStage * kQChunk <= kKStage && kSmemBytes <= 232448, "shared memory");
 
 // n / d for 0 <= n < 2^31 as a multiplication: 2^(32 + s) <= m d < 2^(32 + s) + 2^(s + 1) with 2^s < d <= 2^(s + 1)
@@ -881,7 +881,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (!wait_on(sy, smem_u32(&hd->full[st]), phase)) goto done;
                     fence_proxy_async_smem();  // the rows were written by cp.async
                     const uint64_t a1 = sdesc_sw128(smem_u32(msg), 16, 1024), a2 = sdesc_sw64(smem_u32(msg) + kMsgLo, 512);
-                    const uint64_t a3 = sdesc_sw32(smem_u32(smem + kOutThirds) + (pc & 1) * kThirdBytes, 768);
+                    const uint64_t a3 = sdesc_sw32(smem_u32(smem + kOutThirds) + ps * kThirdBytes, 768);
                     const uint32_t base = smem_u32(ring) + st * kVStage;
 #pragma unroll 1
                     for (int c = 0; c < 2; ++c) {  // 256 value dims each
@@ -892,8 +892,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                             const uint32_t d = tmem + c * 256;
 #pragma unroll
                             for (int i = 0; i < kBK / 32; ++i) {
-                                mma8_ss(d, a1 + 2 * i, b + 256 * i, idesc, (j > it.j0 || i > 0) ? 1u : 0u);
-                                mma8_ss(d, i == 0 ? a1 + 6 : a2 + 2 * (i - 1), b + 256 * i, idesc5, 1u);
+                                const uint64_t a = i < 2 ? a1 + 4 * i : a2;
+                                mma8_ss(d, a, b + 256 * i, idesc, (j > it.j0 || i > 0) ? 1u : 0u);
+                                mma8_ss(d, a + 2, b + 256 * i, idesc5, 1u);
                                 mma8_ss(d, a3 + 16 * i, b + 256 * i, idesc5, 1u);
                             }
                             tc_commit(smem_u32(&hd->pv_done[c][ps]));
@@ -918,7 +919,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool head = h < p.N1;
             const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16);
             const uint32_t sw1 = (h & 7) << 4, sw2 = ((h >> 1) & 3) << 4, sw3 = ((h >> 2) & 1) << 4;
-            uint8_t *const thirds = smem + kOutThirds + g * kThirdBytes + (h >> 3) * 768 + (h & 7) * 32;
+            uint8_t *const thirds = smem + kOutThirds + (h >> 3) * 768 + (h & 7) * 32;
             uint32_t ofc = 0, pc = 0;
             for (uint32_t k = 0;; ++k) {
                 int u;
@@ -947,29 +948,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                             mbar_arrive_remote(map_to_cta(smem_u32(&hd->p_sent[g]), 0));
                         }
                         if ((warp & 3) < quads) {
-                            // the thirds' buffer is free: the product of two tiles before, and the last unit's stores
-                            if (pc >= 2 && !wait_on(sy, smem_u32(&hd->pv_done[1][(pc - 2) % kSlots]), ((pc - 2) / kSlots) & 1)) goto done;
-                            if (lane == 0) bulk_wait_read<0>();
-                            __syncwarp();
-                            uint8_t *row1 = msg + h * 128, *row2 = msg + kMsgLo + h * 64;
-                            uint4 x[12], y[12];
+                            // 32 keys at a time, hi and mid in the place of their weights (short code: one stretch for all 96
+                            // keys takes 0.8 % more of a prefill's time)
+#pragma unroll 1
+                            for (int i = 0; i < kBK / 32; ++i) {
+                                uint8_t *const row = i < 2 ? msg + h * 128 : msg + kMsgLo + h * 64;
+                                const uint32_t g0 = i == 1 ? 64 : 0, sw = i < 2 ? sw1 : sw2;
+                                uint4 x[4], y[4];
 #pragma unroll
-                            for (int v = 0; v < 8; ++v) x[v] = *reinterpret_cast<const uint4 *>(row1 + ((v << 4) ^ sw1));
+                                for (int c = 0; c < 4; ++c) x[c] = *reinterpret_cast<const uint4 *>(row + ((g0 + c * 16) ^ sw));
 #pragma unroll
-                            for (int v = 0; v < 4; ++v) x[8 + v] = *reinterpret_cast<const uint4 *>(row2 + ((v << 4) ^ sw2));
+                                for (int c = 0; c < 2; ++c) {
+                                    uint4 z;
+                                    split4w(x[2 * c].x, x[2 * c].y, y[c].x, y[2 + c].x, z.x);
+                                    split4w(x[2 * c].z, x[2 * c].w, y[c].y, y[2 + c].y, z.y);
+                                    split4w(x[2 * c + 1].x, x[2 * c + 1].y, y[c].z, y[2 + c].z, z.z);
+                                    split4w(x[2 * c + 1].z, x[2 * c + 1].w, y[c].w, y[2 + c].w, z.w);
+                                    *reinterpret_cast<uint4 *>(thirds + ps * kThirdBytes + i * 256 + ((c << 4) ^ sw3)) = z;
+                                }
 #pragma unroll
-                            for (int v = 0; v < 6; ++v) {
-                                uint4 z;
-                                split4w(x[2 * v].x, x[2 * v].y, y[v].x, y[6 + v].x, z.x);
-                                split4w(x[2 * v].z, x[2 * v].w, y[v].y, y[6 + v].y, z.y);
-                                split4w(x[2 * v + 1].x, x[2 * v + 1].y, y[v].z, y[6 + v].z, z.z);
-                                split4w(x[2 * v + 1].z, x[2 * v + 1].w, y[v].w, y[6 + v].w, z.w);
-                                *reinterpret_cast<uint4 *>(thirds + (v >> 1) * 256 + ((v & 1) ? 16 ^ sw3 : sw3)) = z;
+                                for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4 *>(row + ((g0 + c * 16) ^ sw)) = y[c];
                             }
-#pragma unroll
-                            for (int v = 0; v < 8; ++v) *reinterpret_cast<uint4 *>(row1 + ((v << 4) ^ sw1)) = y[v];
-#pragma unroll
-                            for (int v = 0; v < 4; ++v) *reinterpret_cast<uint4 *>(row2 + ((v << 4) ^ sw2)) = y[8 + v];
                             fence_proxy_async_smem();
                         }
                     }
@@ -1015,21 +1014,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // Each warp stages 64 bytes of its 32 head rows (64-byte swizzle) and writes them out: one TMA
                 // store, or 64-byte pieces of rows where a box would reach into the next token's heads.  Whole
                 // tokens in bf16, pieces in fp32, normalised within the piece.  (Direct stores, 16 bytes a lane
-                // to 32 rows, took 9.5 us for a piece; one buffer per warp 0.5 us more than two.)
+                // to 32 rows, took 9.5 us for a piece.)
                 if ((warp & 3) * 32 < p.N1) {
-                    // two buffers: one of its own, and this warp's part of the thirds, which no product reads any more
-                    uint8_t *const buf0 = smem + kOutStage + warp * kWarpSlab;
-                    uint8_t *const buf1 = smem + kOutThirds + g * kThirdBytes + (warp & 3) * (kThirdBytes / 4);
+                    uint8_t *const at = smem + kOutStage + warp * kWarpSlab;
+                    const uint32_t buf = smem_u32(at);
                     const bool piece = it.np > 1;
                     const int row = piece ? ((it.t * p.P + it.piece) * p.NP + (warp & 3) * 32) : it.t * p.N1 + (warp & 3) * 32;
                     const int step = piece ? 16 : 32;
 #pragma unroll 1
                     for (int c = 0; c < kDv / 2; c += step) {
-                        uint8_t *const at = c & step ? buf1 : buf0;
-                        const uint32_t buf = smem_u32(at);
                         uint32_t r[32], w[16];
                         tmem_ld32(tcol + (c & ~31), r);
-                        if (lane == 0) bulk_wait_read<1>();  // the store before the last has read buf
+                        if (lane == 0) bulk_wait_read<0>();  // the last store has read buf
                         __syncwarp();
                         tc_wait_ld();
                         if (piece) {
