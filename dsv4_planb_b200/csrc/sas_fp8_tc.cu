@@ -9,7 +9,7 @@
 // hi in e4m3, then two e5m2 terms, which reach 2^-16 where hi has no bits left.  hi leaves at most 2^-4 of
 // a weight's power of two (2^-10 where it is subnormal), and each e5m2 term cuts three bits off what is left:
 // 2^-10 of a weight, or 2^-16 of a scale in which the row's largest weight is 2^6 or more.  Two e4m3 terms, whose
-// smallest step is 2^-9, took 5 to 9 % less time (1.06 ms instead of 1.16 for 2048 tokens, 69.5 us instead of 73
+// smallest step is 2^-9, took 5 to 8 % less time (1.06 ms instead of 1.14 for 2048 tokens, 67.7 us instead of 71.6
 // for 64; the products of V in the output CTA are 18 MMAs a tile instead of 12), but lost every weight below
 // 2^-16 of the largest: 3 to 50 % of the output where one key with a small value holds 80 to 99 % of a row.
 // One e5m2 term behind hi takes no more time than that, but loses 2^-8 of a weight where two e4m3 terms lose 2^-9.
@@ -36,7 +36,7 @@
 //   8 warps split Q; softmax (thread = head;     8 warps split P (thread = head; warps 0-3 the even
 //           warps 0-3 take the even tiles,               tiles, 4-7 the odd ones); rescale O where a
 //           4-7 the odd ones); P in fp16 and             maximum rose; epilogue
-//           factors go to CTA 1 by bulk copies
+//           factors go to CTA 1 by bulk copies   1 warp  acknowledges messages
 //
 // What the pieces measured on B200, each alone, and what follows from it:
 //   - An MMA of N 64 takes 58 cycles, as one of N 96; N 128 takes 70-83.  96 keys leave room in TMEM for
@@ -94,8 +94,11 @@ static_assert((512 / 64 + kQPerStage - 1) / kQPerStage == kQStages, "the last st
 constexpr int kSoftWarps = 8, kMmaWarp = 8, kProdWarp0 = 9, kProdWarps = 4;
 constexpr int kRows = kBK / kProdWarps;
 static_assert(kRows % 8 == 0 && kProdWarps == 4, "whole swizzle periods, 32 heads of Q a warp");
-constexpr int kThreads = 32 * (kProdWarp0 + kProdWarps);
-constexpr uint32_t kReaders = 2 * (kSoftWarps + 1 + kProdWarps) - 1;  // of the unit queue: every warp but its writer
+// The output CTA's warp that gives the staging of messages back as they arrive.  Done by the warps that split them, after
+// their last rescale, it held the score CTA up: 64 tokens took 73 us instead of 71.6, 256 mixed requests 123 instead of 120.
+constexpr int kAckWarp = kProdWarp0 + kProdWarps;
+constexpr int kThreads = 32 * (kAckWarp + 1);
+constexpr uint32_t kReaders = 2 * kAckWarp;  // of the unit queue: every warp but its writer and the score CTA's last
 constexpr int kTmemCols = 512, kTmemS = 320;
 // Ring of per-tile key constants.  Those of tile n are written once its stage is free: the scores of tile n - 3 are
 // complete, so that their buffer had been given back by tile n - 5, and the other one by tile n - 6 before.
@@ -396,10 +399,11 @@ __device__ void producer(const TcArgs &p, const Sync &sy, const CUtensorMap *q_m
             if constexpr (kScore) {
                 KeyConst &c = consts[tiles % kConsts];
                 const bool row = key.row != nullptr;
-                if (holds) {
+                if (holds) {  // the copies wait for this: approximations, off by 2^-22 (a weight is off by 2^-11 as it is)
+                    const float ls = row ? __log2f(key.s) : -60.f;
                     c.s[key_at] = row ? key.s : key.live ? 0.f : 1.f;
-                    c.ls[key_at] = row ? log2f(key.s) : key.live ? -60.f : -INFINITY;
-                    c.inv[key_at] = row ? __frcp_rn(key.s) : key.live ? 0x1p60f : 0.f;
+                    c.ls[key_at] = key.live ? ls : -INFINITY;
+                    c.inv[key_at] = key.live ? ex2_approx(-ls) : 0.f;
                 }
                 __syncwarp();
                 if (lane == 0) {
@@ -606,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     cluster_sync();  // both CTAs' barriers are initialised before any remote arrive
     tc_fence_after();
-    if (rank == 1 && warp < kProdWarp0) wait_resolved();  // the others wait when they need a record
+    if (rank == 1 && (warp < kProdWarp0 || warp == kAckWarp)) wait_resolved();  // the others wait when they need a record
     if (p.P > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem = hd->tmem_base;
     Sync sy{&hd->abort, p.status, map_to_cta(smem_u32((const void *)&hd->abort), rank ^ 1u), hd->tq_full, hd->tq_empty,
@@ -616,7 +620,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         // ======================= score CTA =======================
         uint8_t *ring = smem + kScoreRing;
         KeyConst *consts = reinterpret_cast<KeyConst *>(smem + kConstOff);
-        if (warp >= kProdWarp0) {
+        if (warp == kAckWarp) {
+            // nothing to do in this CTA
+        } else if (warp >= kProdWarp0) {
             producer<true>(p, sy, &q_map, ring, hd, consts);
         } else if (warp == kMmaWarp) {
             constexpr uint32_t idesc = idesc_f8(128, kBK, 0, 0);
@@ -860,7 +866,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else {
         // ======================= output CTA =======================
         uint8_t *ring = smem + kOutRing, *msgs = smem + kOutMsgs;
-        if (warp >= kProdWarp0) {
+        if (warp == kAckWarp) {  // messages that have arrived: their slots expect the next one, their staging is free
+            uint32_t pc = 0;
+            for (uint32_t k = 0;; ++k) {
+                int u;
+                if (!tq_read(p, sy, rank, k, u)) goto done;
+                if (u < 0) break;
+                const Item it = load_unit(p, u);
+                if (it.skip) continue;
+                for (int j = it.j0; j < it.j1; ++j, ++pc) {
+                    const uint32_t bar = smem_u32(&hd->p_full[pc % kSlots]);
+                    if (!wait_on(sy, bar, (pc / kSlots) & 1, true)) goto done;
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(bar, msg_bytes);
+                        mbar_arrive_remote(map_to_cta(smem_u32(&hd->p_sent[pc & 1]), 0));
+                    }
+                    __syncwarp();
+                }
+            }
+        } else if (warp >= kProdWarp0) {
             producer<false>(p, sy, nullptr, ring, hd, nullptr);
         } else if (warp == kMmaWarp) {
             constexpr uint32_t idesc = idesc_f8(128, 256, 1, 0), idesc5 = idesc_f8(128, 256, 1, 1);
@@ -943,10 +967,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const bool rescale = j > it.j0 && some_alpha(msg);
                     fin = stat.y;
                     if (g == (int)(pc & 1)) {  // this warp's tile: its 32 heads' weights into codes
-                        if (threadIdx.x == g * 128) {
-                            mbar_arrive_expect_tx(smem_u32(&hd->p_full[ps]), msg_bytes);  // the next message
-                            mbar_arrive_remote(map_to_cta(smem_u32(&hd->p_sent[g]), 0));
-                        }
                         if ((warp & 3) < quads) {
                             // 32 keys at a time, hi and mid in the place of their weights (short code: one stretch for all 96
                             // keys takes 0.8 % more of a prefill's time)
