@@ -238,6 +238,8 @@ def sharedkv_cache_append(
     if cache.dim() != 4 or cache.shape[2] != 1:
         raise ValueError(f"cache must be [blocks, block_size, 1, D] (got {tuple(cache.shape)})")
     blocks, _, _, D = cache.shape
+    if D % 16 or D > 1024:
+        raise ValueError(f"the head dim must be a multiple of 16 up to 1024 (got {D})")
     rows = kv.shape
     lead = 1 if layout_q == "TND" else 2
     if len(rows) not in (lead + 1, lead + 2) or rows[-1] != D or (len(rows) == lead + 2 and rows[lead] != 1):

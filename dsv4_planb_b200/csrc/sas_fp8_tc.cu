@@ -50,17 +50,20 @@
 //     would take 2 % more time), and O is rescaled 256 columns at a time, each as soon as the last tile's
 //     product of these columns is complete.
 //
-// Whole calls: 64 tokens of 2176 keys, 128 heads of 576 dims: 65 us (38.8 GFLOP, 98.6 MB); 2048 such
-// tokens: 1.07 ms, 930 TFLOP/s, and 1.21 ms once the card is at its power limit (1.7 GHz).  A tile takes
-// 2800 cycles: 1960 of QK issue, the rest mostly waits for an S to come back: the two passes of the softmax
-// are 1370 and 2140 cycles, so that QK and softmax of two tiles, which share an S buffer, take 5700, and a
-// third S has no room.  The gather warps are busy for 2650.  A unit adds 6500 cycles for the split of Q
+// Whole calls: 64 tokens of 2176 keys, 128 heads of 576 dims: 70 us (38.8 GFLOP, 98.6 MB); 2048 such
+// tokens: 1.14 ms, 870 TFLOP/s, and 1.32 ms once the card is at its power limit (1.7 GHz).  A tile takes
+// about 3000 cycles of a prefill (2800 with two terms per weight, where these were taken): 1960 of QK issue, the
+// rest mostly waits for an S to come back: the two passes of the softmax are 1370 and 2140 cycles, so that
+// QK and softmax of two tiles, which share an S buffer, take 5700, and a third S has no room.  The gather
+// warps are busy for 2650; the 18 products of the output CTA take 2700.  Left out for timing, of 1178 us: the
+// rescale of O 2 %, V's copies 2 %, both 3.5 %, then the third product nothing; the third product alone takes
+// 2 to 8 % of the decode steps.  A unit adds 6500 cycles for the split of Q
 // (conversions and byte shuffles at half and quarter rate), and the first tile 8 us of latency.  What did
 // not help: 6 gather warps, or a warp of its own for the row lookups (they take the softmax's issue slots,
 // 3 and 4 % slower); a tile taken in the last tile's frame and redone where that does not hold (some of 128
 // heads mostly rises, 20 %); TMEM loads a step ahead or of 32 columns (0 to 5 %: longer loops; the roles of an
-// SM share its instruction caches); a
-// staging of 8 boxes, or rows of 128 bytes, in the epilogue.
+// SM share its instruction caches); a staging of 8 boxes, or rows of 128 bytes, in the epilogue; the next
+// tile's weights split before the rescale (2 %); V's ring in halves of a tile (5 %).
 //
 // Keys of a token: first positions, then the window, then the compressed rows.  Slots without a key
 // carry weight 0 (log2 s = -inf); they and rows of unmapped blocks are filled with zeros.
@@ -710,7 +713,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t peer_msgs = map_to_cta(smem_u32(smem + kOutMsgs), 1), peer_full0 = map_to_cta(smem_u32(hd->p_full), 1);
             const float sink = head && p.sinks ? p.sinks[h] : -INFINITY;
             // a warp without heads: its rows of Q, S and P hold whatever lies there, and reach no other row (16 heads,
-            // 11 tiles: 33 us instead of 35 with all warps at work)
+            // 11 tiles: 6 % less time than with all warps at work)
             const bool idle = (warp & 3) >= quads;
             uint32_t sc0 = 0, qc = 0, lc = 0, mine = 0;  // the unit's first tile; units; units of two tiles or more; own tiles
             for (uint32_t k = 0;; ++k) {

@@ -14,11 +14,13 @@ using namespace sas_ptx;
 
 constexpr uint64_t kTimeoutNs = 4000000000ull;
 
-// Unit queue: the score CTA's producer warp 4 takes unit ids from a global counter (the next one
+// Unit queue: one warp of the score CTA, the writer, takes unit ids from a global counter (the next one
 // fetched while the current one runs) and publishes them to every role of both CTAs through a
-// kTq-entry ring; an entry is reused once all kTqReaders consumer warps have read it.
+// kTq-entry ring; an entry is reused once all reader warps have read it, whose number each kernel gives
+// its tq_empty barriers.
 constexpr int kTq = 8;
-constexpr uint32_t kTqReaders = 17;  // every warp of the cluster but the writer: 8 in the score CTA, 9 in the output CTA
+// Readers in the 16-bit kernel: every warp of its cluster but the writer, 8 in the score CTA, 9 in the output CTA.
+constexpr uint32_t kTqReaders = 17;
 
 // What the helpers below need of a kernel's shared header: its abort flag and its unit queue
 // (each kernel lays these out in a header struct of its own).
@@ -102,7 +104,7 @@ __device__ __forceinline__ bool tq_read(const P &p, const Sync &sy, uint32_t ran
     return true;
 }
 
-// Writer side (score CTA, warp 4; warp-uniform).  `pend` (lane 0) holds the id taken while the
+// Writer side (one warp of the score CTA; warp-uniform).  `pend` (lane 0) holds the id taken while the
 // previous unit's last tiles were being gathered (-1: none yet, take one now); taking it only
 // then keeps a cluster from holding a unit it cannot start soon.
 template <class P>

@@ -64,3 +64,12 @@ def test_value_dims(D, Dv, text):
             sparse_attn_sharedkv_fp8(empty(3, 8, D, dtype=torch.bfloat16), ori_kv=empty(4, 128, 1, D, dtype=F8), ori_kv_scale=empty(4),
                                      ori_block_table=empty(1, 4, dtype=i32), cu_seqlens_q=empty(2, dtype=i32), seqused_kv=empty(1, dtype=i32),
                                      softmax_scale=1.0, v_head_dim=Dv)
+
+
+@pytest.mark.parametrize("D", [568, 1040])
+def test_append_dims(D):
+    with FakeTensorMode():
+        a = append_call(F8)
+        a.update(cache=empty(4, 128, 1, D, dtype=F8), q=None, rope_table=None)
+        with pytest.raises(ValueError, match="multiple of 16 up to 1024"):
+            sharedkv_cache_append(empty(3, D, dtype=torch.bfloat16), **a)
