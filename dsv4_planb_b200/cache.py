@@ -100,7 +100,7 @@ def _rows2d(kv: torch.Tensor, T: int, D: int) -> torch.Tensor:
 
 def _rows_meet(rows: torch.Tensor, T: int, D: int, at: int, size: int) -> bool:
     """Whether some of the T rows of D 16-bit elements lie within ``size`` bytes from address ``at`` on."""
-    row, step = rows.data_ptr(), 2 * rows.stride(0)
+    row, step = rows.data_ptr(), 2 * rows.stride(0) if T > 1 else 2 * D  # one row may have any stride, 0 too
     if not size or row >= at + size or row + (T - 1) * step + 2 * D <= at:
         return False
     first = max((at - row - 2 * D) // step + 1, 0)  # the first row that ends behind the address

@@ -308,7 +308,7 @@ int sas_noalloc_read_status(uint32_t *status, void *stream);
  *   kv           [T][kv_row_stride] dtype: head_dim elements of each row are read
  *   q, q_out     [T][num_heads][head_dim] dtype, or NULL (num_heads 0): query heads,
  *                rotated by the same angles; q_out may be q (then only the rotated
- *                dims are written)
+ *                dims are written), and shares nothing with kv
  *   rope_table   [rope_rows][rope_dim] fp32: cos of the rope_dim / 2 angles, then sin
  *   block_table  [B][table_len] int32
  *   cu_seqlens_q [B + 1] int32, or NULL: then request b's rows start at b * max_q_len

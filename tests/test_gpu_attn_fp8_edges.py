@@ -43,6 +43,15 @@ def test_long_index_rows(cuda_device, K, kernel):
         assert torch.equal(again[0], out) and torch.equal(again[1], lse)
 
 
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_long_index_rows_in_pieces(cuda_device, kernel):
+    """Few tokens, which run in pieces: the pieces behind an early stop are empty."""
+    m = make([3, 2], [21000, 30000], N1=40, K=5000, seed=45)
+    for t, s in enumerate((0, 5, 2048, 4096)):
+        m["idx"][t, 0, s] = -1
+    check(m, *run(m, kernel=kernel, check_status=True))
+
+
 def far_rise(tokens, N1, rise, seed):
     """Every head's scores lie near 0 except for one late key, which all heads meet at about ``rise`` nats."""
     m = make([1] * tokens, [900] * tokens, N1=N1, scenario=1, win_left=799, seed=seed)

@@ -68,6 +68,12 @@ def test_queries_beside_rows_in_one_buffer(cuda_device):
             run(m, rope, kv=kv, q=buf, q_out=buf)
         with pytest.raises(ValueError, match="nothing with kv"):
             run(m, rope, kv=kv, q=m["q"].cuda(), q_out=buf)
+    one = make([1], [9], heads=4, seed=65)
+    buf = torch.zeros((1, 4, 576), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="nothing with kv"):
+        run(one, rope, kv=buf[0, 2].expand(1, 576), q=buf, q_out=buf)
+    row = one["kv"][0].cuda().expand(1, 576)
+    check(one, *run(one, rope, kv=row, q=buf, q_out=buf, check_status=True)[:2], rope)
     gaps = torch.zeros((5, 40 * 576), dtype=torch.bfloat16, device="cuda")  # q_out between two rows
     gaps[:, :576] = m["kv"].cuda()
     out = gaps[1, 576:21 * 576].view(5, 4, 576)
